@@ -391,6 +391,75 @@ int pgn_add_layernorm_cb(const void* x, const void* residual, void* sum_out, voi
  */
 int pgn_image_to_uint8(const void* x, int x_dtype, void* y, int N, int C, int H, int W, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * The token stage: drawing the visual tokens that the pixel decoder takes, one at a time, from a language model with
+ * an 8-bit paged cache of keys and values.  Stands in for what `llama.generate` does between two forward passes
+ * (called through lavit.generate_image_tokenids, Pigeon/inference.py:312-315,460-519; GenerationConfig :268-282).
+ *
+ * Cache of one layer, pages of page_size P tokens (16, 32, 64 or 128), head_dim D in {64, 128, 256}:
+ *   k_pages  e4m3 [num_pages, kv_heads, P, D]     k_scale  fp32 [num_pages, kv_heads]
+ *   v_pages  e4m3 [num_pages, kv_heads, D, P]     v_scale  fp32 [num_pages, kv_heads]
+ * key = k_scale * byte, value = v_scale * byte; scales are powers of two.  Pages 16-byte aligned.
+ * Requests: lens int32 [R] tokens held, table int32 [R, W] (row stride table_stride) pages in order; position p of
+ * request r is token p % P of page table[r][p / P], slot page * P + p % P.
+ *
+ * Page bookkeeping of a step, all on the device and in place.  keep (or NULL: all) says how many of its tokens each
+ * request keeps (clamped to [0, lens]; 0 ends it, fewer than lens rolls it back); pages behind them go back on the
+ * stack free_pages[0 .. free_count), so that popping returns them in request order.  add says how many tokens come
+ * (negative: 0); pages are popped for them, in request order, from the stack's end.
+ * A request is refused (status 1, it stays at its kept tokens, its slots are -1) when its tokens do not fit the table's
+ * row or end behind num_slots, or when it needs pages and the pages wanted up to and including it are more than there
+ * are: nobody who needs pages overtakes.  status int32 [R] is 0 otherwise.
+ * starts int32 [R+1]: where each request's new tokens begin (prefix sums of add, at most num_slots); slots int64
+ * [num_slots]: their slots, -1 behind the last.  lens becomes the tokens held after the step.  Table entries behind a
+ * request's pages are left as they were.  One workgroup and, above 8192 slots, a second launch for the slot map. */
+int pgn_page_advance(int32_t* lens, const int32_t* keep, const int32_t* add, int32_t* table, int64_t table_stride,
+                     int32_t* free_pages, int32_t* free_count, int num_pages, int R, int W, int page_size,
+                     int64_t num_slots, int64_t* slots, int32_t* starts, int32_t* status, void* stream);
+
+/* Stores keys and values k, v [num_tokens, kv_heads, D] (bf16 / f16, element strides of token and head, last dimension
+ * contiguous) at their slots.  Slots outside [0, num_pages * P) are left out.  Tokens of one page stand together in a
+ * call, with ascending slots, as pgn_page_advance lists them; a page that two separate stretches of tokens name ends
+ * with unspecified contents (that page only).
+ * Scale of a (page, head): the least power of two, 2^-100 at least, under which the largest finite new magnitude stays
+ * within 448; where the stretch begins behind token 0 of the page, the tokens before it stay valid: the scale does not
+ * fall, and if it grows they are rewritten under the new one (exact but for what falls under the smallest e4m3 step).
+ * Bytes round to nearest even; infinities and NaN become NaN.  Tokens of the page behind the stretch are not written,
+ * and count as free (their bytes keep their values, not their meaning, if the scale moves). */
+int pgn_cache_write(const void* k, const void* v, int dtype, const int64_t* slots, int64_t num_tokens, int kv_heads,
+                    int head_dim, int64_t k_st, int64_t k_sh, int64_t v_st, int64_t v_sh, void* k_pages, void* v_pages,
+                    float* k_scale, float* v_scale, int num_pages, int page_size, void* stream);
+
+/* Attention of new tokens over the cache: q, out [num_tokens, Hq, D] (bf16 / f16; q 16-byte aligned rows), Hq a multiple
+ * of Hkv (query head h reads KV head h / (Hq / Hkv)).  starts int32 [R+1]: request r owns tokens starts[r] ..
+ * starts[r+1); NULL: one token a request, num_tokens == R.  A request's n tokens are the last n of its lens positions.
+ * causal: a token sees the keys up to its own position, with window > 0 the last `window` of those; causal 0: every key
+ * of its request (window must be 0).  A row that sees no key is zero.  Rows of no request (behind starts[R]) are left as
+ * they were.  Table entries that name no page hide their keys.  Keys that a row does not see do not reach it, whatever
+ * their bytes hold.  workspace: pgn_cached_attention_workspace_bytes bytes, 16-byte aligned, contents irrelevant. */
+size_t pgn_cached_attention_workspace_bytes(int num_tokens, int R, int packed, int Hq, int Hkv, int head_dim, int W,
+                                            int page_size);
+int pgn_cached_attention(const void* q, int dtype, const void* k_pages, const void* v_pages, const float* k_scale,
+                         const float* v_scale, const int32_t* table, int64_t table_stride, const int32_t* lens,
+                         const int32_t* starts, void* out, int num_tokens, int R, int Hq, int Hkv, int head_dim,
+                         int num_pages, int W, int page_size, int64_t q_st, int64_t q_sh, int64_t o_st, int64_t o_sh,
+                         float scale, int causal, int window, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Draws one id a row from logits [B, V] (fp32 / bf16 / f16, row stride in elements, V <= PGN_SAMPLE_MAX_IDS) with the
+ * random numbers u [B] in [0, 1).  temperature, top_k, top_p, min_p: device arrays [B], or NULL for one value for all.
+ *   ids rank by (logit descending, index ascending); NaN logits count as -inf, and -inf is never drawn
+ *   top_k >= 1 keeps the first top_k ids; w_i = exp((x_i - max) / temperature)
+ *   top_p < 1 keeps the shortest run of first ids whose weight reaches top_p of all that top_k kept (one at least)
+ *   min_p keeps the ids with w_i >= min_p (of the largest weight, 1)
+ *   the id drawn is the first, in index order, whose running sum of kept weights exceeds u times their sum
+ * temperature <= 0 or NaN takes the first id in rank; a row without any logit above -inf gives -1.  Weights are computed
+ * in 64 bits and summed as integers of 2^-45: the same ids every time. */
+#define PGN_SAMPLE_MAX_IDS 262144
+int pgn_sample_tokens(const void* logits, int dtype, int64_t stride, int B, int V, const float* u,
+                      const float* temperature, float temperature_all, const int32_t* top_k, int top_k_all,
+                      const float* top_p, float top_p_all, const float* min_p, float min_p_all, int64_t* ids,
+                      void* stream);
+
 #ifdef __cplusplus
 }
 #endif

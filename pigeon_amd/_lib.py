@@ -52,6 +52,12 @@ SIGNATURES = {
     "pgn_attention_kernel_class": (_i, [_i, _i, _i, _i, _i, _i]),
     "pgn_attention_fwd": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i] + [_i64] * 12 + [_vp, _i64, _f, _vp]),
     "pgn_attention_causal_fwd": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i] + [_i64] * 12 + [_f, _vp]),
+    "pgn_page_advance": (_i, [_vp, _vp, _vp, _vp, _i64, _vp, _vp, _i, _i, _i, _i, _i64, _vp, _vp, _vp, _vp]),
+    "pgn_cache_write": (_i, [_vp, _vp, _i, _vp, _i64, _i, _i] + [_i64] * 4 + [_vp] * 4 + [_i, _i, _vp]),
+    "pgn_cached_attention_workspace_bytes": (_c.c_size_t, [_i] * 8),
+    "pgn_cached_attention": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp] + [_i] * 8 + [_i64] * 4 +
+                             [_f, _i, _i, _vp, _c.c_size_t, _vp]),
+    "pgn_sample_tokens": (_i, [_vp, _i, _i64, _i, _i, _vp, _vp, _f, _vp, _i, _vp, _f, _vp, _f, _vp, _vp]),
 }
 
 _lib = None

@@ -744,3 +744,189 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: int, sca
         kind = "attention"
     _launch(kind, work, run)
     return out
+
+
+# ------------------------------------------------------------------------------------------------
+# The token stage: block tables, 8-bit paged cache, attention over it, sampling.  Page layout: include/pigeon_hip.h.
+
+def _on(*ts):
+    """All tensors on one device: returns it, with the stream that the caller works on there."""
+    dev = ts[0].device
+    for t in ts:
+        if t is not None and t.device != dev:
+            _dev(t)
+            raise ValueError(f"pigeon_amd: tensors on {dev} and {t.device} in one call")
+    _dev(ts[0])
+    return dev
+
+
+def _call(dev, what, fn, *args):
+    """fn(*args, stream) on `dev`, which need not be the current device."""
+    if dev.index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if rc:
+        _lib.check(rc, what)
+
+
+def _i32(t: torch.Tensor, shape, name: str):
+    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of shape {tuple(shape)}")
+
+
+def _check_pages(k_pages, v_pages, k_scale, v_scale):
+    """(num_pages, kv_heads, page_size, head_dim) of one layer's cache."""
+    if k_pages.dim() != 4 or k_pages.dtype != torch.float8_e4m3fn or v_pages.dtype != torch.float8_e4m3fn:
+        raise TypeError("k_pages / v_pages must be float8_e4m3fn [num_pages, kv_heads, page_size, head_dim] / "
+                        "[num_pages, kv_heads, head_dim, page_size]")
+    N, H, P, D = k_pages.shape
+    if v_pages.shape != (N, H, D, P):
+        raise ValueError("v_pages must be [num_pages, kv_heads, head_dim, page_size] (values lie transposed)")
+    if k_scale.shape != (N, H) or v_scale.shape != (N, H) or k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
+        raise ValueError("k_scale / v_scale must be fp32 [num_pages, kv_heads]")
+    if not (k_pages.is_contiguous() and v_pages.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
+        raise ValueError("cache tensors must be contiguous")
+    return N, H, P, D
+
+
+def page_advance(lens: torch.Tensor, add: torch.Tensor, table: torch.Tensor, free_pages: torch.Tensor,
+                 free_count: torch.Tensor, page_size: int, num_slots: int, keep: Optional[torch.Tensor] = None):
+    """One step of the block tables (pgn_page_advance), in place on lens [R], table [R, W], the stack of free pages
+    free_pages [num_pages] and its height free_count [1], all int32.  `keep` [R]: tokens that each request keeps of those
+    it holds (None: all); `add` [R]: tokens that it gets.  num_slots: length of the slot map, sum(add) or more.
+    Returns dict(slots int64 [num_slots], starts int32 [R + 1], status int32 [R]: 1 where a request was refused).
+    No host sync."""
+    lib = _lib.load()
+    dev = _on(lens, add, table, free_pages, free_count, keep)
+    R = lens.numel()
+    if table.dim() != 2 or table.dtype != torch.int32 or table.shape[0] != R or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError("table must be int32 [R, W] with contiguous rows")
+    _i32(lens, (R,), "lens")
+    _i32(add, (R,), "add")
+    _i32(free_pages, (free_pages.numel(),), "free_pages")
+    _i32(free_count, (1,), "free_count")
+    if keep is not None:
+        _i32(keep, (R,), "keep")
+    W = table.shape[1]
+    if R > 1 and table.stride(0) < W:
+        raise ValueError("the rows of table overlap")
+    slots = torch.empty(num_slots, dtype=torch.int64, device=dev)
+    both = torch.empty(2 * R + 1, dtype=torch.int32, device=dev)
+    starts, status = both[:R + 1], both[R + 1:]
+
+    def run():
+        _call(dev, "pgn_page_advance", lib.pgn_page_advance, lens.data_ptr(), _ptr(keep), add.data_ptr(), table.data_ptr(),
+              table.stride(0) if R > 1 else W, free_pages.data_ptr(), free_count.data_ptr(), free_pages.numel(), R, W,
+              page_size, num_slots, slots.data_ptr(), starts.data_ptr(), status.data_ptr())
+
+    _launch("page_advance", 8.0 * num_slots, run)
+    return {"slots": slots, "starts": starts, "status": status}
+
+
+def cache_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                k_scale: torch.Tensor, v_scale: torch.Tensor) -> None:
+    """Stores k, v [T, kv_heads, head_dim] (bf16 / fp16, any strides with a contiguous last dim) at slots int64 [T] of one
+    layer's cache, in e4m3 with a power-of-two scale per page and head (pgn_cache_write).  Slots below 0 are left out."""
+    lib = _lib.load()
+    dev = _on(k, v, slots, k_pages, v_pages, k_scale, v_scale)
+    N, H, P, D = _check_pages(k_pages, v_pages, k_scale, v_scale)
+    if k.dim() != 3 or k.shape[1:] != (H, D) or v.shape != k.shape or v.dtype != k.dtype:
+        raise ValueError("cache_write: k and v must be [T, kv_heads, head_dim] and share a dtype")
+    T = k.shape[0]
+    if slots.dtype != torch.int64 or slots.shape != (T,) or not slots.is_contiguous():
+        raise ValueError("cache_write: slots must be a contiguous int64 [T]")
+    if T == 0:
+        return
+    k, v = (t if t.stride(2) == 1 else t.contiguous() for t in (k, v))
+
+    def run():
+        _call(dev, "pgn_cache_write", lib.pgn_cache_write, k.data_ptr(), v.data_ptr(), _dt(k), slots.data_ptr(), T, H, D,
+              k.stride(0), k.stride(1), v.stride(0), v.stride(1), k_pages.data_ptr(), v_pages.data_ptr(),
+              k_scale.data_ptr(), v_scale.data_ptr(), N, P)
+
+    _launch("cache_write", 6.0 * T * H * D, run)
+
+
+def cached_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale: torch.Tensor,
+                     v_scale: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
+                     starts: Optional[torch.Tensor] = None, scale: Optional[float] = None, causal: bool = True,
+                     window: int = 0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of q [T, heads, head_dim] (bf16 / fp16) over the 8-bit paged cache (pgn_cached_attention).
+
+    starts int32 [R + 1]: request r owns tokens starts[r] .. starts[r + 1), the last of the lens[r] that it holds, itself
+    among them; None: one token a request.  causal: a token sees keys up to its own position, the last `window` of them
+    if window > 0.  A row that sees nothing is zero.  Rows behind starts[R] are not written: they keep what `out` held,
+    or stay unset in the tensor made here.  Returns [T, heads, head_dim]."""
+    lib = _lib.load()
+    dev = _on(q, k_pages, v_pages, k_scale, v_scale, table, lens, starts, out)
+    N, H, P, D = _check_pages(k_pages, v_pages, k_scale, v_scale)
+    if q.dim() != 3 or q.shape[2] != D or q.shape[1] % H:
+        raise ValueError("cached_attention: q must be [T, heads, head_dim] with heads a multiple of kv_heads")
+    T, Hq, _ = q.shape
+    R = lens.numel()
+    _i32(lens, (R,), "lens")
+    if table.dim() != 2 or table.dtype != torch.int32 or table.shape[0] != R or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError("table must be int32 [R, W] with contiguous rows")
+    W = table.shape[1]
+    if starts is not None:
+        _i32(starts, (R + 1,), "starts")
+    elif T != R:
+        raise ValueError("cached_attention: without starts, q holds one token a request")
+    if out is None:
+        out = torch.empty(T, Hq, D, dtype=q.dtype, device=dev)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
+        raise ValueError("cached_attention: out must match q, with a contiguous last dim")
+    if T == 0:
+        return out
+    if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
+        q = q.contiguous()                                     # rows are read 16 bytes at a time
+        if q.data_ptr() % 16:
+            q = q.clone()
+    packed = starts is not None
+    nbytes = lib.pgn_cached_attention_workspace_bytes(T, R, packed, Hq, H, D, W, P)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    scale = float(D) ** -0.5 if scale is None else float(scale)
+
+    def run():
+        _call(dev, "pgn_cached_attention", lib.pgn_cached_attention, q.data_ptr(), _dt(q), k_pages.data_ptr(),
+              v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), table.data_ptr(),
+              table.stride(0) if R > 1 else W, lens.data_ptr(), _ptr(starts), out.data_ptr(), T, R, Hq, H, D, N, W, P,
+              q.stride(0), q.stride(1), out.stride(0), out.stride(1), scale, int(causal), int(window), _ptr(ws), nbytes)
+
+    _launch("cached_attention", 4.0 * T * Hq * D, run)
+    return out
+
+
+def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0,
+                  min_p=0.0) -> torch.Tensor:
+    """Draws an id for each row of logits [B, V] (fp32 / bf16 / fp16) with the random numbers uniform fp32 [B] in [0, 1)
+    (pgn_sample_tokens).  temperature, top_p, min_p: a number, or fp32 [B]; top_k: a number, or int32 [B].  Off: top_k
+    0, top_p 1, min_p 0.  temperature 0 takes the largest logit.  Returns int64 [B]; -1 for a row that is -inf
+    throughout.  The ids of one row feed `token_gather` as they are."""
+    lib = _lib.load()
+    if logits.dim() != 2:
+        raise ValueError("sample_tokens expects logits [B, V]")
+    B, V = logits.shape
+    tensors = [x if isinstance(x, torch.Tensor) else None for x in (temperature, top_k, top_p, min_p)]
+    dev = _on(logits, uniform, *tensors)
+    for t, dt, name in zip([uniform] + tensors, (torch.float32, torch.float32, torch.int32, torch.float32, torch.float32),
+                           ("uniform", "temperature", "top_k", "top_p", "min_p")):
+        if t is not None and (t.dtype != dt or t.shape != (B,) or not t.is_contiguous()):
+            raise ValueError(f"sample_tokens: {name} must be a contiguous {dt} tensor of shape [B]")
+    ids = torch.empty(B, dtype=torch.int64, device=dev)
+    if B == 0:
+        return ids
+    if logits.stride(1) != 1 and V > 1:
+        logits = logits.contiguous()
+    tt, kt, pt, mt = tensors
+
+    def run():
+        _call(dev, "pgn_sample_tokens", lib.pgn_sample_tokens, logits.data_ptr(), _dt(logits),
+              logits.stride(0) if B > 1 else V, B, V, uniform.data_ptr(), _ptr(tt), 0.0 if tt is not None else temperature,
+              _ptr(kt), 0 if kt is not None else top_k, _ptr(pt), 0.0 if pt is not None else top_p, _ptr(mt),
+              0.0 if mt is not None else min_p, ids.data_ptr())
+
+    _launch("sample", float(B * V * logits.element_size()), run)
+    return ids

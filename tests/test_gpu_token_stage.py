@@ -1,0 +1,734 @@
+"""The token stage's operators on the GPU against oracle/token_stage_ref.py: block tables, 8-bit paged cache, attention
+over it, sampling, and a run of them as a decoding loop uses them."""
+import math
+import random
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import token_stage_ref as ref
+from pigeon_amd import ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+F8 = torch.float8_e4m3fn
+
+
+def i32(v):
+    return torch.tensor(v, dtype=torch.int32, device=DEV)
+
+
+# ------------------------------------------------------------------------------------------------ page_advance
+def _pages_state(R, W, N, seed, held_max):
+    r = random.Random(seed)
+    P = r.choice([16, 32, 64, 128])
+    pool = list(range(N))
+    r.shuffle(pool)
+    table, lens = [[-7] * W for _ in range(R)], []
+    for row in table:
+        h = r.randint(0, min(held_max, W * P))
+        if -(-h // P) > len(pool) - 1:
+            h = 0
+        for j in range(-(-h // P)):
+            row[j] = pool.pop()
+        lens.append(h)
+    return P, lens, table, pool + [-9] * (N - len(pool)), len(pool), r
+
+
+@pytest.mark.parametrize("R,W,N,held,add,steps", [
+    (1, 1, 1, 16, 16, 4), (3, 4, 9, 60, 30, 6), (64, 8, 300, 100, 1, 5), (17, 40, 200, 500, 200, 5),
+    (1024, 3, 2000, 40, 20, 2), (1025, 3, 2000, 40, 20, 2), (2500, 4, 5000, 60, 30, 2), (5, 300, 1500, 4000, 9000, 3)])
+def test_page_advance_against_the_list_form(R, W, N, held, add, steps):
+    P, lens, table, free, count, r = _pages_state(R, W, N, R * 31 + W, held)
+    dl, dt, df, dc = i32(lens), torch.full((R, W + 3), 5, dtype=torch.int32, device=DEV), i32(free), i32([count])
+    dt[:, :W] = i32(table)
+    for step in range(steps):
+        adds = [r.choice([0, r.randint(0, add), 1]) for _ in range(R)]
+        keep = None if step % 3 == 2 else [r.choice([h, h, 0, r.randint(0, h), h + 5]) for h in lens]
+        T = sum(adds) + r.choice([0, 0, 7, -min(3, sum(adds))])
+        if step == 1 and R > 2:
+            adds[R // 2] = -4                                     # counts as 0
+        lens, table, free, count, slots, starts, status = ref.page_advance_ref(lens, keep, adds, table, free, count, P, T)
+        got = ops.page_advance(dl, i32(adds), dt[:, :W], df, dc, P, T, keep=None if keep is None else i32(keep))
+        for name, a, b in (("lens", dl, lens), ("table", dt[:, :W], table), ("free", df, free), ("count", dc, [count]),
+                           ("slots", got["slots"], slots), ("starts", got["starts"], starts), ("status", got["status"], status)):
+            assert a.cpu().tolist() == b, (name, step)
+        assert bool((dt[:, W:] == 5).all())
+
+
+def test_page_advance_refuses_in_order_and_gives_pages_back():
+    # 3 free pages of 16: request 0 takes 2, request 1 wants 2 (refused), request 2 needs none, request 3 wants 1: behind
+    # a refused one, so refused; request 4's tokens do not fit its row
+    lens, table = i32([0, 0, 3, 0, 0]), torch.zeros(5, 2, dtype=torch.int32, device=DEV)
+    table[2, 0] = 6
+    free, count = i32([1, 2, 3, -1, -1, -1, -1, -1]), i32([3])
+    got = ops.page_advance(lens, i32([17, 32, 5, 1, 33]), table, free, count, 16, 88)
+    assert got["status"].tolist() == [0, 1, 0, 1, 1] and lens.tolist() == [17, 0, 8, 0, 0] and count.tolist() == [1]
+    assert table[0].tolist() == [3, 2] and got["starts"].tolist() == [0, 17, 49, 54, 55, 88]
+    s = got["slots"].tolist()
+    assert s[:17] == [48 + i for i in range(16)] + [32] and s[17:49] == [-1] * 32 and s[49:54] == [6 * 16 + 3 + i for i in range(5)]
+    assert s[54:] == [-1] * 34
+    # ending request 0 returns its pages so that the next taker gets them in the same order
+    got = ops.page_advance(lens, i32([0, 17, 0, 0, 0]), table, free, count, 16, 17, keep=i32([0, 9, 9, 9, 9]))
+    assert table[1].tolist() == [3, 2] and got["status"].tolist() == [0] * 5 and count.tolist() == [1]
+
+
+@pytest.mark.parametrize("T", [8191, 8192, 8193, 20001])
+def test_page_advance_slot_map_sizes(T):
+    R, P, W = 7, 16, 400
+    adds = [T // 7, 0, T // 7, 1, T // 3, 0, 0]
+    pages = sum(-(-a // P) for a in adds)
+    lens, table, free, count = [0] * R, [[0] * W for _ in range(R)], list(range(pages)), pages
+    dl, dt, df, dc = i32(lens), i32(table), i32(free), i32([count])
+    want = ref.page_advance_ref(lens, None, adds, table, free, count, P, T)
+    got = ops.page_advance(dl, i32(adds), dt, df, dc, P, T)
+    assert got["slots"].cpu().tolist() == want[4] and got["starts"].tolist() == want[5] and dl.tolist() == want[0]
+
+
+def test_page_advance_stays_inside_its_arrays_on_wrong_counts():
+    """A stack height, lengths and additions that cannot be: nothing outside the arrays is touched."""
+    R, W, N = 4, 2, 6
+    whole = torch.full((64,), -77, dtype=torch.int32, device=DEV)
+    lens, table, free, count = whole[0:4], whole[8:16].view(4, 2), whole[20:26], whole[30:31]
+    lens.copy_(i32([1 << 30, -5, 40, 2]))
+    table.copy_(i32([[0, 1], [2, 3], [4, 5], [900, -900]]))
+    free.copy_(i32([0] * N))
+    count.fill_(1 << 20)
+    got = ops.page_advance(lens, i32([2 ** 31 - 1, -3, 16, 30]), table, free, count, 16, 50, keep=i32([0, 3, -1, 99]))
+    torch.cuda.synchronize()
+    outside = torch.cat([whole[4:8], whole[16:20], whole[26:30], whole[31:]])
+    assert bool((outside == -77).all())
+    assert 0 <= int(count) <= N and got["starts"].tolist()[0] == 0 and max(got["starts"].tolist()) <= 50
+    assert got["status"].tolist()[0] == 1                          # 2^31 - 1 tokens do not fit
+
+
+# ------------------------------------------------------------------------------------------------ cache_write
+def _cache(N, H, P, D, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    kp = (torch.randn(N, H, P, D, generator=g) * 60).clamp(-448, 448).to(F8)
+    vp = (torch.randn(N, H, D, P, generator=g) * 60).clamp(-448, 448).to(F8)
+    ks = torch.ldexp(torch.ones(N, H), torch.randint(-8, -4, (N, H), generator=g))
+    vs = torch.ldexp(torch.ones(N, H), torch.randint(-8, -4, (N, H), generator=g))
+    return [t.to(DEV) for t in (kp, vp, ks, vs)]
+
+
+def _same(a, b):
+    a, b = np.asarray(a), np.asarray(b)
+    return np.array_equal(np.isnan(a), np.isnan(b)) and np.array_equal(a[~np.isnan(a)], b[~np.isnan(b)])
+
+
+def _check_write(k, v, slots, cache):
+    """Runs the kernel and the oracle on copies; every byte value and scale of the whole cache has to be equal."""
+    kp, vp, ks, vs = cache
+    f64 = lambda t: t.cpu().float().double().numpy()               # noqa: E731
+    want_k = ref.cache_write_ref(f64(k), slots.cpu().tolist(), f64(kp), f64(ks))
+    want_v = ref.cache_write_ref(f64(v), slots.cpu().tolist(), f64(vp).swapaxes(2, 3), f64(vs))
+    ops.cache_write(k, v, slots, kp, vp, ks, vs)
+    assert _same(f64(ks), want_k[1]) and _same(f64(vs), want_v[1])
+    assert _same(f64(kp), want_k[0])
+    assert _same(f64(vp).swapaxes(2, 3), want_v[0])
+
+
+def _slots(runs, P):
+    return torch.tensor([page * P + row + i for page, row, n in runs for i in range(n)], dtype=torch.int64, device=DEV)
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("P", [16, 32, 64, 128])
+def test_cache_write_equals_the_oracle(P, D, dt):
+    H, N = 3, 12
+    # whole pages, one token at each end of a page, a run from the middle to the end and on into the next page, odd runs
+    runs = [(3, 0, P), (5, 0, 1), (1, P - 1, 1), (7, P // 2 + 1, P // 2 - 1), (2, 0, 5), (9, 3, 6), (11, 5, P - 6), (0, 1, 2)]
+    slots = _slots(runs, P)
+    g = torch.Generator().manual_seed(P + D)
+    x = torch.randn(2, len(slots), H, D, generator=g) * torch.tensor([0.01, 1.0, 300.0])[None, None, :, None]
+    x[:, ::3] *= 8                                                # some tokens make an old page's scale grow, others do not
+    k, v = x.to(dt).to(DEV)
+    _check_write(k, v, slots, _cache(N, H, P, D, seed=P))
+
+
+def test_cache_write_appends_token_by_token():
+    """A page filled one token at a time, magnitudes rising by 2^14 and falling: scales grow, older bytes shift."""
+    P, D, H = 16, 64, 2
+    cache = _cache(3, H, P, D)
+    g = torch.Generator().manual_seed(3)
+    for row in range(P):
+        size = 2.0 ** (row - 7 if row < 12 else 3 - row)
+        k, v = (torch.randn(2, 1, H, D, generator=g) * size).to(torch.bfloat16).to(DEV)
+        _check_write(k, v, _slots([(1, row, 1)], P), cache)
+    s = cache[2].cpu()
+    assert float(s[1, 0]) >= 2.0 ** -5                            # it did grow: 2^4-sized tokens
+
+
+def test_cache_write_values_without_an_e4m3_form():
+    P, D, H = 16, 64, 2
+    x = torch.zeros(4, H, D)
+    x[0, 0, :6] = torch.tensor([math.inf, -math.inf, math.nan, 1.0, -3.0, 0.0])     # the infinity does not set the scale
+    x[1, 1, :2] = torch.tensor([math.nan, math.inf])                                # nothing finite but zeros
+    x[2, 0, :4] = torch.tensor([1e-30, 3e38, -3e38, 2e-8])
+    x[3, 0, :3] = torch.tensor([1e-38, -1e-33, 5e-36])
+    for n in range(4):
+        k = x[n:n + 1].to(torch.bfloat16).to(DEV)
+        _check_write(k, k.flip(2).contiguous(), _slots([(n % 3, 0, 1)], P), _cache(3, H, P, D, seed=n))
+    k = x.to(torch.float16).to(DEV)
+    _check_write(k, k, _slots([(2, 4, 4)], P), _cache(3, H, P, D))
+
+
+def test_cache_write_scale_borders_and_ties():
+    """Largest magnitudes at, just under and just over 448 * 2^k, and values half way between two e4m3 steps."""
+    P, D, H = 16, 64, 1
+    for top in (448.0, 450.0, 446.0, 896.0, 1.0, 0.875, 0.87890625, 3.5):
+        x = torch.linspace(-1, 1, 4 * D).reshape(4, H, D) * top
+        x[0, 0, 0] = top
+        x[1, 0, :8] = top / 448 * torch.tensor([17.0, 19.0, 2.125, 0.0009765625, 0.0029296875, 0.0048828125, 1.0625, 1.1875])
+        k = x.to(torch.bfloat16).to(DEV)
+        _check_write(k, -k, _slots([(1, 0, 4)], P), _cache(2, H, P, D))
+
+
+@pytest.mark.parametrize("layout", ["fused", "odd", "broadcast", "transposed"])
+def test_cache_write_strides(layout):
+    P, D, H, T = 32, 128, 5, 40
+    g = torch.Generator().manual_seed(1)
+    if layout == "fused":                                         # [T, 3, H, D] projection
+        qkv = torch.randn(T, 3, H, D, generator=g).to(torch.bfloat16).to(DEV)
+        k, v = qkv[:, 1], qkv[:, 2]
+    elif layout == "odd":                                         # rows that start on 2 bytes
+        buf = torch.randn(T, H * (D + 3) + 1, generator=g).to(torch.bfloat16).to(DEV)
+        k = buf[:, 1:].view(T, H, D + 3)[:, :, 1:D + 1]
+        v = buf[:, 1:].view(T, H, D + 3)[:, :, 2:D + 2]
+    elif layout == "broadcast":                                   # one head's key for all: stride 0
+        k = torch.randn(T, 1, D, generator=g).to(torch.bfloat16).to(DEV).expand(T, H, D)
+        v = torch.randn(1, H, D, generator=g).to(torch.bfloat16).to(DEV).expand(T, H, D)
+    else:
+        k = torch.randn(T, D, H, generator=g).to(torch.bfloat16).to(DEV).transpose(1, 2)
+        v = torch.randn(H, T, D, generator=g).to(torch.bfloat16).to(DEV).transpose(0, 1)
+    _check_write(k, v, _slots([(2, 0, 32), (0, 20, 8)], P), _cache(4, H, P, D))
+
+
+def test_cache_write_leaves_out_slots_that_are_none():
+    P, D, H, N = 16, 64, 2, 3
+    slots = torch.tensor([-1, 5, 6, -1, -1, N * P, 1 << 40, -(1 << 40), 32, -1], dtype=torch.int64, device=DEV)
+    g = torch.Generator().manual_seed(1)
+    k, v = torch.randn(2, 10, H, D, generator=g).to(torch.float16).to(DEV)
+    _check_write(k, v, slots, _cache(N, H, P, D))
+
+
+@pytest.mark.parametrize("T", [2047, 2048, 2049, 5000])
+def test_cache_write_many_tokens(T):
+    """Both sizes of workgroup, runs that cross their borders, ragged requests on shuffled pages."""
+    P, D, H = 64, 64, 2
+    r = random.Random(T)
+    runs, left, pages = [], T, list(range(T // P + 200))
+    r.shuffle(pages)
+    while left:
+        row = r.choice([0, 0, 0, r.randrange(P)])
+        n = min(left, r.randint(1, P - row))
+        runs.append((pages.pop(), row, n))
+        left -= n
+    k, v = torch.randn(2, T, H, D, generator=torch.Generator().manual_seed(T)).to(torch.bfloat16).to(DEV)
+    _check_write(k, v, _slots(runs, P), _cache(T // P + 200, H, P, D))
+
+
+# ------------------------------------------------------------------------------------------------ cached_attention
+def _tolerance(dt, want, mag, big, D, keys):
+    """Half a step of the output's type on the result, half a step on each probability (they sum to at most mag), and the
+    fp32 arithmetic: a score of D products and a scaling is off by (D + 4) 2^-24 of its magnitude, which moves every
+    probability by that much relatively, numerator and denominator; sums over the keys are off by keys 2^-24, a few
+    roundings (exp2, rescaling) besides.  fp16 outputs under the normal range round to 2^-25 at worst."""
+    half = torch.finfo(dt).eps / 2
+    fp32 = 2 * (D + 4) * 2.0 ** -24 * big + (2 * keys + 64) * 2.0 ** -24
+    return half * want.abs() + (half + fp32) * mag + (2.0 ** -25 if dt == torch.float16 else 1e-37)
+
+
+def _check_attention(q, cache, table, lens, starts=None, rows=None, **kw):
+    got = ops.cached_attention(q, *cache, table, lens, starts=starts, **kw)
+    want, mag, big = ref.cached_attention_ref(q, *cache, table, lens, starts=starts, **kw)
+    err = (got.cpu().double() - want).abs()
+    tol = _tolerance(q.dtype, want, mag, big, q.shape[2], int(lens.max().clamp(min=1)))
+    rows = slice(None) if rows is None else rows
+    nan = want[rows].isnan()
+    assert torch.equal(nan, got.cpu()[rows].isnan())
+    bad = (err[rows] > tol[rows]) & ~nan
+    assert not bool(bad.any()), (int(bad.sum()), float(err[rows][bad].max()), bad.nonzero()[:5].tolist())
+    return got
+
+
+def _table(lens, P, N, seed=0, extra=1):
+    pool = list(range(N))
+    random.Random(seed).shuffle(pool)
+    W = max(1, max(-(-n // P) for n in lens)) + extra
+    rows = [[pool.pop() for _ in range(-(-max(n, 0) // P))] for n in lens]
+    return i32([r + [-1] * (W - len(r)) for r in rows])
+
+
+def _q(T, H, D, dt, seed=0):
+    return torch.randn(T, H, D, generator=torch.Generator().manual_seed(seed)).to(dt).to(DEV)
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("P", [16, 32, 64, 128])
+def test_decode_against_the_oracle(P, D, dt):
+    lens = [1, 0, 15, 16, 17, 63, 64, 65, 127, 128, 129, 255, 256, 257, 300]
+    cache = _cache(200, 2, P, D, seed=D)
+    got = _check_attention(_q(len(lens), 2, D, dt), cache, _table(lens, P, 200), i32(lens))
+    assert bool((got[1] == 0).all())                              # a request that holds nothing
+
+
+@pytest.mark.parametrize("Hq,Hkv", [(1, 1), (4, 4), (8, 2), (5, 1), (14, 2), (16, 1), (17, 1), (33, 1), (40, 8), (64, 1)])
+def test_decode_head_layouts(Hq, Hkv):
+    lens = [77, 3, 150]
+    _check_attention(_q(3, Hq, 64, torch.bfloat16), _cache(40, Hkv, 16, 64), _table(lens, 16, 40), i32(lens))
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Hq,Hkv,D", [(2, 2, 64), (4, 2, 128), (6, 2, 64), (3, 1, 256)])
+@pytest.mark.parametrize("new", [[5, 1, 33, 0, 64, 17], [1, 2, 1, 3, 1, 1], [100, 130, 70, 5, 64, 200]])
+@pytest.mark.parametrize("window", [0, 1, 20])
+def test_prompts_against_the_oracle(new, Hq, Hkv, D, dt, window):
+    lens = [n + h for n, h in zip(new, [0, 40, 7, 9, 64, 3])]
+    starts = i32(np.cumsum([0] + new).tolist())
+    cache = _cache(120, Hkv, 16, D, seed=1)
+    _check_attention(_q(sum(new), Hq, D, dt), cache, _table(lens, 16, 120), i32(lens), starts=starts, window=window)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("P", [32, 128])
+def test_prompts_without_a_mask_and_with_more_queries_than_keys(causal, P):
+    new, lens = [9, 4, 30, 6], [9, 50, 12, 0]                     # request 2: 18 queries lie before its first key
+    starts = i32(np.cumsum([0] + new).tolist())
+    got = _check_attention(_q(49, 4, 128, torch.float16), _cache(20, 4, P, 128), _table(lens, P, 20), i32(lens), starts=starts,
+                           causal=causal)
+    assert bool((got[43:] == 0).all()) and (not causal or bool((got[13:31] == 0).all()))
+
+
+def test_rows_of_no_request_keep_what_out_held():
+    new, lens = [3, 2], [40, 20]
+    q = _q(12, 4, 64, torch.bfloat16)
+    out = torch.full((12, 4, 64), 7.0, dtype=torch.bfloat16, device=DEV)
+    got = ops.cached_attention(q, *_cache(9, 2, 16, 64), _table(lens, 16, 9), i32(lens), starts=i32([2, 5, 7]), out=out)
+    assert got.data_ptr() == out.data_ptr()
+    assert bool((out[:2] == 7).all()) and bool((out[7:] == 7).all()) and not bool((out[2:7] == 7).any())
+    cache, table = _cache(9, 2, 16, 64), _table(lens, 16, 9)
+    _check_attention(q, cache, table, i32(lens), starts=i32([2, 5, 7]), rows=slice(2, 7))
+
+
+def test_strided_queries_and_output():
+    lens = [100, 31]
+    cache, table = _cache(12, 2, 16, 64), _table([100, 31], 16, 12)
+    qkv = torch.randn(2, 3, 4, 64, generator=torch.Generator().manual_seed(5)).to(torch.bfloat16).to(DEV)
+    want = _check_attention(qkv[:, 0].contiguous(), cache, table, i32(lens))
+    assert torch.equal(_check_attention(qkv[:, 0], cache, table, i32(lens)), want)
+    out = torch.zeros(2, 4, 100, dtype=torch.bfloat16, device=DEV)
+    ops.cached_attention(qkv[:, 0], *cache, table, i32(lens), out=out[:, :, 3:67])
+    assert torch.equal(out[:, :, 3:67], want) and not bool(out[:, :, :3].any()) and not bool(out[:, :, 67:].any())
+    odd = torch.empty(2 * 4 * 64 + 1, dtype=torch.bfloat16, device=DEV)[1:].view(2, 4, 64)     # 2-byte aligned
+    odd.copy_(qkv[:, 0])
+    assert torch.equal(ops.cached_attention(odd, *cache, table, i32(lens)), want)
+    wide = torch.full((2, 40), 3, dtype=torch.int32, device=DEV)                                # a wider table's rows
+    wide[:, :table.shape[1]] = table
+    assert torch.equal(ops.cached_attention(qkv[:, 0], *cache, wide[:, :table.shape[1]], i32(lens)), want)
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("new", [[1, 1, 1], [20, 90, 40]])
+def test_dead_cache_contents_do_not_reach_a_row(new, dt):
+    """Tokens behind a request, pages of others and pages that do not exist: NaN everywhere but in what is held."""
+    P, D, H = 32, 64, 2
+    lens = [33, 95, 64]
+    table = _table(lens, P, 12)
+    cache = _cache(12, H, P, D)
+    starts = i32(np.cumsum([0] + new).tolist())
+    q = _q(sum(new), 4, D, dt)
+    want = _check_attention(q, cache, table, i32(lens), starts=starts)
+    live = torch.zeros(12, P, dtype=torch.bool)
+    for r, L in enumerate(lens):
+        for p in range(L):
+            live[int(table[r, p // P]), p % P] = True
+    dead = ~live.to(DEV)
+    kp, vp, ks, vs = [t.clone() for t in cache]
+    kp.view(torch.uint8)[dead[:, None, :, None].expand(kp.shape)] = 0x7f
+    vp.view(torch.uint8)[dead[:, None, None, :].expand(vp.shape)] = 0xff
+    none = dead.all(1)
+    ks[none], vs[none] = math.nan, math.inf
+    for junk in (-1, 12, 2 ** 31 - 1, -2 ** 31):
+        t = torch.where(table < 0, junk, table)
+        assert torch.equal(ops.cached_attention(q, kp, vp, ks, vs, t, i32(lens), starts=starts), want)
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("window", [0, 9])
+def test_nan_values_reach_exactly_the_rows_that_see_them(window, dt):
+    new, lens = [60, 1, 90], [60, 80, 150]
+    P, D = 16, 64
+    table = _table(lens, P, 30)
+    kp, vp, ks, vs = _cache(30, 2, P, D)
+    for r, p in ((0, 30), (1, 40), (2, 140), (2, 77)):            # a NaN value at one head dim of one token
+        vp.view(torch.uint8)[int(table[r, p // P]), 1, 5, p % P] = 0x7f
+    kp.view(torch.uint8)[int(table[2, 100 // P]), 0, 100 % P, 9] = 0xff          # and a NaN key
+    starts = i32(np.cumsum([0] + new).tolist())
+    got = _check_attention(_q(151, 4, D, dt), (kp, vp, ks, vs), table, i32(lens), starts=starts, window=window)
+    assert bool(got.isnan().any()) and not bool(got[:30].isnan().any())
+
+
+def test_pages_that_are_none_hide_their_keys():
+    lens, P = [100, 64, 90], 16
+    table = _table(lens, P, 30)
+    for junk in (-1, 30, 2 ** 31 - 1):
+        t = table.clone()
+        t[0, 2], t[1, :4], t[2, 5] = junk, junk, junk
+        new = [30, 5, 1]
+        starts = i32(np.cumsum([0] + new).tolist())
+        got = _check_attention(_q(36, 2, 64, torch.bfloat16), _cache(30, 2, P, 64), t, i32(lens), starts=starts)
+        assert bool((got[30:35] == 0).all())                      # every page of request 1 is none
+
+
+def test_lengths_beyond_the_table_and_below_zero():
+    P = 16
+    table = _table([64, 64, 64], P, 12, extra=0)
+    _check_attention(_q(3, 2, 64, torch.bfloat16), _cache(12, 2, P, 64), table, i32([1 << 30, -5, 64]))
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_scales_far_apart(dt):
+    """Pages whose scales differ by up to 2^40, attended to one at a time by keys that dominate: the small pages' values
+    come out with their own precision."""
+    P, D, H, pages = 16, 64, 1, 8
+    kp, vp, ks, vs = _cache(pages, H, P, D)
+    ks.fill_(2.0 ** -6)
+    exps = [0, -30, 5, -12, -32, 8, -20, -25]
+    vs.copy_(torch.tensor([[2.0 ** e] for e in exps]))
+    kp.copy_(torch.zeros_like(kp, dtype=torch.float32).to(F8))
+    kf = torch.zeros(pages, H, P, D)
+    for n in range(pages):
+        kf[n, :, :, n] = 64.0                                     # key of page n: one at head dim n
+    kp.copy_(kf.to(F8).to(DEV))
+    table = i32([[3, 1, 4, 6, 0, 7, 2, 5]] * 8)
+    q = torch.zeros(8, 1, D)
+    for n in range(pages):
+        q[n, 0, n] = 900.0                                        # attends to page n alone
+    got = _check_attention(q.to(dt).to(DEV), (kp, vp, ks, vs), table, i32([128] * 8))
+    want, _, _ = ref.cached_attention_ref(q.to(dt).to(DEV), kp, vp, ks, vs, table, i32([128] * 8))
+    if dt == torch.bfloat16:                                      # relative to each page's own values
+        for n in range(pages):
+            assert float((got[n].cpu().double() - want[n]).norm() / want[n].norm()) < 2.0 ** -7
+    vs.zero_()                                                    # a cache of zeros
+    assert bool((ops.cached_attention(q.to(dt).to(DEV), kp, vp, ks, vs, table, i32([128] * 8)) == 0).all())
+
+
+def test_large_scores_keep_their_maximum():
+    lens = [200, 130]
+    cache = _cache(25, 2, 16, 64)
+    q = _q(2, 4, 64, torch.float16) * 40
+    _check_attention(q, cache, _table(lens, 16, 25), i32(lens), scale=1.0)
+    _check_attention(q, cache, _table(lens, 16, 25), i32(lens), scale=-0.5)
+
+
+@pytest.mark.parametrize("lens", [[5000], [9000, 70, 0, 2500]])
+def test_long_requests_are_split_and_joined(lens):
+    P = 64
+    _check_attention(_q(len(lens), 2, 64, torch.bfloat16), _cache(200, 1, P, 64), _table(lens, P, 200), i32(lens))
+
+
+def test_offsets_beyond_32_bits():
+    """A cache of 4.3 GB each for keys and values, the request on its last pages."""
+    H, P, D = 8, 128, 256
+    N = (1 << 32) // (H * P * D) + 40
+    kp = torch.zeros(N, H, P, D, dtype=torch.uint8, device=DEV).view(F8)
+    vp = torch.zeros(N, H, D, P, dtype=torch.uint8, device=DEV).view(F8)
+    ks, vs = torch.ones(N, H, device=DEV), torch.ones(N, H, device=DEV)
+    g = torch.Generator().manual_seed(0)
+    slots = torch.cat([torch.arange(P) + (N - 1) * P, torch.arange(20) + (N - 7) * P]).to(DEV)
+    k, v = torch.randn(2, P + 20, H, D, generator=g).to(torch.bfloat16).to(DEV)
+    ops.cache_write(k, v, slots, kp, vp, ks, vs)
+    assert float((kp[N - 1].float() * ks[N - 1][:, None, None] - k[:P].transpose(0, 1).float()).abs().max()) < 0.3
+    small = [t[N - 8:].clone() for t in (kp, vp, ks, vs)]
+    q = _q(1, 16, D, torch.bfloat16)
+    got = ops.cached_attention(q, kp, vp, ks, vs, i32([[N - 1, N - 7]]), i32([P + 20]))
+    want = _check_attention(q, small, i32([[7, 1]]), i32([P + 20]))
+    assert torch.equal(got, want)
+
+
+# ------------------------------------------------------------------------------------------------ sample_tokens
+def _check_sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    got = ops.sample_tokens(logits, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p).cpu().tolist()
+    x, un = logits.cpu().double().numpy(), u.cpu().double().numpy()
+    at = lambda v, b: v[b].item() if isinstance(v, torch.Tensor) else float(np.float32(v)) if isinstance(v, float) else v   # noqa: E731
+    want = [ref.sample_tokens_ref(x[b], un[b], at(temperature, b), at(top_k, b), at(top_p, b), at(min_p, b)) for b in range(len(x))]
+    assert got == want
+    return got
+
+
+def _logits(B, V, dt, seed=0, spread=2.0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(B, V, generator=g) * spread + 8 * torch.rand(B, V, generator=g).pow(30)
+    return x.to(dt).to(DEV), torch.rand(B, generator=g).to(DEV)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("V", [1, 2, 63, 64, 65, 1000, 1025, 5000, 48386, 131072, 262144])
+@pytest.mark.parametrize("filters", [(0, 1.0, 0.0), (50, 1.0, 0.0), (0, 0.9, 0.0), (0, 1.0, 0.05), (40, 0.8, 0.02), (700, 0.97, 0.0)])
+def test_sampling_against_the_oracle(V, dt, filters):
+    k, p, q = filters
+    x, u = _logits(6, V, dt, seed=V + k)
+    t = torch.tensor([1.0, 0.3, 0.7, 1.5, 3.0, 0.0], device=DEV)
+    _check_sample(x, u, temperature=t, top_k=k, top_p=p, min_p=q)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_sampling_ties_go_by_the_lowest_index(dt):
+    x = torch.zeros(9, 777, dtype=dt, device=DEV)
+    x[:, 500:] = 1.0
+    x[:, 3] = 1.0
+    x[:, 7] = -0.0
+    u = torch.linspace(0, 0.999, 9, device=DEV)
+    for k in (1, 2, 5, 278, 279, 500):
+        _check_sample(x, u, top_k=k)
+    for p in (0.1, 0.25, 0.5, 0.75, 0.9):
+        _check_sample(x, u, top_p=p, temperature=0.5)
+    assert _check_sample(x, u, temperature=0.0) == [3] * 9
+    flat = torch.zeros(9, 4096, dtype=dt, device=DEV)               # exact halves and quarters of equal weights
+    for p in (0.25, 0.5, 0.75):
+        _check_sample(flat, u, top_p=p)
+    _check_sample(flat, u, top_k=64, top_p=0.5)
+
+
+def test_sampling_masked_and_infinite_logits():
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(10, 500, generator=g)
+    x[0] = -math.inf                                                # nothing may be drawn
+    x[1] = math.nan
+    x[2, :] = -math.inf
+    x[2, 77] = -3.0                                                 # one id
+    x[3, 10:490] = -math.inf
+    x[4, 20] = x[4, 33] = math.inf                                  # only these two weigh anything
+    x[5, 5:] = torch.finfo(torch.float32).min                       # masks of the type's lowest value
+    x[6] = torch.finfo(torch.float32).min                           # all ids masked that way: equal logits
+    x[7, ::2] = math.nan
+    x[8, 5:] = -65504.0
+    x[9] = 3e38
+    x[9, 40] = -3e38
+    u = torch.linspace(0, 0.99, 10)[torch.randperm(10, generator=g)]
+    for kw in ({}, {"top_k": 5}, {"top_p": 0.6}, {"min_p": 0.3}, {"top_k": 300, "top_p": 0.9, "min_p": 0.01}, {"temperature": 0.0},
+               {"temperature": 1e-3}, {"temperature": math.inf, "top_p": 0.5}, {"top_k": 1}, {"top_p": 0.0}):
+        got = _check_sample(x.to(DEV), u.to(DEV), **kw)
+        assert got[0] == got[1] == -1 and got[2] == 77 and got[4] in (20, 33)
+    half = x.clone()
+    half[5, 5:] = torch.finfo(torch.bfloat16).min
+    _check_sample(half.to(torch.bfloat16).to(DEV), u.to(DEV), top_p=0.9, top_k=20)
+
+
+def test_sampling_borders_of_the_random_number():
+    x, _ = _logits(8, 300, torch.float32)
+    u = torch.tensor([0.0, 1.0 - 2.0 ** -24, 1.0, 2.0, -1.0, math.nan, math.inf, 0.5], device=DEV)
+    got = ops.sample_tokens(x, u).tolist()
+    assert got[0] == 0 and got[1] >= 298 and got[2] == got[3] == got[6] == 299 and got[4] == got[5] == 0
+    got = ops.sample_tokens(x, u, min_p=1.0).tolist()               # only the largest logit is left
+    assert got == x.argmax(1).tolist()
+    assert ops.sample_tokens(x, u, min_p=2.0).tolist() == got and ops.sample_tokens(x, u, temperature=-1.0).tolist() == got
+    assert ops.sample_tokens(x, u, temperature=math.nan).tolist() == got
+
+
+def test_sampling_rows_with_parameters_of_their_own():
+    x, u = _logits(64, 3000, torch.bfloat16, seed=4)
+    g = torch.Generator().manual_seed(9)
+    _check_sample(x, u, temperature=(torch.rand(64, generator=g) * 2).to(DEV), top_k=torch.randint(-1, 3500, (64,), generator=g, dtype=torch.int32).to(DEV),
+                  top_p=(torch.rand(64, generator=g) * 1.2).to(DEV), min_p=(torch.rand(64, generator=g) * 0.2).to(DEV))
+
+
+def test_sampling_strided_and_unaligned_rows():
+    x, u = _logits(5, 1003, torch.bfloat16)
+    want = _check_sample(x, u, top_p=0.95)
+    wide = torch.full((5, 1111), 99.0, dtype=torch.bfloat16, device=DEV)
+    wide[:, 7:1010] = x
+    assert ops.sample_tokens(wide[:, 7:1010], u, top_p=0.95).tolist() == want
+    assert ops.sample_tokens(x.t().contiguous().t(), u, top_p=0.95).tolist() == want
+    assert ops.sample_tokens(x[:1].expand(5, 1003), u, temperature=0.0).tolist() == [int(x[0].float().argmax())] * 5
+
+
+def test_sampling_follows_the_distribution():
+    """Frequencies of 40000 draws from one row: within six standard deviations of every probability."""
+    n = 40000
+    x = torch.tensor([2.0, 0.0, -1.0, 1.0, -math.inf, 1.5], device=DEV)
+    u = torch.rand(n, generator=torch.Generator().manual_seed(2)).to(DEV)
+    got = ops.sample_tokens(x.expand(n, 6), u, temperature=0.8)
+    p = torch.softmax(x.double().cpu() / 0.8, 0)
+    f = torch.bincount(got, minlength=6).cpu().double() / n
+    assert bool(((f - p).abs() <= 6 * (p * (1 - p) / n).sqrt()).all())
+
+
+# ------------------------------------------------------------------------------------------------ streams, graphs, a run
+def test_calls_on_another_stream():
+    lens = [90, 40]
+    cache, table, q = _cache(20, 2, 16, 64), _table([90, 40], 16, 20), _q(2, 4, 64, torch.bfloat16)
+    x, u = _logits(4, 5000, torch.float32)
+    want, ids = ops.cached_attention(q, *cache, table, i32(lens)), ops.sample_tokens(x, u, top_p=0.9)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        side.wait_stream(torch.cuda.default_stream())
+        got, ids2 = ops.cached_attention(q, *cache, table, i32(lens)), ops.sample_tokens(x, u, top_p=0.9)
+    side.synchronize()
+    assert torch.equal(got, want) and torch.equal(ids, ids2)
+
+
+class _Loop:
+    """A decoding loop without a model: keys, values, queries and logits are functions of the drawn ids."""
+
+    def __init__(self, R=3, V=500, seed=0):
+        g = torch.Generator().manual_seed(seed)
+        self.H, self.Hq, self.D, self.P, self.N, self.R, W = 2, 4, 64, 16, 40, R, 8
+        self.emb = (torch.randn(V, 2 * self.H + self.Hq, self.D, generator=g)).to(torch.bfloat16).to(DEV)
+        self.head = torch.randn(self.Hq * self.D, V, generator=g).to(torch.bfloat16).to(DEV)
+        self.cache = _cache(self.N, self.H, self.P, self.D)
+        self.lens, self.table = torch.zeros(R, dtype=torch.int32, device=DEV), torch.full((R, W), -1, dtype=torch.int32, device=DEV)
+        self.free, self.count = torch.arange(self.N, dtype=torch.int32, device=DEV), i32([self.N])
+        self.u = torch.rand(64, R, generator=g).to(DEV)
+        self.one = torch.ones(R, dtype=torch.int32, device=DEV)
+
+    def feed(self, ids, add, T, starts=True):
+        plan = ops.page_advance(self.lens, add, self.table, self.free, self.count, self.P, T)
+        x = self.emb[ids]
+        ops.cache_write(x[:, :self.H], x[:, self.H:2 * self.H], plan["slots"], *self.cache)
+        o = ops.cached_attention(x[:, 2 * self.H:], *self.cache, self.table, self.lens, starts=plan["starts"] if starts else None)
+        return o, plan
+
+    def draw(self, o, u):
+        logits = o.reshape(len(o), -1) @ self.head
+        return ops.sample_tokens(logits, u, temperature=0.7, top_k=100, top_p=0.95)
+
+
+def test_prompts_then_single_tokens_as_a_loop_uses_them():
+    """Prompts of different lengths, then 40 drawn tokens a request: every attention output against the oracle on the
+    cache as it stands, every slot and page accounted for, the ids taken by the token gather as they are."""
+    s = _Loop()
+    prompts = [5, 30, 1]
+    ids = torch.randint(0, 500, (36,), generator=torch.Generator().manual_seed(3)).to(DEV)
+    o, plan = s.feed(ids, i32(prompts), 36)
+    drawn = []
+    for step in range(40):
+        last = plan["starts"][1:].long() - 1
+        q = s.emb[ids][:, 2 * s.H:]
+        if step % 8 == 0:
+            want, mag, big = ref.cached_attention_ref(q, *s.cache, s.table, s.lens, starts=plan["starts"])
+            tol = _tolerance(torch.bfloat16, want, mag, big, s.D, 128)
+            assert bool(((o.cpu().double() - want).abs() <= tol).all())
+        ids = s.draw(o[last], s.u[step])
+        drawn.append(ids)
+        o, plan = s.feed(ids, s.one, s.R)
+    assert s.lens.tolist() == [45, 70, 41] and s.count.tolist() == [s.N - 3 - 5 - 3]
+    used = [int(p) for r in range(3) for p in s.table[r, :-(-int(s.lens[r]) // s.P)]]
+    assert len(set(used)) == len(used)
+    tokens = torch.stack(drawn, 1) + ops.LAVIT_ID_OFFSET            # drawn ids as codebook ids
+    e = ops.token_gather(tokens, torch.randn(500, 32, device=DEV), check=True)
+    assert e["token_nums"].tolist() == [40] * 3
+    again = _Loop()                                                 # the same inputs give the same ids
+    ids = torch.randint(0, 500, (36,), generator=torch.Generator().manual_seed(3)).to(DEV)
+    o, plan = again.feed(ids, i32(prompts), 36)
+    for step in range(40):
+        ids = again.draw(o[plan["starts"][1:].long() - 1], again.u[step])
+        assert torch.equal(ids, drawn[step])
+        o, plan = again.feed(ids, again.one, again.R)
+
+
+def test_a_captured_step_replays_like_the_eager_one():
+    """One decoding step as a graph, replayed between eager work; then a second graph of another size beside it."""
+    eager, graphed, other = _Loop(seed=1), _Loop(seed=1), _Loop(R=2, seed=2)
+    first = torch.tensor([4, 9, 2], device=DEV)
+    feeds = {}
+    for s, n in ((graphed, 3), (other, 2)):
+        ids, u = first[:n].clone(), s.u[0].clone()
+        saved = [t.clone() for t in (s.lens, s.table, s.free, s.count, *s.cache[:2], *s.cache[2:])]
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):                                # warm up outside the capture
+            side.wait_stream(torch.cuda.default_stream())
+            s.draw(s.feed(ids, s.one, n, starts=False)[0], u)
+        side.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = s.draw(s.feed(ids, s.one, n, starts=False)[0], u)
+        for t, was in zip((s.lens, s.table, s.free, s.count, *s.cache), saved):
+            t.view(torch.uint8).copy_(was.view(torch.uint8))
+        feeds[n] = (g, ids, u, out)
+    check = _Loop(R=2, seed=2)
+    ids3, ids2 = first.clone(), first[:2].clone()
+    for step in range(24):
+        want = eager.draw(eager.feed(ids3, eager.one, 3, starts=False)[0], eager.u[step])
+        g, ids, u, out = feeds[3]
+        ids.copy_(ids3)
+        u.copy_(eager.u[step])
+        g.replay()
+        want2 = check.draw(check.feed(ids2, check.one, 2, starts=False)[0], check.u[step])
+        g2, i2, u2, out2 = feeds[2]
+        i2.copy_(ids2)
+        u2.copy_(check.u[step])
+        g2.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(out2, want2), step
+        ids3, ids2 = want, want2
+    assert torch.equal(graphed.lens, eager.lens) and torch.equal(graphed.table, eager.table)
+    assert torch.equal(graphed.cache[0].view(torch.uint8), eager.cache[0].view(torch.uint8))
+    assert torch.equal(graphed.cache[1].view(torch.uint8), eager.cache[1].view(torch.uint8))
+
+
+def test_two_runs_give_the_same_bits():
+    lens = [3000, 700]
+    cache, table = _cache(60, 2, 64, 128), _table([3000, 700], 64, 60)
+    q = _q(2, 8, 128, torch.bfloat16)
+    assert torch.equal(ops.cached_attention(q, *cache, table, i32(lens)), ops.cached_attention(q, *cache, table, i32(lens)))
+    x, u = _logits(32, 48386, torch.bfloat16)
+    assert torch.equal(ops.sample_tokens(x, u, top_p=0.9), ops.sample_tokens(x, u, top_p=0.9))
+
+
+# ------------------------------------------------------------------------------------------------ refusals
+def test_wrong_arguments_are_refused():
+    cache, table, lens = _cache(4, 2, 16, 64), _table([20, 20], 16, 4, extra=0), i32([20, 20])
+    kp, vp, ks, vs = cache
+    q = _q(2, 4, 64, torch.bfloat16)
+    slots = torch.zeros(2, dtype=torch.int64, device=DEV)
+    k = _q(2, 2, 64, torch.bfloat16)
+    bad = [
+        (ValueError, lambda: ops.cached_attention(q[:, :3], *cache, table, lens)),
+        (ValueError, lambda: ops.cached_attention(q, *cache, table, i32([20]))),
+        (ValueError, lambda: ops.cached_attention(q[:1], *cache, table, lens)),
+        (ValueError, lambda: ops.cached_attention(q, *cache, table, lens, starts=i32([0, 2]))),
+        (ValueError, lambda: ops.cached_attention(q, *cache, table, lens.long())),
+        (ValueError, lambda: ops.cached_attention(q, *cache, table.long(), lens)),
+        (ValueError, lambda: ops.cached_attention(q, *cache, table, lens, window=-1)),
+        (ValueError, lambda: ops.cached_attention(q, *cache, table, lens, window=4, causal=False)),
+        (ValueError, lambda: ops.cached_attention(q, *cache, table, lens, scale=math.nan)),
+        (ValueError, lambda: ops.cached_attention(q, *cache, table, lens, out=q.float())),
+        (TypeError, lambda: ops.cached_attention(q.double(), *cache, table, lens)),
+        (NotImplementedError, lambda: ops.cached_attention(q.float(), *cache, table, lens)),
+        (TypeError, lambda: ops.cached_attention(q, kp.float(), vp, ks, vs, table, lens)),
+        (ValueError, lambda: ops.cached_attention(q, kp, kp, ks, vs, table, lens)),
+        (ValueError, lambda: ops.cached_attention(q, kp, vp, ks[:2], vs, table, lens)),
+        (RuntimeError, lambda: ops.cached_attention(q, *cache, table, lens.cpu())),
+        (NotImplementedError, lambda: ops.cached_attention(_q(2, 2, 80, torch.bfloat16), *_cache(4, 2, 16, 80), table, lens)),
+        (NotImplementedError, lambda: ops.cached_attention(q, *_cache(4, 2, 8, 64), table, lens)),
+        (ValueError, lambda: ops.cache_write(k, k[:1], slots, *cache)),
+        (ValueError, lambda: ops.cache_write(k, k, slots.int(), *cache)),
+        (ValueError, lambda: ops.cache_write(k[:, :1], k[:, :1], slots, *cache)),
+        (NotImplementedError, lambda: ops.cache_write(k.float(), k.float(), slots, *cache)),
+        (RuntimeError, lambda: ops.cache_write(k, k, slots.cpu(), *cache)),
+        (ValueError, lambda: ops.page_advance(lens, lens, table, i32([0]).long(), i32([0]), 16, 4)),
+        (ValueError, lambda: ops.page_advance(lens, i32([1]), table, i32([0]), i32([0]), 16, 4)),
+        (ValueError, lambda: ops.page_advance(lens, lens, table, i32([0]), i32([0, 0]), 16, 4)),
+        (NotImplementedError, lambda: ops.page_advance(lens, lens, table, i32([0]), i32([0]), 24, 4)),
+        (ValueError, lambda: ops.sample_tokens(q, torch.zeros(2, device=DEV))),
+        (ValueError, lambda: ops.sample_tokens(q[0], torch.zeros(3, device=DEV))),
+        (ValueError, lambda: ops.sample_tokens(q[0], torch.zeros(4, device=DEV), top_k=torch.zeros(4, device=DEV))),
+        (TypeError, lambda: ops.sample_tokens(q[0].double(), torch.zeros(4, device=DEV))),
+        (NotImplementedError, lambda: ops.sample_tokens(torch.zeros(1, 262145, device=DEV), torch.zeros(1, device=DEV))),
+        (RuntimeError, lambda: ops.sample_tokens(q[0].cpu(), torch.zeros(4))),
+    ]
+    for n, (kind, call) in enumerate(bad):
+        with pytest.raises(kind):
+            call()
+            pytest.fail(f"case {n} was not refused")
+    # nothing to do is no error
+    assert ops.cached_attention(q[:0], *cache, table, lens, starts=i32([0, 0, 0])).shape == (0, 4, 64)
+    ops.cache_write(k[:0], k[:0], slots[:0], *cache)
+    assert ops.sample_tokens(q[0][:0], torch.zeros(0, device=DEV)).shape == (0,)
