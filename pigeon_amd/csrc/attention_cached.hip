@@ -32,7 +32,10 @@ struct CachedArgs {
     float* part_o;
     float2* part_ml;
     int64_t table_stride, q_st, q_sh, o_st, o_sh;
-    int T, R, Hq, Hkv, G, W, shift, N, causal, window, split_keys, nsplit, tiles_per_request;
+    int T, R, Hq, Hkv, G, W, shift, N, causal, window;
+    int split_keys, nsplit, tiles_per_request;               // of the 16-row kernel
+    int big_split_keys, big_nsplit;                          // of the 128-row kernel
+    int out_vec;                                             // rows of `out` begin on 8 bytes
     float c;                                                 // scale * log2(e)
 };
 
@@ -49,6 +52,9 @@ struct Mat<PGN_BF16> {
     static __device__ __forceinline__ v2 cvt(unsigned w, float s) {
         return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, HI);
     }
+    static __device__ __forceinline__ f32x16_t mfma32(v8 a, v8 b, f32x16_t c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
     static __device__ __forceinline__ __bf16 one(float f) { return (__bf16)f; }
 };
 template <>
@@ -61,6 +67,9 @@ struct Mat<PGN_F16> {
     template <bool HI>
     static __device__ __forceinline__ v2 cvt(unsigned w, float s) {
         return __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, s, HI);
+    }
+    static __device__ __forceinline__ f32x16_t mfma32(v8 a, v8 b, f32x16_t c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
     }
     static __device__ __forceinline__ _Float16 one(float f) { return (_Float16)f; }
 };
@@ -90,41 +99,56 @@ __device__ __forceinline__ unsigned key_bytes(int first, int word, int lo, int h
     return m;
 }
 
-// The rows of a workgroup: `rows` consecutive (token, head-in-group) pairs of one request, ROWS to a tile.  Tile numbers
-// leave each request floor(start * G / ROWS) + r and up, which is room for its ceil(n * G / ROWS) tiles whatever the
-// lengths are, so the launch needs to know only the number of tokens and requests.
+// Requests of up to this many rows (a row: a token and a query head of the KV head's group) go to the 16-row kernel, the
+// others to the 128-row kernel, in one call if need be.
+#define PGN_CA_FEW_ROWS 64
+
+// The rows of a workgroup: consecutive rows of one request, ROWS to a tile.  16-row tiles: a fixed number for every
+// request.  128-row tiles leave each request the numbers floor(start * G / 128) + r and up, which is room for its
+// ceil(n * G / 128) tiles whatever the lengths are, so the launch needs to know only the number of tokens and requests.
 struct TileRows {
     int r, first, count, begin, n, len;                      // first row of the tile in its request, its valid rows
 };
 
-template <int ROWS>
-__device__ __forceinline__ bool find_tile(const CachedArgs& a, int tile, TileRows& t) {
-    int local;
+__device__ __forceinline__ bool request_rows(const CachedArgs& a, int r, TileRows& t) {
+    t.r = r;
     if (a.starts == nullptr) {
-        t.r = tile / a.tiles_per_request;
-        local = tile - t.r * a.tiles_per_request;
-        t.begin = t.r;
+        t.begin = r;
         t.n = 1;
     } else {
-        int lo = 0, hi = a.R;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if ((int64_t)a.starts[mid] * a.G / ROWS + mid <= tile) lo = mid;
-            else hi = mid;
-        }
-        t.r = lo;
-        t.begin = a.starts[lo];
-        const int end = a.starts[lo + 1];
+        t.begin = a.starts[r];
+        const int end = a.starts[r + 1];
         if (t.begin < 0 || end < t.begin || end > a.T) return false;
         t.n = end - t.begin;
-        local = tile - (int)((int64_t)t.begin * a.G / ROWS + lo);
     }
-    t.first = local * ROWS;
-    t.count = min(ROWS, t.n * a.G - t.first);
-    if (local < 0 || t.count <= 0) return false;
     const int64_t room = (int64_t)a.W << a.shift;
-    const int len = a.lens[t.r];
+    const int len = a.lens[r];
     t.len = len < 0 ? 0 : (len > room ? (int)room : len);
+    return true;
+}
+
+__device__ __forceinline__ bool few_rows_tile(const CachedArgs& a, int tile, TileRows& t) {
+    const int r = tile / a.tiles_per_request, local = tile - r * a.tiles_per_request;
+    if (!request_rows(a, r, t)) return false;
+    const int rows = t.n * a.G;
+    if (a.starts != nullptr && rows > PGN_CA_FEW_ROWS) return false;
+    t.first = local * 16;
+    t.count = min(16, rows - t.first);
+    return t.count > 0;
+}
+
+__device__ __forceinline__ bool many_rows_tile(const CachedArgs& a, int tile, TileRows& t) {
+    int lo = 0, hi = a.R;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if ((int64_t)a.starts[mid] * a.G / 128 + mid <= tile) lo = mid;
+        else hi = mid;
+    }
+    if (!request_rows(a, lo, t) || t.n * a.G <= PGN_CA_FEW_ROWS) return false;
+    const int64_t local = tile - ((int64_t)t.begin * a.G / 128 + lo);
+    if (local < 0 || local * 128 >= t.n * a.G) return false;
+    t.first = (int)local * 128;
+    t.count = min(128, t.n * a.G - t.first);
     return true;
 }
 
@@ -145,9 +169,9 @@ __global__ __launch_bounds__(PGN_CA_THREADS) void pgn_cached_rows16_kernel(const
     __shared__ float lds_m[4][16], lds_l[4][16];
     const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
     const int g = lane >> 4, col = lane & 15;
-    const int h = blockIdx.y, split = blockIdx.z;
+    const int h = blockIdx.x, split = blockIdx.z;
     TileRows t;
-    if (!find_tile<16>(a, blockIdx.x, t)) return;
+    if (!few_rows_tile(a, blockIdx.y, t)) return;
     int lo, hi;
     key_range(a, t, lo, hi);
     const int kb = (lo & ~63) + split * a.split_keys;
@@ -344,51 +368,401 @@ __global__ __launch_bounds__(PGN_CA_THREADS) void pgn_cached_rows16_kernel(const
     }
 }
 
-// Joins the splits of each row: the same tiles, one wave a row.
+// The kernel for prompts: 128 rows of a request, 32 to a wave, 64 keys at a time.
+//
+// What bounds it is arithmetic: the two products take as many matrix cycles as the softmax takes vector cycles (32 keys
+// and 16 rows a lane: scaling, exp2, sum, maximum and rounding of 32 numbers against 32 matrix instructions at head
+// dim 128), so the bytes are widened ONCE per workgroup, on their way into LDS, not in every wave.  Tiles of 16-bit keys
+// [64][D] and transposed values [D][64] are double buffered; while one is used, the next one's bytes are in flight
+// to registers.  Each wave fetches one 16-key chunk of a tile, which lies in one page.
+//
+// Keys are stored in the row order in which the 32x32 result hands its rows to lanes: row b + 4 h + 8 a of a half tile is
+// key 16 h + 4 a + b, so a lane ends up with 16 consecutive keys of its query and the probabilities are, without any
+// exchange, the second operand of O^T = V^T P^T.  16-byte units of a row are permuted by its low three bits, which
+// spreads the operand loads over the banks.
+// The running maximum moves only when it has to: probabilities may grow to 2^8 before the accumulator is rescaled.
 template <int DT, int D>
-__global__ __launch_bounds__(PGN_CA_THREADS) void pgn_cached_join_kernel(const CachedArgs a) {
-    constexpr int E = D / 64;
-    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, h = blockIdx.y;
+struct BigTile {
+    unsigned short k[64 * D];
+    unsigned short v[D * 64];
+};
+
+template <int DT, int D>
+struct BigLds {
+    BigTile<DT, D> tile[2];
+    float ks[2][4], raise[2][4], pscale[2][4], ref[2];
+    int nan[2][4], live[2][4];
+};
+
+template <int DT, int D>
+__global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void pgn_cached_rows128_kernel(const CachedArgs a) {
+    typedef typename Mat<DT>::v8 v8;
+    constexpr int L = D / 64, KS = D / 16, DTILES = D / 32, UNITS = D / 8;
+    extern __shared__ unsigned char smem_big[];
+    BigLds<DT, D>& s = *reinterpret_cast<BigLds<DT, D>*>(smem_big);
+    const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int hf = lane >> 5, col = lane & 31;
+    const int h = blockIdx.x, split = blockIdx.z;
     TileRows t;
-    if (!find_tile<16>(a, blockIdx.x, t)) return;
-    for (int rr = wid; rr < t.count; rr += 4) {
-        const int rw = t.first + rr, tok = t.begin + rw / a.G, hd = h * a.G + rw % a.G;
-        const int64_t row = (int64_t)tok * a.Hq + hd, step = (int64_t)a.T * a.Hq;
-        float big = -INFINITY;
-        for (int s = 0; s < a.nsplit; ++s) big = fmaxf(big, a.part_ml[s * step + row].x);
-        const float at = big == -INFINITY ? 0.f : big;
-        float den = 0.f, num[E] = {};
-        for (int s = 0; s < a.nsplit; ++s) {
-            const float2 ml = a.part_ml[s * step + row];
-            if (ml.x == -INFINITY && ml.y == 0.f) continue;  // nothing seen: its output was not written
-            const float f = __builtin_amdgcn_exp2f(ml.x - at);
-            den = fmaf(ml.y, f, den);
+    if (!many_rows_tile(a, gridDim.y - 1 - blockIdx.y, t)) return;      // the tiles with the most keys first
+    int lo, hi;
+    key_range(a, t, lo, hi);
+    const int kb = (lo & ~63) + split * a.big_split_keys;
+    const int kend = min(hi, kb + a.big_split_keys);
+
+    const int wrow = wid * 32;                               // first row of the wave in the tile
+    const int mine = min(wrow + col, t.count - 1);           // rows past the last repeat it and are not written
+    const int row = t.first + mine;
+    const int token = t.begin + row / a.G, head = h * a.G + row % a.G;
+    const int pos = t.len - t.n + row / a.G;
+    const int vis_hi = a.causal ? min(t.len, pos + 1) : t.len;
+    const int vis_lo = a.window ? max(0, pos - a.window + 1) : 0;
+    // keys that every row of the wave sees, and that any does
+    const int pos0 = t.len - t.n + (t.first + min(wrow, t.count - 1)) / a.G;
+    const int pos1 = t.len - t.n + (t.first + min(wrow + 31, t.count - 1)) / a.G;
+    const int all_hi = a.causal ? min(t.len, pos0 + 1) : t.len, any_hi = a.causal ? min(t.len, pos1 + 1) : t.len;
+    const int all_lo = a.window ? max(0, pos1 - a.window + 1) : 0, any_lo = a.window ? max(0, pos0 - a.window + 1) : 0;
+
+    const bool flip = a.c < 0.f;                             // the maximum is taken before the scaling: c has to be positive
+    const float c = fabsf(a.c);
+    v8 qf[KS];
+    {
+        const unsigned short* qp = a.q + token * a.q_st + head * a.q_sh + hf * 8;
 #pragma unroll
-            for (int e = 0; e < E; ++e) num[e] = fmaf(a.part_o[(s * step + row) * D + e * 64 + lane], f, num[e]);
+        for (int i = 0; i < KS; ++i) {
+            uint4 w = *reinterpret_cast<const uint4*>(qp + i * 16);
+            if (flip) {
+                w.x ^= 0x80008000u;
+                w.y ^= 0x80008000u;
+                w.z ^= 0x80008000u;
+                w.w ^= 0x80008000u;
+            }
+            qf[i] = __builtin_bit_cast(v8, w);
+        }
+    }
+    f32x16_t o[DTILES];
+#pragma unroll
+    for (int d = 0; d < DTILES; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+    float m = -INFINITY, l = 0.f, ref = 0.f;
+
+    const int* table = a.table + t.r * a.table_stride;
+    const int P = 1 << a.shift;
+    uint4 kw[L], vw[L];
+    float ks = 0.f, vs[4];
+    bool good = false;
+
+    // bytes of the wave's chunk of the tile at `base`, and the scales of the tile
+    auto fetch = [&](int base) {
+        const int key = base + 16 * wid;
+        const int page = table[min(key >> a.shift, a.W - 1)];
+        good = key < hi && key + 16 > lo && (unsigned)page < (unsigned)a.N;
+        const int64_t at = (int64_t)(good ? page : 0) * a.Hkv + h;
+        const unsigned char* kp = a.k_pages + (at * P + (key & (P - 1)) + (lane >> 2)) * D + (lane & 3) * (D / 4);
+        const unsigned char* vp = a.v_pages + (at * D + lane) * P + (key & (P - 1));
+#pragma unroll
+        for (int i = 0; i < L; ++i) {
+            kw[i] = good ? *reinterpret_cast<const uint4*>(kp + i * 16) : uint4{0, 0, 0, 0};
+            vw[i] = good ? *reinterpret_cast<const uint4*>(vp + (int64_t)i * 64 * P) : uint4{0, 0, 0, 0};
+        }
+        ks = good ? a.k_scale[at] : 1.f;
+        if constexpr (DT == PGN_F16) {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const int kw_ = base + 16 * w, pw = table[min(kw_ >> a.shift, a.W - 1)];
+                const bool gw = kw_ < hi && kw_ + 16 > lo && (unsigned)pw < (unsigned)a.N;
+                vs[w] = gw ? a.v_scale[(int64_t)pw * a.Hkv + h] : 0.f;
+            }
+        } else {
+            vs[0] = good ? a.v_scale[at] : 0.f;
+        }
+    };
+    float store_ref = 0.f;
+    auto store = [&](int base, int buf) {
+        BigTile<DT, D>& tile = s.tile[buf];
+        const int key = lane >> 2, mrow = (key & 3) + 4 * (wid & 1) + 8 * (key >> 2);
+        unsigned short* kp = tile.k + (32 * (wid >> 1) + mrow) * D;
+#pragma unroll
+        for (int i = 0; i < L; ++i) {
+            const int u = (lane & 3) * (UNITS / 4) + i * 2;
+            *reinterpret_cast<v8*>(kp + ((u ^ (mrow & 7)) * 8)) = widen8<DT>(kw[i].x, kw[i].y, 1.f);
+            *reinterpret_cast<v8*>(kp + (((u + 1) ^ (mrow & 7)) * 8)) = widen8<DT>(kw[i].z, kw[i].w, 1.f);
+        }
+        float vmul = 1.f, raise = 0.f, pscale = 1.f, vscale;
+        if constexpr (DT == PGN_F16) {                       // as in the 16-row kernel, raised by 2^7: maxima lag by 2^8
+            vscale = vs[0];
+#pragma unroll
+            for (int w = 1; w < 4; ++w) vscale = wid == w ? vs[w] : vscale;
+            store_ref = fmaxf(store_ref, fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3])));
+            const float ratio = good ? fmaxf(vscale / store_ref, 0x1p-60f) : 1.f;
+            vmul = fmaxf(ratio, 0x1p-15f);
+            pscale = 0x1p-7f * (vmul / ratio);
+            raise = (float)(127 - (int)(__float_as_uint(pscale) >> 23));
+        } else {
+            vscale = vs[0];
+            vmul = good ? vscale : 1.f;
+        }
+        // bytes that no row sees may hold anything: they count as 0, as do those of a page whose scale is 0
+        const int vkey = base + 16 * wid;
+        unsigned bad = 0;
+        if (vkey < lo || vkey + 16 > hi || vscale == 0.f) {
+            const bool give = good && vscale != 0.f;
+            const unsigned b0 = give ? key_bytes(vkey, 0, lo, hi) : 0u, b1 = give ? key_bytes(vkey, 1, lo, hi) : 0u;
+            const unsigned b2 = give ? key_bytes(vkey, 2, lo, hi) : 0u, b3 = give ? key_bytes(vkey, 3, lo, hi) : 0u;
+#pragma unroll
+            for (int i = 0; i < L; ++i) {
+                vw[i].x &= b0;
+                vw[i].y &= b1;
+                vw[i].z &= b2;
+                vw[i].w &= b3;
+            }
         }
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-            a.out[tok * a.o_st + hd * a.o_sh + e * 64 + lane] = Cvt<DT>::from_f32(den == 0.f ? 0.f : num[e] / den);
+        for (int i = 0; i < L; ++i) {
+            const int d = lane + 64 * i;
+            bad |= nan_bytes(vw[i].x) | nan_bytes(vw[i].y) | nan_bytes(vw[i].z) | nan_bytes(vw[i].w);
+            unsigned short* vp = tile.v + d * 64;
+            *reinterpret_cast<v8*>(vp + (((2 * wid) ^ (d & 7)) * 8)) = widen8<DT>(vw[i].x, vw[i].y, vmul);
+            *reinterpret_cast<v8*>(vp + (((2 * wid + 1) ^ (d & 7)) * 8)) = widen8<DT>(vw[i].z, vw[i].w, vmul);
+        }
+        const bool any_nan = __any(bad != 0);
+        if (lane == 0) {
+            s.ks[buf][wid] = fmaxf(ks * c, 0x1p-126f);       // 0 would turn a masked -inf into NaN
+            s.raise[buf][wid] = raise;
+            s.pscale[buf][wid] = pscale;
+            s.nan[buf][wid] = any_nan;
+            s.live[buf][wid] = good;
+            s.ref[buf] = store_ref;
+        }
+    };
+
+    if (kb < kend) {
+        fetch(kb);
+        store(kb, 0);
+    }
+    __syncthreads();
+    for (int base = kb, buf = 0; base < kend; base += 64, buf ^= 1) {
+        const bool more = base + 64 < kend;
+        if (more) fetch(base + 64);
+        if (base < any_hi && base + 64 > any_lo) {
+            const BigTile<DT, D>& tile = s.tile[buf];
+            f32x16_t x[2];
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[kt][i] = 0.f;
+                const unsigned short* kp = tile.k + (32 * kt + col) * D;
+#pragma unroll
+                for (int i = 0; i < KS; ++i)
+                    x[kt] = Mat<DT>::mfma32(*reinterpret_cast<const v8*>(kp + (((2 * i + hf) ^ (col & 7)) * 8)), qf[i], x[kt]);
+            }
+            const bool whole = base >= all_lo && base + 64 <= all_hi &&
+                               (s.live[buf][0] & s.live[buf][1] & s.live[buf][2] & s.live[buf][3]);
+            if (!whole) {
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt) {
+                    const bool live = s.live[buf][2 * kt + hf];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int key = base + 32 * kt + 16 * hf + i;
+                        x[kt][i] = live && key >= vis_lo && key < vis_hi ? x[kt][i] : -INFINITY;
+                    }
+                }
+            }
+            const float kc0 = s.ks[buf][hf], kc1 = s.ks[buf][2 + hf];
+            float mx0 = x[0][0], mx1 = x[1][0];
+#pragma unroll
+            for (int i = 1; i < 16; ++i) {
+                mx0 = fmaxf(mx0, x[0][i]);
+                mx1 = fmaxf(mx1, x[1][i]);
+            }
+            float mx = fmaxf(mx0 * kc0, mx1 * kc1);
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            float oscale = 1.f;
+            bool move = false;
+            if constexpr (DT == PGN_F16) {
+                const float now = s.ref[buf];
+                if (now != ref) {
+                    oscale = ref > 0.f ? ref / now : 1.f;
+                    move = true;
+                }
+                ref = now;
+            }
+            if (__any(mx > m + 8.f) || move) {               // also from -inf to the first score
+                const float m_new = mx > m + 8.f ? mx : m;
+                const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new);
+                m = m_new;
+                l *= alpha;
+                oscale *= alpha;
+#pragma unroll
+                for (int d = 0; d < DTILES; ++d)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[d][i] *= oscale;
+            }
+            const float base_m = m == -INFINITY ? 0.f : m;
+            float off0 = base_m, off1 = base_m;
+            if constexpr (DT == PGN_F16) {
+                off0 -= s.raise[buf][hf];
+                off1 -= s.raise[buf][2 + hf];
+            }
+            float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                x[0][i] = __builtin_amdgcn_exp2f(fmaf(x[0][i], kc0, -off0));
+                x[1][i] = __builtin_amdgcn_exp2f(fmaf(x[1][i], kc1, -off1));
+                sum0 += x[0][i];
+                sum1 += x[1][i];
+            }
+            if constexpr (DT == PGN_F16) {
+                sum0 *= s.pscale[buf][hf];
+                sum1 *= s.pscale[buf][2 + hf];
+            }
+            l += sum0 + sum1;
+            const bool nans = !whole && (s.nan[buf][0] | s.nan[buf][1] | s.nan[buf][2] | s.nan[buf][3]);
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    v8 p;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) p[j] = Mat<DT>::one(x[kt][8 * half + j]);
+#pragma unroll
+                    for (int d = 0; d < DTILES; ++d) {
+                        const unsigned short* vp = tile.v + (32 * d + col) * 64;
+                        v8 v = *reinterpret_cast<const v8*>(vp + (((4 * kt + 2 * hf + half) ^ (col & 7)) * 8));
+                        if (nans) {                          // as in the 16-row kernel: NaN values by a product of their own
+                            v8 is, see;
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                const int key = base + 32 * kt + 16 * hf + 8 * half + j;
+                                const bool n = v[j] != v[j];
+                                is[j] = Mat<DT>::one(n ? 1.f : 0.f);
+                                v[j] = n ? Mat<DT>::one(0.f) : v[j];
+                                see[j] = Mat<DT>::one(s.live[buf][2 * kt + hf] && key >= vis_lo && key < vis_hi ? 1.f : 0.f);
+                            }
+                            f32x16_t hit;
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) hit[i] = 0.f;
+                            hit = Mat<DT>::mfma32(is, see, hit);
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) o[d][i] = hit[i] > 0.f ? NAN : o[d][i];
+                        }
+                        o[d] = Mat<DT>::mfma32(v, p, o[d]);
+                    }
+                }
+        }
+        if (more) store(base + 64, buf ^ 1);
+        __syncthreads();
+    }
+
+    l += __shfl_xor(l, 32);
+    const float unit = DT == PGN_F16 ? ref * 0x1p-7f : 1.f;
+    if (wrow + col >= t.count) return;
+    if (a.big_nsplit == 1) {
+        const float inv = l == 0.f ? 0.f : unit / l;
+        unsigned short* op = a.out + token * a.o_st + head * a.o_sh;
+#pragma unroll
+        for (int d = 0; d < DTILES; ++d)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                u16x4_t w;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[j] = Cvt<DT>::from_f32(l == 0.f ? 0.f : o[d][4 * q + j] * inv);
+                unsigned short* p = op + d * 32 + q * 8 + hf * 4;
+                if (a.out_vec) {
+                    *reinterpret_cast<u16x4_t*>(p) = w;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) p[j] = w[j];
+                }
+            }
+    } else {
+        const int64_t at_row = ((int64_t)split * a.T + token) * a.Hq + head;
+        if (kb < kend) {
+#pragma unroll
+            for (int d = 0; d < DTILES; ++d)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    f32x4_t w;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) w[j] = o[d][4 * q + j] * unit;
+                    *reinterpret_cast<f32x4_t*>(a.part_o + at_row * D + d * 32 + q * 8 + hf * 4) = w;
+                }
+        }
+        if (hf == 0) a.part_ml[at_row] = make_float2(m, l);
     }
 }
 
+// Joins the splits of each row, one wave a row; rows whose kernel did not split are left alone.
+template <int DT, int D>
+__global__ __launch_bounds__(PGN_CA_THREADS) void pgn_cached_join_kernel(const CachedArgs a) {
+    constexpr int E = D / 64;
+    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t row = (int64_t)blockIdx.x * 4 + wid, step = (int64_t)a.T * a.Hq;
+    if (row >= step) return;
+    const int tok = (int)(row / a.Hq), hd = (int)(row - (int64_t)tok * a.Hq);
+    int nsplit = a.nsplit;
+    if (a.starts != nullptr) {
+        int lo = 0, hi = a.R;                                // the request that owns the token, if one does
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (a.starts[mid] <= tok) lo = mid;
+            else hi = mid;
+        }
+        TileRows t;
+        if (!request_rows(a, lo, t) || tok < t.begin || tok >= t.begin + t.n) return;
+        if (t.n * a.G > PGN_CA_FEW_ROWS) nsplit = a.big_nsplit;
+    }
+    if (nsplit == 1) return;
+    float big = -INFINITY;
+    for (int s = 0; s < nsplit; ++s) big = fmaxf(big, a.part_ml[s * step + row].x);
+    const float at = big == -INFINITY ? 0.f : big;
+    float den = 0.f, num[E] = {};
+    for (int s = 0; s < nsplit; ++s) {
+        const float2 ml = a.part_ml[s * step + row];
+        if (ml.x == -INFINITY && ml.y == 0.f) continue;      // nothing seen: its output was not written
+        const float f = __builtin_amdgcn_exp2f(ml.x - at);
+        den = fmaf(ml.y, f, den);
+#pragma unroll
+        for (int e = 0; e < E; ++e) num[e] = fmaf(a.part_o[(s * step + row) * D + e * 64 + lane], f, num[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        a.out[tok * a.o_st + hd * a.o_sh + e * 64 + lane] = Cvt<DT>::from_f32(den == 0.f ? 0.f : num[e] / den);
+}
+
 struct CachedPlan {
-    int tiles, tiles_per_request, nsplit, split_keys;
+    int tiles, tiles_per_request, nsplit, split_keys;        // 16-row kernel
+    int big_tiles, big_nsplit, big_split_keys;               // 128-row kernel; no tiles: not launched
 };
 
-// Tiles and splits of a call.  Enough workgroups for every CU to hold four are wanted; a split is 256 keys at least (one
-// round of the workgroup's four waves).
-static CachedPlan cached_plan(int T, int R, bool packed, int G, int Hkv, int64_t max_keys) {
-    CachedPlan p;
-    p.tiles_per_request = (G + 15) / 16;
-    p.tiles = packed ? (int)(((int64_t)T * G) / 16 + R) : R * p.tiles_per_request;
-    const int64_t wgs = (int64_t)p.tiles * Hkv, most = (max_keys + 255) / 256;
-    int64_t n = (1024 + wgs - 1) / wgs;
+// Splits of the keys so that `want` workgroups are there, each with `least` keys or more.
+static void split_keys(int64_t wgs, int64_t want, int64_t max_keys, int least, int* nsplit, int* keys) {
+    const int64_t most = (max_keys + least - 1) / least;
+    int64_t n = (want + wgs - 1) / wgs;
     n = n < most ? n : most;
     n = n < 1 ? 1 : (n > 64 ? 64 : n);
-    p.split_keys = (int)(((max_keys + 64 + n - 1) / n + 255) / 256 * 256);
-    p.nsplit = (int)((max_keys + 64 + p.split_keys - 1) / p.split_keys);
+    *keys = (int)(((max_keys + 64 + n - 1) / n + least - 1) / least * least);
+    *nsplit = (int)((max_keys + 64 + *keys - 1) / *keys);
+}
+
+static CachedPlan cached_plan(int T, int R, bool packed, int G, int Hkv, int64_t max_keys) {
+    CachedPlan p;
+    const int few = packed ? (PGN_CA_FEW_ROWS < (int64_t)T * G ? PGN_CA_FEW_ROWS : T * G) : G;
+    p.tiles_per_request = (few + 15) / 16;
+    p.tiles = R * p.tiles_per_request;
+    split_keys((int64_t)(packed ? R : p.tiles) * Hkv, 1024, max_keys, 256, &p.nsplit, &p.split_keys);
+    p.big_tiles = packed && (int64_t)T * G > PGN_CA_FEW_ROWS ? (int)((int64_t)T * G / 128 + R) : 0;
+    p.big_nsplit = 1;
+    p.big_split_keys = 0;
+    if (p.big_tiles) split_keys((int64_t)p.big_tiles * Hkv, 512, max_keys, 512, &p.big_nsplit, &p.big_split_keys);
     return p;
+}
+
+static size_t cached_workspace(const CachedPlan& p, int64_t rows, int D) {
+    const int n = p.nsplit > p.big_nsplit ? p.nsplit : p.big_nsplit;
+    return n == 1 ? 0 : (size_t)n * rows * (D * 4 + 8);
 }
 
 }  // namespace
@@ -403,7 +777,7 @@ extern "C" size_t pgn_cached_attention_workspace_bytes(int num_tokens, int R, in
                                                        int W, int page_size) {
     if (!cached_sizes(num_tokens, R, Hq, Hkv, head_dim, W, page_size)) return 0;
     const CachedPlan p = cached_plan(num_tokens, R, packed != 0, Hq / Hkv, Hkv, (int64_t)W * page_size);
-    return p.nsplit == 1 ? 0 : (size_t)p.nsplit * num_tokens * Hq * (head_dim * 4 + 8);
+    return cached_workspace(p, (int64_t)num_tokens * Hq, head_dim);
 }
 
 extern "C" int pgn_cached_attention(const void* q, int dtype, const void* k_pages, const void* v_pages,
@@ -427,7 +801,7 @@ extern "C" int pgn_cached_attention(const void* q, int dtype, const void* k_page
         !pgn_aligned(out, 2))
         return PGN_ERR_INVALID;
     const CachedPlan p = cached_plan(num_tokens, R, starts != nullptr, Hq / Hkv, Hkv, (int64_t)W << shift);
-    const size_t need = p.nsplit == 1 ? 0 : (size_t)p.nsplit * num_tokens * Hq * (head_dim * 4 + 8);
+    const size_t need = cached_workspace(p, (int64_t)num_tokens * Hq, head_dim);
     if (need > 0 && (workspace == nullptr || workspace_bytes < need || !pgn_aligned(workspace, 16))) return PGN_ERR_INVALID;
     CachedArgs a;
     a.q = (const unsigned short*)q;
@@ -440,7 +814,7 @@ extern "C" int pgn_cached_attention(const void* q, int dtype, const void* k_page
     a.starts = starts;
     a.out = (unsigned short*)out;
     a.part_o = (float*)workspace;
-    a.part_ml = need ? (float2*)((char*)workspace + (size_t)p.nsplit * num_tokens * Hq * head_dim * 4) : nullptr;
+    a.part_ml = need ? (float2*)((char*)workspace + need / (head_dim * 4 + 8) * (head_dim * 4)) : nullptr;
     a.table_stride = table_stride;
     a.q_st = q_st;
     a.q_sh = q_sh;
@@ -459,23 +833,30 @@ extern "C" int pgn_cached_attention(const void* q, int dtype, const void* k_page
     a.split_keys = p.split_keys;
     a.nsplit = p.nsplit;
     a.tiles_per_request = p.tiles_per_request;
+    a.big_split_keys = p.big_split_keys;
+    a.big_nsplit = p.big_nsplit;
+    a.out_vec = pgn_aligned(out, 8) && o_st % 4 == 0 && o_sh % 4 == 0;
     a.c = scale * 1.4426950408889634f;
     hipStream_t s = (hipStream_t)stream;
-    const dim3 grid(p.tiles, Hkv, p.nsplit), join(p.tiles, Hkv), block(PGN_CA_THREADS);
-    const size_t lds = (size_t)4 * 16 * head_dim * 4;        // 64 KiB at head dim 256
-#define PGN_CA_LAUNCH(DT, D)                                                                                           \
+    const dim3 block(PGN_CA_THREADS);
+#define PGN_CA_KERNEL(kernel, lds, grid)                                                                               \
     do {                                                                                                               \
-        if (D == 256) {                                      /* 64 KiB and the maxima beside it */                     \
-            hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(pgn_cached_rows16_kernel<DT, D>),         \
-                                               hipFuncAttributeMaxDynamicSharedMemorySize, 72 * 1024);                 \
+        if ((lds) > 64 * 1024 - 1024) {                                                                                \
+            hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),                                  \
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, (int)(lds));                \
             if (e != hipSuccess) return (int)e;                                                                        \
         }                                                                                                              \
-        hipLaunchKernelGGL((pgn_cached_rows16_kernel<DT, D>), grid, block, lds, s, a);                                 \
+        hipLaunchKernelGGL(kernel, grid, block, lds, s, a);                                                            \
         PGN_LAUNCH_CHECK();                                                                                            \
-        if (p.nsplit > 1) {                                                                                            \
-            hipLaunchKernelGGL((pgn_cached_join_kernel<DT, D>), join, block, 0, s, a);                                 \
-            PGN_LAUNCH_CHECK();                                                                                        \
-        }                                                                                                              \
+    } while (0)
+#define PGN_CA_LAUNCH(DT, D)                                                                                           \
+    do {                                                                                                               \
+        if (p.big_tiles)                                                                                               \
+            PGN_CA_KERNEL((pgn_cached_rows128_kernel<DT, D>), sizeof(BigLds<DT, D>),                                   \
+                          dim3(Hkv, p.big_tiles, p.big_nsplit));                                                       \
+        PGN_CA_KERNEL((pgn_cached_rows16_kernel<DT, D>), (size_t)4 * 16 * D * 4, dim3(Hkv, p.tiles, p.nsplit));        \
+        if (need)                                                                                                      \
+            PGN_CA_KERNEL((pgn_cached_join_kernel<DT, D>), 0, dim3((unsigned)(((int64_t)num_tokens * Hq + 3) / 4)));   \
     } while (0)
 #define PGN_CA_DIMS(DT)                                                                                                \
     do {                                                                                                               \
@@ -487,5 +868,6 @@ extern "C" int pgn_cached_attention(const void* q, int dtype, const void* k_page
     else PGN_CA_DIMS(PGN_F16);
 #undef PGN_CA_DIMS
 #undef PGN_CA_LAUNCH
+#undef PGN_CA_KERNEL
     return PGN_OK;
 }

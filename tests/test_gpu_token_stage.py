@@ -294,6 +294,27 @@ def test_prompts_against_the_oracle(new, Hq, Hkv, D, dt, window):
     _check_attention(_q(sum(new), Hq, D, dt), cache, _table(lens, 16, 120), i32(lens), starts=starts, window=window)
 
 
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D,Hq,Hkv,new,held,window", [
+    (128, 2, 2, [300, 129, 64, 65], [0, 77, 0, 500], 0), (64, 4, 1, [257], [1000], 0), (64, 3, 1, [43, 21, 22], [11, 3000, 0], 0),
+    (256, 1, 1, [200, 70], [60, 0], 0), (128, 2, 1, [150, 40], [400, 900], 128), (64, 1, 1, [90], [6000], 0), (64, 1, 1, [100], [5000], 700)])
+@pytest.mark.parametrize("P", [16, 64])
+def test_long_prompts_against_the_oracle(D, Hq, Hkv, new, held, window, P, dt):
+    """More rows than a tile, requests on either side of the 64 rows that tell the two kernels apart, few rows against many
+    keys (split), a window that leaves whole tiles out."""
+    lens = [n + h for n, h in zip(new, held)]
+    starts = i32(np.cumsum([0] + new).tolist())
+    N = sum(-(-n // P) for n in lens) + 3
+    _check_attention(_q(sum(new), Hq, D, dt), _cache(N, Hkv, P, D, seed=1), _table(lens, P, N), i32(lens), starts=starts, window=window)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.125, 2.0])
+def test_scales_of_the_scores(scale):
+    lens, new = [130, 200], [130, 3]
+    _check_attention(_q(133, 2, 64, torch.bfloat16), _cache(30, 2, 16, 64), _table(lens, 16, 30), i32(lens),
+                     starts=i32([0, 130, 133]), scale=scale)
+
+
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("P", [32, 128])
 def test_prompts_without_a_mask_and_with_more_queries_than_keys(causal, P):
@@ -493,6 +514,23 @@ def test_sampling_ties_go_by_the_lowest_index(dt):
     for p in (0.25, 0.5, 0.75):
         _check_sample(flat, u, top_p=p)
     _check_sample(flat, u, top_k=64, top_p=0.5)
+
+
+def test_sampling_more_equal_logits_than_a_list_holds():
+    """Thousands of ids in one bin of the histogram: the border is searched for by the key's digits."""
+    x = torch.zeros(4, 30011, device=DEV)
+    x[1, 5000:] = -1.0
+    x[2, ::3] = 0.5
+    x[3, 7] = 6.0
+    u = torch.tensor([0.1, 0.55, 0.8, 0.999], device=DEV)
+    for kw in ({"top_p": 0.5}, {"top_p": 0.9}, {"top_k": 6000}, {"top_k": 6000, "top_p": 0.3}, {"top_k": 12000, "top_p": 0.99}, {"top_k": 40},
+               {"top_k": 40, "top_p": 0.5, "temperature": 3.0}, {"min_p": 0.7}):
+        _check_sample(x, u, **kw)
+    far = torch.full((2, 9000), -500.0, device=DEV)                 # the top-k reaches ids 700 octaves under the largest
+    far[:, 4] = 0.0
+    far[1, ::2] = -1000.0
+    _check_sample(far, u[:2], top_k=5000)
+    _check_sample(far, u[:2], top_k=5000, top_p=0.9999, temperature=200.0)
 
 
 def test_sampling_masked_and_infinite_logits():
