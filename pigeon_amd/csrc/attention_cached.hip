@@ -34,7 +34,7 @@ struct CachedArgs {
     int64_t table_stride, q_st, q_sh, o_st, o_sh;
     int T, R, Hq, Hkv, G, W, shift, N, causal, window;
     int split_keys, nsplit, tiles_per_request;               // of the 16-row kernel
-    int big_split_keys, big_nsplit;                          // of the 128-row kernel
+    int big_split_keys, big_nsplit, big_tiles;               // of the 128-row kernel
     int out_vec;                                             // rows of `out` begin on 8 bytes
     float c;                                                 // scale * log2(e)
 };
@@ -169,9 +169,10 @@ __global__ __launch_bounds__(PGN_CA_THREADS) void pgn_cached_rows16_kernel(const
     __shared__ float lds_m[4][16], lds_l[4][16];
     const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
     const int g = lane >> 4, col = lane & 15;
-    const int h = blockIdx.x, split = blockIdx.z;
+    // heads fastest: 88 us against 101 with all heads of a stretch of keys on one XCD (16 requests of up to 4096, 32 heads)
+    const int h = blockIdx.x % a.Hkv, split = blockIdx.y;
     TileRows t;
-    if (!few_rows_tile(a, blockIdx.y, t)) return;
+    if (!few_rows_tile(a, blockIdx.x / a.Hkv, t)) return;
     int lo, hi;
     key_range(a, t, lo, hi);
     const int kb = (lo & ~63) + split * a.split_keys;
@@ -402,9 +403,9 @@ __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void pgn_cached_rows128_ke
     BigLds<DT, D>& s = *reinterpret_cast<BigLds<DT, D>*>(smem_big);
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hf = lane >> 5, col = lane & 31;
-    const int h = blockIdx.x, split = blockIdx.z;
+    const int h = blockIdx.x % a.Hkv, split = blockIdx.y;    // heads fastest: a head's tiles share one XCD's L2
     TileRows t;
-    if (!many_rows_tile(a, gridDim.y - 1 - blockIdx.y, t)) return;      // the tiles with the most keys first
+    if (!many_rows_tile(a, a.big_tiles - 1 - (int)(blockIdx.x / a.Hkv), t)) return;     // a request's longest rows first
     int lo, hi;
     key_range(a, t, lo, hi);
     const int kb = (lo & ~63) + split * a.big_split_keys;
@@ -694,38 +695,49 @@ __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void pgn_cached_rows128_ke
     }
 }
 
-// Joins the splits of each row, one wave a row; rows whose kernel did not split are left alone.
-template <int DT, int D>
+// Joins the splits of the rows of one kernel's tiles, a wave a row, four rows a workgroup.  Each lane takes one split's
+// maximum and sum (64 splits at most), so that every weight is known before the first partial output is read and the
+// reads do not wait for one another.
+template <int DT, int D, bool MANY>
 __global__ __launch_bounds__(PGN_CA_THREADS) void pgn_cached_join_kernel(const CachedArgs a) {
     constexpr int E = D / 64;
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t row = (int64_t)blockIdx.x * 4 + wid, step = (int64_t)a.T * a.Hq;
-    if (row >= step) return;
-    const int tok = (int)(row / a.Hq), hd = (int)(row - (int64_t)tok * a.Hq);
-    int nsplit = a.nsplit;
-    if (a.starts != nullptr) {
-        int lo = 0, hi = a.R;                                // the request that owns the token, if one does
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (a.starts[mid] <= tok) lo = mid;
-            else hi = mid;
-        }
-        TileRows t;
-        if (!request_rows(a, lo, t) || tok < t.begin || tok >= t.begin + t.n) return;
-        if (t.n * a.G > PGN_CA_FEW_ROWS) nsplit = a.big_nsplit;
-    }
-    if (nsplit == 1) return;
-    float big = -INFINITY;
-    for (int s = 0; s < nsplit; ++s) big = fmaxf(big, a.part_ml[s * step + row].x);
-    const float at = big == -INFINITY ? 0.f : big;
-    float den = 0.f, num[E] = {};
-    for (int s = 0; s < nsplit; ++s) {
-        const float2 ml = a.part_ml[s * step + row];
-        if (ml.x == -INFINITY && ml.y == 0.f) continue;      // nothing seen: its output was not written
-        const float f = __builtin_amdgcn_exp2f(ml.x - at);
-        den = fmaf(ml.y, f, den);
+    TileRows t;
+    const int h = blockIdx.x % a.Hkv, tile = blockIdx.x / a.Hkv;
+    if (!(MANY ? many_rows_tile(a, tile, t) : few_rows_tile(a, tile, t))) return;
+    const int rr = blockIdx.y * 4 + wid;
+    if (rr >= t.count) return;
+    const int nsplit = MANY ? a.big_nsplit : a.nsplit;
+    const int rw = t.first + rr, tok = t.begin + rw / a.G, hd = h * a.G + rw % a.G;
+    const int64_t row = (int64_t)tok * a.Hq + hd, step = (int64_t)a.T * a.Hq;
+    const float2 ml = lane < nsplit ? a.part_ml[lane * step + row] : make_float2(-INFINITY, 0.f);
+    float big = ml.x;
 #pragma unroll
-        for (int e = 0; e < E; ++e) num[e] = fmaf(a.part_o[(s * step + row) * D + e * 64 + lane], f, num[e]);
+    for (int off = 32; off > 0; off >>= 1) big = fmaxf(big, __shfl_xor(big, off));
+    const float at = big == -INFINITY ? 0.f : big;
+    const float f = __builtin_amdgcn_exp2f(ml.x - at);
+    // a split that saw nothing has written no output
+    uint64_t seen = __ballot(!(ml.x == -INFINITY && ml.y == 0.f));
+    float den = ml.y * f;
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) den += __shfl_xor(den, off);
+    float num[E] = {};
+    const float* part = a.part_o + row * D + lane;
+    while (seen) {
+        float w[8], v[8][E];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {                        // eight splits at a time; the last ones may repeat, weighing 0
+            const int s = seen ? __builtin_ctzll(seen) : 0;
+            w[i] = seen ? __shfl(f, s) : 0.f;
+            const bool on = seen != 0;
+            seen &= seen - 1;
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[i][e] = on ? part[s * step * D + e * 64] : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int e = 0; e < E; ++e) num[e] = fmaf(v[i][e], w[i], num[e]);
     }
 #pragma unroll
     for (int e = 0; e < E; ++e)
@@ -795,12 +807,13 @@ extern "C" int pgn_cached_attention(const void* q, int dtype, const void* k_page
     if (dtype != PGN_BF16 && dtype != PGN_F16) return PGN_ERR_UNSUPPORTED;
     const int shift = cached_shift(page_size);
     if (shift < 0 || (head_dim != 64 && head_dim != 128 && head_dim != 256)) return PGN_ERR_UNSUPPORTED;
-    if (((int64_t)W << shift) > 0x7fffff00 - 65536 || Hkv > 65535 || (int64_t)num_tokens * (Hq / Hkv) > 0x7fffffff - 65536)
+    if (((int64_t)W << shift) > 0x7fffff00 - 65536 || Hkv > 65535 || R > (1 << 26) || (int64_t)num_tokens * (Hq / Hkv) > 0x7fffffff - 65536)
         return PGN_ERR_UNSUPPORTED;
     if (!pgn_aligned(q, 16) || q_st % 8 != 0 || q_sh % 8 != 0 || !pgn_aligned(k_pages, 16) || !pgn_aligned(v_pages, 16) ||
         !pgn_aligned(out, 2))
         return PGN_ERR_INVALID;
     const CachedPlan p = cached_plan(num_tokens, R, starts != nullptr, Hq / Hkv, Hkv, (int64_t)W << shift);
+    if ((int64_t)p.tiles * Hkv > 0x7fffffff || (int64_t)p.big_tiles * Hkv > 0x7fffffff) return PGN_ERR_UNSUPPORTED;
     const size_t need = cached_workspace(p, (int64_t)num_tokens * Hq, head_dim);
     if (need > 0 && (workspace == nullptr || workspace_bytes < need || !pgn_aligned(workspace, 16))) return PGN_ERR_INVALID;
     CachedArgs a;
@@ -835,6 +848,7 @@ extern "C" int pgn_cached_attention(const void* q, int dtype, const void* k_page
     a.tiles_per_request = p.tiles_per_request;
     a.big_split_keys = p.big_split_keys;
     a.big_nsplit = p.big_nsplit;
+    a.big_tiles = p.big_tiles;
     a.out_vec = pgn_aligned(out, 8) && o_st % 4 == 0 && o_sh % 4 == 0;
     a.c = scale * 1.4426950408889634f;
     hipStream_t s = (hipStream_t)stream;
@@ -853,10 +867,12 @@ extern "C" int pgn_cached_attention(const void* q, int dtype, const void* k_page
     do {                                                                                                               \
         if (p.big_tiles)                                                                                               \
             PGN_CA_KERNEL((pgn_cached_rows128_kernel<DT, D>), sizeof(BigLds<DT, D>),                                   \
-                          dim3(Hkv, p.big_tiles, p.big_nsplit));                                                       \
-        PGN_CA_KERNEL((pgn_cached_rows16_kernel<DT, D>), (size_t)4 * 16 * D * 4, dim3(Hkv, p.tiles, p.nsplit));        \
-        if (need)                                                                                                      \
-            PGN_CA_KERNEL((pgn_cached_join_kernel<DT, D>), 0, dim3((unsigned)(((int64_t)num_tokens * Hq + 3) / 4)));   \
+                          dim3(Hkv * p.big_tiles, p.big_nsplit));                                                      \
+        PGN_CA_KERNEL((pgn_cached_rows16_kernel<DT, D>), (size_t)4 * 16 * D * 4, dim3(Hkv * p.tiles, p.nsplit));       \
+        if (p.nsplit > 1)                                                                                              \
+            PGN_CA_KERNEL((pgn_cached_join_kernel<DT, D, false>), 0, dim3(Hkv * p.tiles, 4));                          \
+        if (p.big_nsplit > 1)                                                                                          \
+            PGN_CA_KERNEL((pgn_cached_join_kernel<DT, D, true>), 0, dim3(Hkv * p.big_tiles, 32));                      \
     } while (0)
 #define PGN_CA_DIMS(DT)                                                                                                \
     do {                                                                                                               \

@@ -17,6 +17,8 @@ namespace {
 // One workgroup does the bookkeeping: it is a chain of three prefix sums over the requests (pages given back, tokens
 // added, pages wanted) whose results every later step needs, 4 bytes a request.  The pages themselves are then moved
 // flat, one thread a page: a thread finds its request by bisection in the prefix sums, which lie in LDS.
+// A chain of short steps is bound by their latency, and a barrier of 16 waves is the longest of them, so a small call
+// runs in one wave or four.
 #define PGN_ADV_THREADS 1024
 // Up to this many slots the bookkeeping workgroup fills the slot map itself (one launch); above it a second, wide launch
 // does.  At 8192 slots the workgroup's 8 rounds cost what the second launch would.
@@ -27,25 +29,31 @@ __device__ __forceinline__ int64_t adv_pages(int64_t tokens, int shift) {
 }
 
 // inclusive prefix sum over the workgroup; `total` is the sum of all
-__device__ int64_t adv_scan(int64_t v, int64_t* wave_sums, int64_t& total) {
+template <int NT, typename I>
+__device__ I adv_scan(I v, int64_t* wave_sums, I& total) {
     const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
-        const int64_t o = __shfl_up(v, off);
+        const I o = __shfl_up(v, off);
         if (lane >= off) v += o;
     }
-    if (lane == 63) wave_sums[wid] = v;
-    __syncthreads();
-    int64_t before = 0, all = 0;
+    if constexpr (NT == 64) {
+        total = __shfl(v, 63);
+        return v;
+    } else {
+        if (lane == 63) wave_sums[wid] = v;
+        __syncthreads();
+        I before = 0, all = 0;
 #pragma unroll
-    for (int w = 0; w < PGN_ADV_THREADS / 64; ++w) {
-        const int64_t x = wave_sums[w];
-        before += w < wid ? x : 0;
-        all += x;
+        for (int w = 0; w < NT / 64; ++w) {
+            const I x = (I)wave_sums[w];
+            before += w < wid ? x : 0;
+            all += x;
+        }
+        total = all;
+        __syncthreads();
+        return v + before;
     }
-    total = all;
-    __syncthreads();
-    return v + before;
 }
 
 // last index i in [0, n) with at[i] <= x (at[] ascending, at[0] <= x)
@@ -60,7 +68,8 @@ __device__ __forceinline__ int adv_find(const int* at, int n, int x) {
 }
 
 struct AdvRequest {
-    int64_t held, keep, add, have, kept;
+    int64_t held, keep, add;
+    int have, kept;
 };
 
 __device__ __forceinline__ AdvRequest adv_request(const int* lens, const int* keep, const int* add, int r, int R, int W,
@@ -68,100 +77,111 @@ __device__ __forceinline__ AdvRequest adv_request(const int* lens, const int* ke
     AdvRequest q = {0, 0, 0, 0, 0};
     if (r < R) {
         const int64_t room = (int64_t)W << shift;
-        const int64_t h = lens[r];
+        const int64_t h = lens[r], k = keep ? keep[r] : h, a = add[r];
         q.held = h < 0 ? 0 : (h > room ? room : h);          // a length beyond the table names pages that do not exist
-        const int64_t k = keep ? (int64_t)keep[r] : q.held;
         q.keep = k < 0 ? 0 : (k > q.held ? q.held : k);
-        const int64_t a = add[r];
         q.add = a < 0 ? 0 : a;
-        q.have = adv_pages(q.held, shift);
-        q.kept = adv_pages(q.keep, shift);
+        q.have = (int)adv_pages(q.held, shift);
+        q.kept = (int)adv_pages(q.keep, shift);
     }
     return q;
 }
 
-__global__ __launch_bounds__(PGN_ADV_THREADS) void pgn_page_advance_kernel(
-    int* lens, const int* keep, const int* add, int* __restrict__ table,
-    int64_t table_stride, int* __restrict__ free_pages, int* __restrict__ free_count, int N, int R, int W, int shift,
-    int T, int fill_slots, int64_t* __restrict__ slots, int* __restrict__ starts, int* __restrict__ status) {
-    __shared__ int64_t wave_sums[PGN_ADV_THREADS / 64];
-    __shared__ int at[PGN_ADV_THREADS + 1];                  // prefix of what is being moved, within the chunk
-    __shared__ int col[PGN_ADV_THREADS];                     // first table column concerned (or the kept length)
+template <int NT>
+__global__ __launch_bounds__(NT) void pgn_page_advance_kernel(
+    int* lens, const int* keep, const int* add, int* __restrict__ table, int64_t table_stride,
+    int* __restrict__ free_pages, int* __restrict__ free_count, int N, int R, int W, int shift, int T, int fill_slots,
+    int64_t* __restrict__ slots, int* __restrict__ starts, int* __restrict__ status) {
+    __shared__ int64_t wave_sums[NT / 64];
+    __shared__ int at[NT + 1];                               // prefix of what is being moved, within the chunk
+    __shared__ int col[NT];                                  // first table column concerned (or the kept length)
     const int tid = threadIdx.x;
+    AdvRequest q = adv_request(lens, keep, add, tid, R, W, shift);       // of the chunk at hand, here the first
     int64_t count = free_count[0];
     count = count < 0 ? 0 : (count > N ? N : count);
 
     // pages given back in all: the stack is filled so that popping returns them in request order
-    int64_t released = 0;
-    for (int r0 = 0; r0 < R; r0 += PGN_ADV_THREADS) {
-        const AdvRequest q = adv_request(lens, keep, add, r0 + tid, R, W, shift);
-        int64_t total;
-        adv_scan(q.have - q.kept, wave_sums, total);
-        released += total;
+    int total, mine = q.have - q.kept, upto = adv_scan<NT>(mine, wave_sums, total);
+    int64_t released = total;
+    for (int r0 = NT; r0 < R; r0 += NT) {
+        const AdvRequest o = adv_request(lens, keep, add, r0 + tid, R, W, shift);
+        int more;
+        adv_scan<NT>(o.have - o.kept, wave_sums, more);
+        released += more;
     }
-    int64_t done = 0;
     if (released > 0) {
-        for (int r0 = 0; r0 < R; r0 += PGN_ADV_THREADS) {
-            const AdvRequest q = adv_request(lens, keep, add, r0 + tid, R, W, shift);
-            int64_t total;
-            const int64_t mine = q.have - q.kept;
-            at[tid] = (int)(adv_scan(mine, wave_sums, total) - mine);
-            col[tid] = (int)q.kept;
+        int64_t done = 0;
+        for (int r0 = 0;;) {
+            at[tid] = upto - mine;
+            col[tid] = q.kept;
             __syncthreads();
-            for (int64_t e = tid; e < total; e += PGN_ADV_THREADS) {
-                const int i = adv_find(at, PGN_ADV_THREADS, (int)e);
+            for (int e = tid; e < total; e += NT) {
+                const int i = adv_find(at, NT, e);
                 const int64_t place = count + released - 1 - (done + e);
                 if (place < N)                               // more pages back than the pool holds: a caller's mistake
-                    free_pages[place] = table[(r0 + i) * table_stride + col[i] + ((int)e - at[i])];
+                    free_pages[place] = table[(r0 + i) * table_stride + col[i] + (e - at[i])];
             }
             done += total;
             __syncthreads();
+            r0 += NT;
+            if (r0 >= R) break;
+            q = adv_request(lens, keep, add, r0 + tid, R, W, shift);
+            mine = q.have - q.kept;
+            upto = adv_scan<NT>(mine, wave_sums, total);
         }
+        if (R > NT) q = adv_request(lens, keep, add, tid, R, W, shift);
     }
     int64_t top = count + released;
     top = top > N ? N : top;
 
     int64_t tokens = 0, wanted = 0, popped = 0;
-    for (int r0 = 0; r0 < R; r0 += PGN_ADV_THREADS) {
+    for (int r0 = 0; r0 < R; r0 += NT) {
         const int r = r0 + tid;
-        const AdvRequest q = adv_request(lens, keep, add, r, R, W, shift);
-        int64_t total;
-        const int64_t end = tokens + adv_scan(q.add, wave_sums, total);
+        if (r0 > 0) q = adv_request(lens, keep, add, r, R, W, shift);
+        int64_t chunk_tokens;
+        const int64_t end = tokens + adv_scan<NT>(q.add, wave_sums, chunk_tokens);
         const int64_t begin = end - q.add;
-        tokens += total;
+        tokens += chunk_tokens;
         const bool fits = r < R && q.keep + q.add <= ((int64_t)W << shift) && end <= T;
-        int64_t want = fits ? adv_pages(q.keep + q.add, shift) - q.kept : 0;
-        const int64_t taken = wanted + adv_scan(want, wave_sums, total);
-        wanted += total;
-        const bool ok = fits && (want == 0 || taken <= top);
-        want = ok ? want : 0;
-        const int64_t first = adv_scan(want, wave_sums, total) - want;
+        int want = fits ? (int)adv_pages(q.keep + q.add, shift) - q.kept : 0;
+        int first = adv_scan<NT>(want, wave_sums, total);
+        bool ok = fits;
+        if (wanted + total > top) {                          // not enough pages: nobody who needs some overtakes
+            ok = fits && (want == 0 || wanted + first <= top);
+            wanted += total;
+            want = ok ? want : 0;
+            first = adv_scan<NT>(want, wave_sums, total);
+        } else {
+            wanted += total;
+        }
+        first -= want;
         if (r < R) {
             lens[r] = (int)(ok ? q.keep + q.add : q.keep);
             status[r] = ok ? 0 : 1;
             starts[r + 1] = (int)(end < T ? end : T);
             if (r == 0) starts[0] = 0;
         }
-        at[tid] = (int)first;
-        col[tid] = (int)q.kept;
-        __syncthreads();
-        for (int64_t e = tid; e < total; e += PGN_ADV_THREADS) {
-            const int i = adv_find(at, PGN_ADV_THREADS, (int)e);
-            table[(r0 + i) * table_stride + col[i] + ((int)e - at[i])] = free_pages[top - 1 - popped - e];
+        if (total > 0) {
+            at[tid] = first;
+            col[tid] = q.kept;
+            __syncthreads();
+            for (int e = tid; e < total; e += NT) {
+                const int i = adv_find(at, NT, e);
+                table[(r0 + i) * table_stride + col[i] + (e - at[i])] = free_pages[top - 1 - popped - e];
+            }
+            popped += total;
+            __syncthreads();
         }
-        popped += total;
-        __syncthreads();
         if (fill_slots) {                                    // T <= PGN_ADV_FUSED_SLOTS here
-            const int64_t b = begin < T ? begin : T;
-            at[tid] = (int)b;
-            if (tid == PGN_ADV_THREADS - 1) at[PGN_ADV_THREADS] = (int)(end < T ? end : T);
+            at[tid] = (int)(begin < T ? begin : T);
+            if (tid == NT - 1) at[NT] = (int)(end < T ? end : T);
             col[tid] = ok ? (int)q.keep : -1;
             __syncthreads();
-            for (int64_t t = at[0] + tid; t < at[PGN_ADV_THREADS]; t += PGN_ADV_THREADS) {
-                const int i = adv_find(at, PGN_ADV_THREADS, (int)t);
+            for (int t = at[0] + tid; t < at[NT]; t += NT) {
+                const int i = adv_find(at, NT, t);
                 int64_t slot = -1;
                 if (col[i] >= 0) {
-                    const int pos = col[i] + ((int)t - at[i]);
+                    const int pos = col[i] + (t - at[i]);
                     slot = ((int64_t)table[(r0 + i) * table_stride + (pos >> shift)] << shift) + (pos & ((1 << shift) - 1));
                 }
                 slots[t] = slot;
@@ -170,7 +190,7 @@ __global__ __launch_bounds__(PGN_ADV_THREADS) void pgn_page_advance_kernel(
         }
     }
     if (fill_slots)
-        for (int64_t t = (tokens < T ? tokens : T) + tid; t < T; t += PGN_ADV_THREADS) slots[t] = -1;
+        for (int t = (int)(tokens < T ? tokens : T) + tid; t < T; t += NT) slots[t] = -1;
     if (tid == 0) free_count[0] = (int)(top - popped);
 }
 
@@ -210,23 +230,12 @@ __global__ __launch_bounds__(256) void pgn_page_slots_kernel(const int* __restri
 // A run is a stretch of consecutive tokens whose slots follow one another inside one page; the slot map makes at most
 // one run of a page in a call.  One workgroup takes the runs that begin among its `chunk` tokens, for one head and one
 // of the two halves, so it owns the (page, head) pairs that it writes: their scale is found, the older tokens of the
-// page are rescaled if it grew, and the new ones are stored, with no exchange between workgroups.  The tokens are read
-// twice (the scale needs their largest magnitude first); the second read hits the caches.
-#define PGN_CW_THREADS 256
-
-// 8 consecutive elements of a token's row as fp32
-template <int DT>
-__device__ __forceinline__ void cw_load8(const unsigned short* p, bool vec, float* f) {
-    u16x8_t v;
-    if (vec) {
-        v = *reinterpret_cast<const u16x8_t*>(p);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = p[j];
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = Cvt<DT>::to_f32(v[j]);
-}
+// page are rescaled if it grew, and the new ones are stored, with no exchange between workgroups.
+//
+// A wave keeps 16 rows in registers between finding the largest magnitude and storing, so a run of up to 64 tokens is
+// read once.  Keys: 8 consecutive dims a lane, 16 bytes in and 8 out.  Values: the 16 page rows by D / 64 consecutive
+// dims a lane, and they leave as they have to lie: the conversions pack four TOKENS of one dim, 16 tokens of a dim are
+// one 16-byte store.
 
 // The least power of two s >= 2^-100 with amax <= 448 s (448 = 1.75 * 2^8 is e4m3's largest value), from the bits.
 __device__ __forceinline__ float cw_scale(float amax) {
@@ -236,124 +245,266 @@ __device__ __forceinline__ float cw_scale(float amax) {
     return __uint_as_float((unsigned)(k + 127) << 23);
 }
 
+// Magnitudes are compared as the 16-bit patterns that they are, two at a time (larger magnitude, larger pattern); from
+// `CwInf` on they are not finite.
 template <int DT>
-__global__ __launch_bounds__(PGN_CW_THREADS) void pgn_cache_write_kernel(
+struct CwInf {
+    static constexpr unsigned bits = DT == PGN_BF16 ? 0x7f80u : 0x7c00u;
+};
+__device__ __forceinline__ unsigned cw_max2(unsigned amax, unsigned pair) {
+    const u16x2_t m = __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, amax),
+                                                __builtin_bit_cast(u16x2_t, pair & 0x7fff7fffu));
+    return __builtin_bit_cast(unsigned, m);
+}
+// a pair with what is not finite left out
+template <int DT>
+__device__ __forceinline__ unsigned cw_finite2(unsigned pair) {
+    const unsigned m = pair & 0x7fff7fffu;
+    return ((m & 0xffffu) < CwInf<DT>::bits ? m & 0xffffu : 0) | ((m >> 16) < CwInf<DT>::bits ? m & 0xffff0000u : 0);
+}
+
+template <int DT>
+__device__ __forceinline__ float cw_lo(unsigned pair) { return Cvt<DT>::to_f32((unsigned short)(pair & 0xffffu)); }
+template <int DT>
+__device__ __forceinline__ float cw_hi(unsigned pair) { return Cvt<DT>::to_f32((unsigned short)(pair >> 16)); }
+
+// N consecutive elements in (N + 1) / 2 words
+template <int N>
+struct CwVec {
+    unsigned w[(N + 1) / 2];
+};
+
+template <int N>
+__device__ __forceinline__ CwVec<N> cw_load(const unsigned short* p, bool vec) {
+    CwVec<N> v;
+    if constexpr (N == 1) {
+        v.w[0] = p[0];
+    } else if (vec) {
+        if constexpr (N == 8) {
+            const uint4 u = *reinterpret_cast<const uint4*>(p);
+            v.w[0] = u.x, v.w[1] = u.y, v.w[2] = u.z, v.w[3] = u.w;
+        } else if constexpr (N == 4) {
+            const uint2 u = *reinterpret_cast<const uint2*>(p);
+            v.w[0] = u.x, v.w[1] = u.y;
+        } else {
+            v.w[0] = *reinterpret_cast<const unsigned*>(p);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < N / 2; ++j) v.w[j] = p[2 * j] | ((unsigned)p[2 * j + 1] << 16);
+    }
+    return v;
+}
+
+// The largest pattern over the workgroup.
+template <int NW>
+__device__ __forceinline__ unsigned cw_block_max(unsigned amax, unsigned* wave_max) {
+    amax = max(amax & 0xffffu, amax >> 16);
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) amax = max(amax, (unsigned)__shfl_xor((int)amax, off));
+    if constexpr (NW > 1) {
+        __syncthreads();                                     // what was there before has been read
+        if ((threadIdx.x & 63) == 0) wave_max[threadIdx.x >> 6] = amax;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < NW; ++w) amax = max(amax, wave_max[w]);
+    }
+    return amax;
+}
+
+// Tokens x[0 .. count) of one head, for rows row0 .. row0 + count of the page half at dst.  NW waves.
+template <int DT, int D, int NW>
+__device__ __forceinline__ void cw_keys(const unsigned short* x, int64_t x_st, bool vec, int row0, int count,
+                                        unsigned char* dst, float* scale, unsigned* wave_max) {
+    constexpr int PER_ROW = D / 8, KEEP = PER_ROW / 4;       // 16 rows a wave in registers
+    const int tid = threadIdx.x, n = count * PER_ROW;
+    const auto load = [&](int e) { return cw_load<8>(x + (int64_t)(e / PER_ROW) * x_st + (e % PER_ROW) * 8, vec); };
+    CwVec<8> v[KEEP];
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i) v[i] = load(min(tid + i * NW * 64, n - 1));
+    const float old = row0 > 0 ? *scale : 0.f;
+    unsigned amax = 0;
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) amax = cw_max2(amax, v[i].w[j]);
+    for (int e = tid + KEEP * NW * 64; e < n; e += NW * 64) {            // a longer run: read again below
+        const CwVec<8> u = load(e);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) amax = cw_max2(amax, u.w[j]);
+    }
+    unsigned top = cw_block_max<NW>(amax, wave_max);
+    const bool odd = top >= CwInf<DT>::bits;                 // infinities or NaN: they do not count
+    if (odd) {
+        amax = 0;
+        for (int e = tid; e < n; e += NW * 64) {
+            const CwVec<8> u = load(e);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) amax = cw_max2(amax, cw_finite2<DT>(u.w[j]));
+        }
+        top = cw_block_max<NW>(amax, wave_max);
+    }
+    const float s = fmaxf(cw_scale(cw_lo<DT>(top)), old), inv = 1.0f / s;        // exact: s is a power of two
+    if (old < s && row0 > 0) {                               // older tokens of the page, under the larger scale
+        const float f = old * inv;
+        for (int e = tid; e < row0 * PER_ROW; e += NW * 64) {
+            uint2 w = *reinterpret_cast<const uint2*>(dst + e * 8);
+            w.x = pgn_fp8_rescale4(w.x, f);
+            w.y = pgn_fp8_rescale4(w.y, f);
+            *reinterpret_cast<uint2*>(dst + e * 8) = w;
+        }
+    }
+    const auto put = [&](int e, const CwVec<8>& u) {
+        unsigned w[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const float f0 = cw_lo<DT>(u.w[2 * j]) * inv, f1 = cw_hi<DT>(u.w[2 * j]) * inv;
+            const float f2 = cw_lo<DT>(u.w[2 * j + 1]) * inv, f3 = cw_hi<DT>(u.w[2 * j + 1]) * inv;
+            w[j] = odd ? pgn_fp8_pack4_any(f0, f1, f2, f3) : pgn_fp8_pack4(f0, f1, f2, f3);
+        }
+        *reinterpret_cast<uint2*>(dst + (int64_t)row0 * D + e * 8) = uint2{w[0], w[1]};
+    };
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i)
+        if (tid + i * NW * 64 < n) put(tid + i * NW * 64, v[i]);
+    for (int e = tid + KEEP * NW * 64; e < n; e += NW * 64) put(e, load(e));
+    if (NW > 1) __syncthreads();                             // every thread has read the old scale
+    if (tid == 0) *scale = s;
+}
+
+template <int DT, int D, int NW>
+__device__ __forceinline__ void cw_values(const unsigned short* x, int64_t x_st, bool vec, int row0, int count, int P,
+                                          unsigned char* dst, float* scale, unsigned* wave_max) {
+    constexpr int DV = D / 64, DW = (DV + 1) / 2;
+    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+    const int slab0 = row0 >> 4, slabs = ((row0 + count + 15) >> 4) - slab0;     // slabs of 16 page rows that the run touches
+    const auto row = [&](int slab, int j) { return (slab0 + slab) * 16 + j - row0; };    // token of the run, if in [0, count)
+    const auto load = [&](int slab, CwVec<DV>* u) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)                         // rows outside the run repeat one of it: no branch, same maximum
+            u[j] = cw_load<DV>(x + (int64_t)min(max(row(slab, j), 0), count - 1) * x_st + lane * DV, vec);
+    };
+    CwVec<DV> v[16];
+    if (wid < slabs) {
+        load(wid, v);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] = CwVec<DV>{};
+    }
+    const float old = row0 > 0 ? *scale : 0.f;
+    unsigned amax = 0;
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+#pragma unroll
+        for (int d = 0; d < DW; ++d) amax = cw_max2(amax, v[j].w[d]);
+    for (int slab = wid + NW; slab < slabs; slab += NW) {    // a longer run: read again below
+        CwVec<DV> u[16];
+        load(slab, u);
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+#pragma unroll
+            for (int d = 0; d < DW; ++d) amax = cw_max2(amax, u[j].w[d]);
+    }
+    unsigned top = cw_block_max<NW>(amax, wave_max);
+    const bool odd = top >= CwInf<DT>::bits;
+    if (odd) {
+        amax = 0;
+        for (int slab = wid; slab < slabs; slab += NW) {
+            CwVec<DV> u[16];
+            load(slab, u);
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+#pragma unroll
+                for (int d = 0; d < DW; ++d) amax = cw_max2(amax, cw_finite2<DT>(u[j].w[d]));
+        }
+        top = cw_block_max<NW>(amax, wave_max);
+    }
+    const float s = fmaxf(cw_scale(cw_lo<DT>(top)), old), inv = 1.0f / s;
+    if (old < s && row0 > 0) {
+        const float f = old * inv;
+        const int words = (row0 + 3) >> 2;                   // the last word may hold tokens behind row0: bytes there
+        for (int e = threadIdx.x; e < D * words; e += NW * 64) {
+            const int d = e / words, w = e - d * words;
+            unsigned char* p = dst + (int64_t)d * P + w * 4;
+            const unsigned is = pgn_fp8_rescale4(*reinterpret_cast<const unsigned*>(p), f);
+            if (w * 4 + 4 <= row0) {
+                *reinterpret_cast<unsigned*>(p) = is;
+            } else {
+                for (int j = 0; w * 4 + j < row0; ++j) p[j] = (unsigned char)(is >> (8 * j));
+            }
+        }
+    }
+    const auto put = [&](int slab, const CwVec<DV>* u) {
+        const bool whole = row(slab, 0) >= 0 && row(slab, 15) < count;
+#pragma unroll
+        for (int d = 0; d < DV; ++d) {
+            unsigned char* p = dst + (int64_t)(lane * DV + d) * P + (slab0 + slab) * 16;
+            unsigned w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float f[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) f[i] = (d & 1 ? cw_hi<DT>(u[4 * j + i].w[d / 2]) : cw_lo<DT>(u[4 * j + i].w[d / 2])) * inv;
+                w[j] = odd ? pgn_fp8_pack4_any(f[0], f[1], f[2], f[3]) : pgn_fp8_pack4(f[0], f[1], f[2], f[3]);
+            }
+            if (whole) {
+                *reinterpret_cast<uint4*>(p) = uint4{w[0], w[1], w[2], w[3]};
+            } else {
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    if (row(slab, j) >= 0 && row(slab, j) < count) p[j] = (unsigned char)(w[j / 4] >> (8 * (j % 4)));
+            }
+        }
+    };
+    if (wid < slabs) put(wid, v);
+    for (int slab = wid + NW; slab < slabs; slab += NW) {
+        CwVec<DV> u[16];
+        load(slab, u);
+        put(slab, u);
+    }
+    if (NW > 1) __syncthreads();
+    if (threadIdx.x == 0) *scale = s;
+}
+
+template <int DT, int D, int NW>
+__global__ __launch_bounds__(NW * 64) void pgn_cache_write_kernel(
     const unsigned short* __restrict__ k, const unsigned short* __restrict__ v, const int64_t* __restrict__ slots, int T,
-    int H, int D, int shift, int64_t N, int chunk, int64_t k_st, int64_t k_sh, int64_t v_st, int64_t v_sh, int k_vec,
-    int v_vec, unsigned char* __restrict__ k_pages, unsigned char* __restrict__ v_pages, float* __restrict__ k_scale,
-    float* __restrict__ v_scale) {
-    extern __shared__ unsigned char tile[];                  // values: [tokens of the run][D + 4] bytes
-    __shared__ float wave_max[PGN_CW_THREADS / 64];
-    const int tid = threadIdx.x, h = blockIdx.y;
-    const bool values = blockIdx.z != 0;
+    int H, int shift, int64_t N, int chunk, int64_t k_st, int64_t k_sh, int64_t v_st, int64_t v_sh, int k_vec, int v_vec,
+    unsigned char* k_pages, unsigned char* v_pages, float* k_scale, float* v_scale) {
+    __shared__ unsigned wave_max[NW];
+    // Workgroups go round the 8 XCDs.  One XCD takes all heads of a chunk, one after another: a token's heads lie side by
+    // side, and an XCD that read only every eighth of them would use few of its L2's channels.
+    const int lane = threadIdx.x & 63, xcd = blockIdx.x & 7, j = blockIdx.x >> 3, h = j % H;
     const int P = 1 << shift;
     const int64_t limit = N << shift;
-    const unsigned short* x = (values ? v + h * v_sh : k + h * k_sh);
-    const int64_t x_st = values ? v_st : k_st;
-    const bool vec = values ? v_vec : k_vec;
-    unsigned char* pages = values ? v_pages : k_pages;
-    float* scales = values ? v_scale : k_scale;
-    const int per_row = D >> 3;
 
     // which of the chunk's tokens begin a run: one lane a token, the same in every wave (chunk <= 64)
-    const int lane = tid & 63, t0 = blockIdx.x * chunk;
-    const bool mine = lane < chunk && t0 + lane < T;
-    const int64_t my_slot = mine ? slots[t0 + lane] : -1;
-    const int64_t my_before = mine && t0 + lane > 0 ? slots[t0 + lane - 1] : -2;
-    uint64_t runs = __ballot(my_slot >= 0 && my_slot < limit && ((my_slot & (P - 1)) == 0 || my_before != my_slot - 1));
+    const int t0 = (j / H * 8 + xcd) * chunk;                // may lie behind the last token: then nothing begins a run
+    const int64_t my_slot = t0 + lane < T ? slots[t0 + lane] : -1;
+    const int64_t next_slot = t0 + 64 + lane < T ? slots[t0 + 64 + lane] : -1;
+    int64_t my_before = __shfl_up(my_slot, 1);
+    if (lane == 0) my_before = t0 > 0 && t0 < T ? slots[t0 - 1] : -2;
+    uint64_t runs = __ballot(lane < chunk && my_slot >= 0 && my_slot < limit &&
+                             ((my_slot & (P - 1)) == 0 || my_before != my_slot - 1));
     for (; runs != 0; runs &= runs - 1) {                    // every bound here is the same for the whole workgroup
         const int first = __builtin_ctzll(runs), t = t0 + first;
         const int64_t slot = __shfl(my_slot, first);
-        const int row0 = (int)(slot & (P - 1));
-        int count = 0;                                       // tokens of the run: up to the page's end, 64 at a time
-        for (int c = 0; c < P - row0; c += 64) {
-            const int i = c + lane;
-            const uint64_t on = __ballot(i < P - row0 && t + i < T && slots[t + i] == slot + i);
-            const int n = ~on == 0 ? 64 : __builtin_ctzll(~on);
-            count += n;
-            if (n < 64) break;
+        const int row0 = (int)(slot & (P - 1)), most = P - row0;
+        // tokens of the run, up to the page's end: among the 128 that the lanes hold, then 64 at a time
+        uint64_t on = ~__ballot(lane >= first && lane - first < most && my_slot == slot + (lane - first)) >> first;
+        int count = on == 0 ? 64 - first : __builtin_ctzll(on);
+        for (int c = 64 - first; count == c && c < most; c += 64) {
+            const int64_t sl = c == 64 - first ? next_slot : t + c + lane < T ? slots[t + c + lane] : -1;
+            on = ~__ballot(c + lane < most && sl == slot + (c + lane));
+            count += on == 0 ? 64 : __builtin_ctzll(on);
         }
-        const int64_t page = slot >> shift;
-        unsigned char* dst = pages + (page * H + h) * (int64_t)P * D;
-
-        float amax = 0.f;
-        for (int e = tid; e < count * per_row; e += PGN_CW_THREADS) {
-            const int i = e / per_row, c = (e - i * per_row) * 8;
-            float f[8];
-            cw_load8<DT>(x + (int64_t)(t + i) * x_st + c, vec, f);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float a = fabsf(f[j]);
-                amax = a < INFINITY ? fmaxf(amax, a) : amax;  // infinities and NaN do not count
-            }
-        }
-#pragma unroll
-        for (int off = 32; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor(amax, off));
-        if ((tid & 63) == 0) wave_max[tid >> 6] = amax;
-        const float old = row0 > 0 ? scales[page * H + h] : 0.f;
-        __syncthreads();
-        amax = fmaxf(fmaxf(wave_max[0], wave_max[1]), fmaxf(wave_max[2], wave_max[3]));
-        const float s = fmaxf(cw_scale(amax), old);          // a stored NaN loses against the new scale
-        const float inv = 1.0f / s;                          // exact: s is a power of two
-
-        if (row0 > 0 && old < s) {                           // older tokens of the page, under the larger scale
-            const float f = old * inv;
-            if (!values) {
-                for (int e = tid; e < row0 * per_row; e += PGN_CW_THREADS) {
-                    uint2 w = *reinterpret_cast<const uint2*>(dst + e * 8);
-                    w.x = pgn_fp8_rescale4(w.x, f);
-                    w.y = pgn_fp8_rescale4(w.y, f);
-                    *reinterpret_cast<uint2*>(dst + e * 8) = w;
-                }
-            } else {
-                const int words = (row0 + 3) >> 2;           // the last word may hold tokens behind row0: bytes there
-                for (int e = tid; e < D * words; e += PGN_CW_THREADS) {
-                    const int d = e / words, w = e - d * words;
-                    unsigned char* p = dst + (int64_t)d * P + w * 4;
-                    const unsigned was = *reinterpret_cast<const unsigned*>(p), is = pgn_fp8_rescale4(was, f);
-                    if (w * 4 + 4 <= row0) {
-                        *reinterpret_cast<unsigned*>(p) = is;
-                    } else {
-                        for (int j = 0; w * 4 + j < row0; ++j) p[j] = (unsigned char)(is >> (8 * j));
-                    }
-                }
-            }
-        }
-
-        for (int e = tid; e < count * per_row; e += PGN_CW_THREADS) {
-            const int i = e / per_row, c = (e - i * per_row) * 8;
-            float f[8];
-            cw_load8<DT>(x + (int64_t)(t + i) * x_st + c, vec, f);
-            uint2 w;
-            w.x = pgn_fp8_pack4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv);
-            w.y = pgn_fp8_pack4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv);
-            if (!values) {
-                *reinterpret_cast<uint2*>(dst + (int64_t)(row0 + i) * D + c) = w;
-            } else {
-                *reinterpret_cast<unsigned*>(tile + i * (D + 4) + c) = w.x;
-                *reinterpret_cast<unsigned*>(tile + i * (D + 4) + c + 4) = w.y;
-            }
-        }
-        __syncthreads();                                     // the tile is whole; every thread has read the old scale
-        if (values) {
-            const int w0 = row0 >> 2, words = ((row0 + count + 3) >> 2) - w0;
-            for (int e = tid; e < D * words; e += PGN_CW_THREADS) {
-                const int w = e / D, d = e - w * D;
-                const int r = (w0 + w) * 4;                  // tokens r .. r + 3 of the page, one word
-                unsigned char* p = dst + (int64_t)d * P + r;
-                if (r >= row0 && r + 4 <= row0 + count) {
-                    unsigned word = 0;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) word |= (unsigned)tile[(r - row0 + j) * (D + 4) + d] << (8 * j);
-                    *reinterpret_cast<unsigned*>(p) = word;
-                } else {
-                    for (int j = 0; j < 4; ++j)
-                        if (r + j >= row0 && r + j < row0 + count) p[j] = tile[(r - row0 + j) * (D + 4) + d];
-                }
-            }
-        }
-        if (tid == 0) scales[page * H + h] = s;
-        __syncthreads();                                     // the tile and wave_max are used again
+        const int64_t page = slot >> shift, half = (page * H + h) * (int64_t)P * D;
+        if (blockIdx.y == 0)
+            cw_keys<DT, D, NW>(k + (int64_t)t * k_st + h * k_sh, k_st, k_vec, row0, count, k_pages + half,
+                               k_scale + page * H + h, wave_max);
+        else
+            cw_values<DT, D, NW>(v + (int64_t)t * v_st + h * v_sh, v_st, v_vec, row0, count, P, v_pages + half,
+                                 v_scale + page * H + h, wave_max);
     }
 }
 
@@ -374,8 +525,13 @@ extern "C" int pgn_page_advance(int32_t* lens, const int32_t* keep, const int32_
     if (((int64_t)W << shift) > 0x7fffffff || (int64_t)W * PGN_ADV_THREADS > 0x7fffffff) return PGN_ERR_UNSUPPORTED;
     hipStream_t s = (hipStream_t)stream;
     const int T = (int)num_slots, fused = T <= PGN_ADV_FUSED_SLOTS;
-    hipLaunchKernelGGL(pgn_page_advance_kernel, dim3(1), dim3(PGN_ADV_THREADS), 0, s, lens, keep, add, table,
-                       table_stride, free_pages, free_count, num_pages, R, W, shift, T, fused, slots, starts, status);
+#define PGN_ADV_LAUNCH(NT)                                                                                             \
+    hipLaunchKernelGGL((pgn_page_advance_kernel<NT>), dim3(1), dim3(NT), 0, s, lens, keep, add, table, table_stride,   \
+                       free_pages, free_count, num_pages, R, W, shift, T, fused, slots, starts, status)
+    if (R <= 64 && T <= 512) PGN_ADV_LAUNCH(64);
+    else if (R <= 256 && T <= 2048) PGN_ADV_LAUNCH(256);
+    else PGN_ADV_LAUNCH(PGN_ADV_THREADS);
+#undef PGN_ADV_LAUNCH
     PGN_LAUNCH_CHECK();
     if (!fused) {
         hipLaunchKernelGGL(pgn_page_slots_kernel, dim3((T + 1023) / 1024), dim3(256), 0, s, lens, table, table_stride, R,
@@ -400,21 +556,38 @@ extern "C" int pgn_cache_write(const void* k, const void* v, int dtype, const in
         return PGN_ERR_UNSUPPORTED;
     if (!pgn_aligned(k, 2) || !pgn_aligned(v, 2) || !pgn_aligned(k_pages, 16) || !pgn_aligned(v_pages, 16))
         return PGN_ERR_INVALID;
+    // keys are read 16 bytes at a time, values head_dim / 64 elements
+    const int dv = head_dim / 64;
     const int k_vec = pgn_aligned(k, 16) && k_st % 8 == 0 && k_sh % 8 == 0;
-    const int v_vec = pgn_aligned(v, 16) && v_st % 8 == 0 && v_sh % 8 == 0;
-    const int T = (int)num_tokens, D = head_dim;
-    // One token a workgroup while the launch is small (a decoding step: every token is a run of its own and latency
-    // counts), 16 above: most tokens then lie inside a run and only cost a look at the slot map.
-    const int chunk = T <= 2048 ? 1 : 16;
-    const dim3 grid((T + chunk - 1) / chunk, kv_heads, 2), block(PGN_CW_THREADS);
-    const size_t lds = (size_t)page_size * (D + 4);          // <= 128 * 260 bytes
+    const int v_vec = pgn_aligned(v, 2 * dv) && v_st % dv == 0 && v_sh % dv == 0;
+    const int T = (int)num_tokens;
+    // A decoding step (every token a run of its own, latency counts): one token and one wave a workgroup.  Above that,
+    // four waves and 16 tokens, or 64 where that still makes 1024 workgroups: most tokens lie inside a run that began
+    // before, and a workgroup without a run costs its look at the slot map all the same.
+    const bool few = T <= 2048;
+    const int chunk = few ? 1 : ((int64_t)T * kv_heads >= 64 * 1024 ? 64 : 16);
+    const int64_t wgs = (int64_t)(((T + chunk - 1) / chunk + 7) / 8 * 8) * kv_heads;
+    if (wgs > 0x7fffffff) return PGN_ERR_UNSUPPORTED;
+    const dim3 grid((unsigned)wgs, 2);
     hipStream_t s = (hipStream_t)stream;
-#define PGN_CW_LAUNCH(DT)                                                                                              \
-    hipLaunchKernelGGL((pgn_cache_write_kernel<DT>), grid, block, lds, s, (const unsigned short*)k,                    \
-                       (const unsigned short*)v, slots, T, kv_heads, D, shift, (int64_t)num_pages, chunk, k_st, k_sh,  \
-                       v_st, v_sh, k_vec, v_vec, (unsigned char*)k_pages, (unsigned char*)v_pages, k_scale, v_scale)
-    if (dtype == PGN_BF16) PGN_CW_LAUNCH(PGN_BF16);
-    else PGN_CW_LAUNCH(PGN_F16);
+#define PGN_CW_LAUNCH(DT, D, NW)                                                                                       \
+    hipLaunchKernelGGL((pgn_cache_write_kernel<DT, D, NW>), grid, dim3(NW * 64), 0, s, (const unsigned short*)k,       \
+                       (const unsigned short*)v, slots, T, kv_heads, shift, (int64_t)num_pages, chunk, k_st, k_sh, v_st, \
+                       v_sh, k_vec, v_vec, (unsigned char*)k_pages, (unsigned char*)v_pages, k_scale, v_scale)
+#define PGN_CW_DIMS(DT, NW)                                                                                            \
+    do {                                                                                                               \
+        if (head_dim == 64) PGN_CW_LAUNCH(DT, 64, NW);                                                                 \
+        else if (head_dim == 128) PGN_CW_LAUNCH(DT, 128, NW);                                                          \
+        else PGN_CW_LAUNCH(DT, 256, NW);                                                                               \
+    } while (0)
+    if (dtype == PGN_BF16) {
+        if (few) PGN_CW_DIMS(PGN_BF16, 1);
+        else PGN_CW_DIMS(PGN_BF16, 4);
+    } else {
+        if (few) PGN_CW_DIMS(PGN_F16, 1);
+        else PGN_CW_DIMS(PGN_F16, 4);
+    }
+#undef PGN_CW_DIMS
 #undef PGN_CW_LAUNCH
     PGN_LAUNCH_CHECK();
     return PGN_OK;

@@ -4,6 +4,7 @@ Every function takes CUDA(HIP) tensors, enqueues on torch's current stream and r
 allocated through torch's caching allocator.  Nothing here computes on the CPU and nothing falls back to
 a PyTorch implementation: non-device tensors or unsupported shapes raise.
 """
+import functools
 import os
 from typing import List, Optional, Sequence, Tuple, Union
 
@@ -761,14 +762,21 @@ def _on(*ts):
 
 
 def _call(dev, what, fn, *args):
-    """fn(*args, stream) on `dev`, which need not be the current device."""
-    if dev.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    """fn(*args, stream) on `dev`, which need not be the current device.  The stream is asked for by its handle alone:
+    these calls take a few microseconds on the GPU, and a torch.cuda.Stream object takes four to make."""
+    index = dev.index
+    if index == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc:
         _lib.check(rc, what)
+
+
+@functools.lru_cache(maxsize=256)
+def _cached_attention_bytes(*sizes) -> int:
+    return _lib.load().pgn_cached_attention_workspace_bytes(*sizes)
 
 
 def _i32(t: torch.Tensor, shape, name: str):
@@ -885,7 +893,7 @@ def cached_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
         if q.data_ptr() % 16:
             q = q.clone()
     packed = starts is not None
-    nbytes = lib.pgn_cached_attention_workspace_bytes(T, R, packed, Hq, H, D, W, P)
+    nbytes = _cached_attention_bytes(T, R, packed, Hq, H, D, W, P)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     scale = float(D) ** -0.5 if scale is None else float(scale)
 
