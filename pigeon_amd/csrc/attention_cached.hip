@@ -137,18 +137,19 @@ __device__ __forceinline__ bool few_rows_tile(const CachedArgs& a, int tile, Til
     return t.count > 0;
 }
 
+template <int ROWS>
 __device__ __forceinline__ bool many_rows_tile(const CachedArgs& a, int tile, TileRows& t) {
     int lo = 0, hi = a.R;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if ((int64_t)a.starts[mid] * a.G / 128 + mid <= tile) lo = mid;
+        if ((int64_t)a.starts[mid] * a.G / ROWS + mid <= tile) lo = mid;
         else hi = mid;
     }
     if (!request_rows(a, lo, t) || t.n * a.G <= PGN_CA_FEW_ROWS) return false;
-    const int64_t local = tile - ((int64_t)t.begin * a.G / 128 + lo);
-    if (local < 0 || local * 128 >= t.n * a.G) return false;
-    t.first = (int)local * 128;
-    t.count = min(128, t.n * a.G - t.first);
+    const int64_t local = tile - ((int64_t)t.begin * a.G / ROWS + lo);
+    if (local < 0 || local * ROWS >= t.n * a.G) return false;
+    t.first = (int)local * ROWS;
+    t.count = min(ROWS, t.n * a.G - t.first);
     return true;
 }
 
@@ -379,9 +380,15 @@ __global__ __launch_bounds__(PGN_CA_THREADS) void pgn_cached_rows16_kernel(const
 //
 // Keys are stored in the row order in which the 32x32 result hands its rows to lanes: row b + 4 h + 8 a of a half tile is
 // key 16 h + 4 a + b, so a lane ends up with 16 consecutive keys of its query and the probabilities are, without any
-// exchange, the second operand of O^T = V^T P^T.  16-byte units of a row are permuted by its low three bits, which
-// spreads the operand loads over the banks.
+// exchange, the second operand of O^T = V^T P^T.
 // The running maximum moves only when it has to: probabilities may grow to 2^8 before the accumulator is rescaled.
+// The 16-byte units of a row are permuted by its number, so that 16 lanes that read one unit of 16 rows meet all 64 banks:
+// rows of 128 bytes take two to go round them.
+template <int ROW>
+__device__ __forceinline__ int key_swizzle(int row) {
+    return ROW == 64 ? (row >> 1) & 7 : row & 15;
+}
+
 template <int DT, int D>
 struct BigTile {
     unsigned short k[64 * D];
@@ -393,19 +400,20 @@ struct BigLds {
     BigTile<DT, D> tile[2];
     float ks[2][4], raise[2][4], pscale[2][4], ref[2];
     int nan[2][4], live[2][4];
+    unsigned short nans[2][4][D];                            // of each chunk and head dim: which of its 16 values are NaN
 };
 
 template <int DT, int D>
 __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void pgn_cached_rows128_kernel(const CachedArgs a) {
     typedef typename Mat<DT>::v8 v8;
-    constexpr int L = D / 64, KS = D / 16, DTILES = D / 32, UNITS = D / 8;
+    constexpr int L = D / 64, KS = D / 16, DTILES = D / 32;
     extern __shared__ unsigned char smem_big[];
     BigLds<DT, D>& s = *reinterpret_cast<BigLds<DT, D>*>(smem_big);
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hf = lane >> 5, col = lane & 31;
     const int h = blockIdx.x % a.Hkv, split = blockIdx.y;    // heads fastest: a head's tiles share one XCD's L2
     TileRows t;
-    if (!many_rows_tile(a, a.big_tiles - 1 - (int)(blockIdx.x / a.Hkv), t)) return;     // a request's longest rows first
+    if (!many_rows_tile<128>(a, a.big_tiles - 1 - (int)(blockIdx.x / a.Hkv), t)) return;     // a request's longest rows first
     int lo, hi;
     key_range(a, t, lo, hi);
     const int kb = (lo & ~63) + split * a.big_split_keys;
@@ -460,11 +468,11 @@ __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void pgn_cached_rows128_ke
         const int page = table[min(key >> a.shift, a.W - 1)];
         good = key < hi && key + 16 > lo && (unsigned)page < (unsigned)a.N;
         const int64_t at = (int64_t)(good ? page : 0) * a.Hkv + h;
-        const unsigned char* kp = a.k_pages + (at * P + (key & (P - 1)) + (lane >> 2)) * D + (lane & 3) * (D / 4);
+        const unsigned char* kp = a.k_pages + (at * P + (key & (P - 1)) + (lane >> 2)) * D + (lane & 3) * 16;
         const unsigned char* vp = a.v_pages + (at * D + lane) * P + (key & (P - 1));
 #pragma unroll
         for (int i = 0; i < L; ++i) {
-            kw[i] = good ? *reinterpret_cast<const uint4*>(kp + i * 16) : uint4{0, 0, 0, 0};
+            kw[i] = good ? *reinterpret_cast<const uint4*>(kp + i * 64) : uint4{0, 0, 0, 0};
             vw[i] = good ? *reinterpret_cast<const uint4*>(vp + (int64_t)i * 64 * P) : uint4{0, 0, 0, 0};
         }
         ks = good ? a.k_scale[at] : 1.f;
@@ -486,9 +494,9 @@ __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void pgn_cached_rows128_ke
         unsigned short* kp = tile.k + (32 * (wid >> 1) + mrow) * D;
 #pragma unroll
         for (int i = 0; i < L; ++i) {
-            const int u = (lane & 3) * (UNITS / 4) + i * 2;
-            *reinterpret_cast<v8*>(kp + ((u ^ (mrow & 7)) * 8)) = widen8<DT>(kw[i].x, kw[i].y, 1.f);
-            *reinterpret_cast<v8*>(kp + (((u + 1) ^ (mrow & 7)) * 8)) = widen8<DT>(kw[i].z, kw[i].w, 1.f);
+            const int u = (lane & 3) * 2 + i * 8;
+            *reinterpret_cast<v8*>(kp + ((u ^ key_swizzle<D>(mrow)) * 8)) = widen8<DT>(kw[i].x, kw[i].y, 1.f);
+            *reinterpret_cast<v8*>(kp + (((u + 1) ^ key_swizzle<D>(mrow)) * 8)) = widen8<DT>(kw[i].z, kw[i].w, 1.f);
         }
         float vmul = 1.f, raise = 0.f, pscale = 1.f, vscale;
         if constexpr (DT == PGN_F16) {                       // as in the 16-row kernel, raised by 2^7: maxima lag by 2^8
@@ -520,14 +528,32 @@ __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void pgn_cached_rows128_ke
             }
         }
 #pragma unroll
+        for (int i = 0; i < L; ++i)
+            bad |= nan_bytes(vw[i].x) | nan_bytes(vw[i].y) | nan_bytes(vw[i].z) | nan_bytes(vw[i].w);
+        const bool any_nan = __any(bad != 0);
+        if (any_nan) {
+            // A NaN value must reach the rows that see it and no other, but 0 * NaN would reach all.  It is kept apart as
+            // a bit, and counts as 0 in the product.
+#pragma unroll
+            for (int i = 0; i < L; ++i) {
+                unsigned bits = 0;
+                unsigned* w = reinterpret_cast<unsigned*>(&vw[i]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const unsigned f = nan_bytes(w[j]) >> 7;          // 0x01 in the NaN bytes
+                    w[j] &= ~(f * 0xffu);
+                    bits |= (((f * 0x01020408u) >> 24) & 15u) << (4 * j);         // byte n -> bit n
+                }
+                s.nans[buf][wid][lane + 64 * i] = (unsigned short)bits;
+            }
+        }
+#pragma unroll
         for (int i = 0; i < L; ++i) {
             const int d = lane + 64 * i;
-            bad |= nan_bytes(vw[i].x) | nan_bytes(vw[i].y) | nan_bytes(vw[i].z) | nan_bytes(vw[i].w);
             unsigned short* vp = tile.v + d * 64;
-            *reinterpret_cast<v8*>(vp + (((2 * wid) ^ (d & 7)) * 8)) = widen8<DT>(vw[i].x, vw[i].y, vmul);
-            *reinterpret_cast<v8*>(vp + (((2 * wid + 1) ^ (d & 7)) * 8)) = widen8<DT>(vw[i].z, vw[i].w, vmul);
+            *reinterpret_cast<v8*>(vp + (((2 * wid) ^ key_swizzle<64>(d)) * 8)) = widen8<DT>(vw[i].x, vw[i].y, vmul);
+            *reinterpret_cast<v8*>(vp + (((2 * wid + 1) ^ key_swizzle<64>(d)) * 8)) = widen8<DT>(vw[i].z, vw[i].w, vmul);
         }
-        const bool any_nan = __any(bad != 0);
         if (lane == 0) {
             s.ks[buf][wid] = fmaxf(ks * c, 0x1p-126f);       // 0 would turn a masked -inf into NaN
             s.raise[buf][wid] = raise;
@@ -556,7 +582,8 @@ __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void pgn_cached_rows128_ke
                 const unsigned short* kp = tile.k + (32 * kt + col) * D;
 #pragma unroll
                 for (int i = 0; i < KS; ++i)
-                    x[kt] = Mat<DT>::mfma32(*reinterpret_cast<const v8*>(kp + (((2 * i + hf) ^ (col & 7)) * 8)), qf[i], x[kt]);
+                    x[kt] = Mat<DT>::mfma32(*reinterpret_cast<const v8*>(kp + (((2 * i + hf) ^ key_swizzle<D>(col)) * 8)),
+                                              qf[i], x[kt]);
             }
             const bool whole = base >= all_lo && base + 64 <= all_hi &&
                                (s.live[buf][0] & s.live[buf][1] & s.live[buf][2] & s.live[buf][3]);
@@ -620,7 +647,6 @@ __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void pgn_cached_rows128_ke
                 sum1 *= s.pscale[buf][2 + hf];
             }
             l += sum0 + sum1;
-            const bool nans = !whole && (s.nan[buf][0] | s.nan[buf][1] | s.nan[buf][2] | s.nan[buf][3]);
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
@@ -631,27 +657,24 @@ __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void pgn_cached_rows128_ke
 #pragma unroll
                     for (int d = 0; d < DTILES; ++d) {
                         const unsigned short* vp = tile.v + (32 * d + col) * 64;
-                        v8 v = *reinterpret_cast<const v8*>(vp + (((4 * kt + 2 * hf + half) ^ (col & 7)) * 8));
-                        if (nans) {                          // as in the 16-row kernel: NaN values by a product of their own
-                            v8 is, see;
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) {
-                                const int key = base + 32 * kt + 16 * hf + 8 * half + j;
-                                const bool n = v[j] != v[j];
-                                is[j] = Mat<DT>::one(n ? 1.f : 0.f);
-                                v[j] = n ? Mat<DT>::one(0.f) : v[j];
-                                see[j] = Mat<DT>::one(s.live[buf][2 * kt + hf] && key >= vis_lo && key < vis_hi ? 1.f : 0.f);
-                            }
-                            f32x16_t hit;
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) hit[i] = 0.f;
-                            hit = Mat<DT>::mfma32(is, see, hit);
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) o[d][i] = hit[i] > 0.f ? NAN : o[d][i];
-                        }
-                        o[d] = Mat<DT>::mfma32(v, p, o[d]);
+                        o[d] = Mat<DT>::mfma32(*reinterpret_cast<const v8*>(vp + (((4 * kt + 2 * hf + half) ^ key_swizzle<64>(col)) * 8)), p, o[d]);
                     }
                 }
+            if (s.nan[buf][0] | s.nan[buf][1] | s.nan[buf][2] | s.nan[buf][3]) {
+                for (int w = 0; w < 4; ++w) {
+                    if (!s.nan[buf][w]) continue;
+                    unsigned see = 0;                        // of the chunk's keys
+                    for (int i = 0; i < 16; ++i) {
+                        const int key = base + 16 * w + i;
+                        see |= key >= vis_lo && key < vis_hi ? 1u << i : 0u;
+                    }
+#pragma unroll
+                    for (int d = 0; d < DTILES; ++d)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            o[d][i] = see & s.nans[buf][w][32 * d + 8 * (i >> 2) + 4 * hf + (i & 3)] ? NAN : o[d][i];
+                }
+            }
         }
         if (more) store(base + 64, buf ^ 1);
         __syncthreads();
@@ -698,16 +721,16 @@ __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void pgn_cached_rows128_ke
 // Joins the splits of the rows of one kernel's tiles, a wave a row, four rows a workgroup.  Each lane takes one split's
 // maximum and sum (64 splits at most), so that every weight is known before the first partial output is read and the
 // reads do not wait for one another.
-template <int DT, int D, bool MANY>
+template <int DT, int D, int ROWS>
 __global__ __launch_bounds__(PGN_CA_THREADS) void pgn_cached_join_kernel(const CachedArgs a) {
     constexpr int E = D / 64;
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     TileRows t;
     const int h = blockIdx.x % a.Hkv, tile = blockIdx.x / a.Hkv;
-    if (!(MANY ? many_rows_tile(a, tile, t) : few_rows_tile(a, tile, t))) return;
+    if (!(ROWS > 16 ? many_rows_tile<ROWS>(a, tile, t) : few_rows_tile(a, tile, t))) return;
     const int rr = blockIdx.y * 4 + wid;
     if (rr >= t.count) return;
-    const int nsplit = MANY ? a.big_nsplit : a.nsplit;
+    const int nsplit = ROWS > 16 ? a.big_nsplit : a.nsplit;
     const int rw = t.first + rr, tok = t.begin + rw / a.G, hd = h * a.G + rw % a.G;
     const int64_t row = (int64_t)tok * a.Hq + hd, step = (int64_t)a.T * a.Hq;
     const float2 ml = lane < nsplit ? a.part_ml[lane * step + row] : make_float2(-INFINITY, 0.f);
@@ -870,9 +893,9 @@ extern "C" int pgn_cached_attention(const void* q, int dtype, const void* k_page
                           dim3(Hkv * p.big_tiles, p.big_nsplit));                                                      \
         PGN_CA_KERNEL((pgn_cached_rows16_kernel<DT, D>), (size_t)4 * 16 * D * 4, dim3(Hkv * p.tiles, p.nsplit));       \
         if (p.nsplit > 1)                                                                                              \
-            PGN_CA_KERNEL((pgn_cached_join_kernel<DT, D, false>), 0, dim3(Hkv * p.tiles, 4));                          \
+            PGN_CA_KERNEL((pgn_cached_join_kernel<DT, D, 16>), 0, dim3(Hkv * p.tiles, 4));                          \
         if (p.big_nsplit > 1)                                                                                          \
-            PGN_CA_KERNEL((pgn_cached_join_kernel<DT, D, true>), 0, dim3(Hkv * p.big_tiles, 32));                      \
+            PGN_CA_KERNEL((pgn_cached_join_kernel<DT, D, 128>), 0, dim3(Hkv * p.big_tiles, 32));                       \
     } while (0)
 #define PGN_CA_DIMS(DT)                                                                                                \
     do {                                                                                                               \
