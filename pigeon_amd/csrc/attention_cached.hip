@@ -381,7 +381,8 @@ __global__ __launch_bounds__(PGN_CA_THREADS) void pgn_cached_rows16_kernel(const
 // Keys are stored in the row order in which the 32x32 result hands its rows to lanes: row b + 4 h + 8 a of a half tile is
 // key 16 h + 4 a + b, so a lane ends up with 16 consecutive keys of its query and the probabilities are, without any
 // exchange, the second operand of O^T = V^T P^T.
-// The running maximum moves only when it has to: probabilities may grow to 2^8 before the accumulator is rescaled.
+// The reference that probabilities are taken against is not the running maximum: it stays as long as a lane's sum of
+// probabilities says that none is above 2^8, so the common path takes no maximum and rescales nothing.
 // The 16-byte units of a row are permuted by its number, so that 16 lanes that read one unit of 16 rows meet all 64 banks:
 // rows of 128 bytes take two to go round them.
 template <int ROW>
@@ -458,29 +459,31 @@ __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void pgn_cached_rows128_ke
 
     const int* table = a.table + t.r * a.table_stride;
     const int P = 1 << a.shift;
+    const int chunk = wid;                                   // of 16 keys of a tile, which the wave fetches
     uint4 kw[L], vw[L];
     float ks = 0.f, vs[4];
     bool good = false;
+    const auto page_at = [&](int key) { return table[min(key >> a.shift, a.W - 1)]; };
+    int page = page_at(kb + 16 * chunk);                     // of the tile that is fetched next, looked up one tile ahead
 
     // bytes of the wave's chunk of the tile at `base`, and the scales of the tile
     auto fetch = [&](int base) {
-        const int key = base + 16 * wid;
-        const int page = table[min(key >> a.shift, a.W - 1)];
+        const int key = base + 16 * chunk;
         good = key < hi && key + 16 > lo && (unsigned)page < (unsigned)a.N;
         const int64_t at = (int64_t)(good ? page : 0) * a.Hkv + h;
+        page = page_at(key + 64);
         const unsigned char* kp = a.k_pages + (at * P + (key & (P - 1)) + (lane >> 2)) * D + (lane & 3) * 16;
+#pragma unroll
+        for (int i = 0; i < L; ++i) kw[i] = *reinterpret_cast<const uint4*>(kp + i * 64);
+        ks = good ? a.k_scale[at] : 1.f;
         const unsigned char* vp = a.v_pages + (at * D + lane) * P + (key & (P - 1));
 #pragma unroll
-        for (int i = 0; i < L; ++i) {
-            kw[i] = good ? *reinterpret_cast<const uint4*>(kp + i * 64) : uint4{0, 0, 0, 0};
-            vw[i] = good ? *reinterpret_cast<const uint4*>(vp + (int64_t)i * 64 * P) : uint4{0, 0, 0, 0};
-        }
-        ks = good ? a.k_scale[at] : 1.f;
+        for (int i = 0; i < L; ++i) vw[i] = *reinterpret_cast<const uint4*>(vp + (int64_t)i * 64 * P);
         if constexpr (DT == PGN_F16) {
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-                const int kw_ = base + 16 * w, pw = table[min(kw_ >> a.shift, a.W - 1)];
-                const bool gw = kw_ < hi && kw_ + 16 > lo && (unsigned)pw < (unsigned)a.N;
+                const int wkey = base + 16 * w, pw = page_at(wkey);
+                const bool gw = wkey < hi && wkey + 16 > lo && (unsigned)pw < (unsigned)a.N;
                 vs[w] = gw ? a.v_scale[(int64_t)pw * a.Hkv + h] : 0.f;
             }
         } else {
@@ -490,19 +493,23 @@ __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void pgn_cached_rows128_ke
     float store_ref = 0.f;
     auto store = [&](int base, int buf) {
         BigTile<DT, D>& tile = s.tile[buf];
-        const int key = lane >> 2, mrow = (key & 3) + 4 * (wid & 1) + 8 * (key >> 2);
-        unsigned short* kp = tile.k + (32 * (wid >> 1) + mrow) * D;
+        const int key = lane >> 2, mrow = (key & 3) + 4 * (chunk & 1) + 8 * (key >> 2);
+        unsigned short* kp = tile.k + (32 * (chunk >> 1) + mrow) * D;
 #pragma unroll
         for (int i = 0; i < L; ++i) {
             const int u = (lane & 3) * 2 + i * 8;
             *reinterpret_cast<v8*>(kp + ((u ^ key_swizzle<D>(mrow)) * 8)) = widen8<DT>(kw[i].x, kw[i].y, 1.f);
             *reinterpret_cast<v8*>(kp + (((u + 1) ^ key_swizzle<D>(mrow)) * 8)) = widen8<DT>(kw[i].z, kw[i].w, 1.f);
         }
+        if (lane == 0) {
+            s.ks[buf][chunk] = fmaxf(ks * c, 0x1p-126f); // 0 would turn a masked -inf into NaN
+            s.live[buf][chunk] = good;
+        }
         float vmul = 1.f, raise = 0.f, pscale = 1.f, vscale;
-        if constexpr (DT == PGN_F16) {                       // as in the 16-row kernel, raised by 2^7: maxima lag by 2^8
+        if constexpr (DT == PGN_F16) {                   // as in the 16-row kernel, raised by 2^7: probabilities reach 2^8
             vscale = vs[0];
 #pragma unroll
-            for (int w = 1; w < 4; ++w) vscale = wid == w ? vs[w] : vscale;
+            for (int w = 1; w < 4; ++w) vscale = chunk == w ? vs[w] : vscale;
             store_ref = fmaxf(store_ref, fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3])));
             const float ratio = good ? fmaxf(vscale / store_ref, 0x1p-60f) : 1.f;
             vmul = fmaxf(ratio, 0x1p-15f);
@@ -513,8 +520,7 @@ __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void pgn_cached_rows128_ke
             vmul = good ? vscale : 1.f;
         }
         // bytes that no row sees may hold anything: they count as 0, as do those of a page whose scale is 0
-        const int vkey = base + 16 * wid;
-        unsigned bad = 0;
+        const int vkey = base + 16 * chunk;
         if (vkey < lo || vkey + 16 > hi || vscale == 0.f) {
             const bool give = good && vscale != 0.f;
             const unsigned b0 = give ? key_bytes(vkey, 0, lo, hi) : 0u, b1 = give ? key_bytes(vkey, 1, lo, hi) : 0u;
@@ -527,39 +533,38 @@ __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void pgn_cached_rows128_ke
                 vw[i].w &= b3;
             }
         }
+        unsigned bad = 0;
 #pragma unroll
         for (int i = 0; i < L; ++i)
             bad |= nan_bytes(vw[i].x) | nan_bytes(vw[i].y) | nan_bytes(vw[i].z) | nan_bytes(vw[i].w);
         const bool any_nan = __any(bad != 0);
         if (any_nan) {
-            // A NaN value must reach the rows that see it and no other, but 0 * NaN would reach all.  It is kept apart as
-            // a bit, and counts as 0 in the product.
+            // A NaN value must reach the rows that see it and no other, but 0 * NaN would reach all.  It is kept
+            // apart as a bit, and counts as 0 in the product.
 #pragma unroll
             for (int i = 0; i < L; ++i) {
                 unsigned bits = 0;
                 unsigned* w = reinterpret_cast<unsigned*>(&vw[i]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const unsigned f = nan_bytes(w[j]) >> 7;          // 0x01 in the NaN bytes
+                    const unsigned f = nan_bytes(w[j]) >> 7;      // 0x01 in the NaN bytes
                     w[j] &= ~(f * 0xffu);
-                    bits |= (((f * 0x01020408u) >> 24) & 15u) << (4 * j);         // byte n -> bit n
+                    bits |= (((f * 0x01020408u) >> 24) & 15u) << (4 * j);     // byte n -> bit n
                 }
-                s.nans[buf][wid][lane + 64 * i] = (unsigned short)bits;
+                s.nans[buf][chunk][lane + 64 * i] = (unsigned short)bits;
             }
         }
 #pragma unroll
         for (int i = 0; i < L; ++i) {
             const int d = lane + 64 * i;
             unsigned short* vp = tile.v + d * 64;
-            *reinterpret_cast<v8*>(vp + (((2 * wid) ^ key_swizzle<64>(d)) * 8)) = widen8<DT>(vw[i].x, vw[i].y, vmul);
-            *reinterpret_cast<v8*>(vp + (((2 * wid + 1) ^ key_swizzle<64>(d)) * 8)) = widen8<DT>(vw[i].z, vw[i].w, vmul);
+            *reinterpret_cast<v8*>(vp + (((2 * chunk) ^ key_swizzle<64>(d)) * 8)) = widen8<DT>(vw[i].x, vw[i].y, vmul);
+            *reinterpret_cast<v8*>(vp + (((2 * chunk + 1) ^ key_swizzle<64>(d)) * 8)) = widen8<DT>(vw[i].z, vw[i].w, vmul);
         }
         if (lane == 0) {
-            s.ks[buf][wid] = fmaxf(ks * c, 0x1p-126f);       // 0 would turn a masked -inf into NaN
-            s.raise[buf][wid] = raise;
-            s.pscale[buf][wid] = pscale;
-            s.nan[buf][wid] = any_nan;
-            s.live[buf][wid] = good;
+            s.raise[buf][chunk] = raise;
+            s.pscale[buf][chunk] = pscale;
+            s.nan[buf][chunk] = any_nan;
             s.ref[buf] = store_ref;
         }
     };
@@ -598,68 +603,69 @@ __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void pgn_cached_rows128_ke
                     }
                 }
             }
-            const float kc0 = s.ks[buf][hf], kc1 = s.ks[buf][2 + hf];
-            float mx0 = x[0][0], mx1 = x[1][0];
-#pragma unroll
-            for (int i = 1; i < 16; ++i) {
-                mx0 = fmaxf(mx0, x[0][i]);
-                mx1 = fmaxf(mx1, x[1][i]);
-            }
-            float mx = fmaxf(mx0 * kc0, mx1 * kc1);
-            mx = fmaxf(mx, __shfl_xor(mx, 32));
-            float oscale = 1.f;
-            bool move = false;
             if constexpr (DT == PGN_F16) {
                 const float now = s.ref[buf];
-                if (now != ref) {
-                    oscale = ref > 0.f ? ref / now : 1.f;
-                    move = true;
+                if (now != ref) {                            // another unit for the accumulator
+                    const float f = ref > 0.f ? ref / now : 1.f;
+                    ref = now;
+#pragma unroll
+                    for (int d = 0; d < DTILES; ++d)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[d][i] *= f;
                 }
-                ref = now;
             }
-            if (__any(mx > m + 8.f) || move) {               // also from -inf to the first score
-                const float m_new = mx > m + 8.f ? mx : m;
-                const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new);
-                m = m_new;
-                l *= alpha;
-                oscale *= alpha;
 #pragma unroll
-                for (int d = 0; d < DTILES; ++d)
+            for (int kt = 0; kt < 2; ++kt) {
+                const float kc = s.ks[buf][2 * kt + hf];
+                const float raise = DT == PGN_F16 ? s.raise[buf][2 * kt + hf] : 0.f;
+                const float pscale = DT == PGN_F16 ? s.pscale[buf][2 * kt + hf] : 1.f;
+                f32x16_t e;
+                float off = (m == -INFINITY ? 0.f : m) - raise, sum = 0.f;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) o[d][i] *= oscale;
-            }
-            const float base_m = m == -INFINITY ? 0.f : m;
-            float off0 = base_m, off1 = base_m;
-            if constexpr (DT == PGN_F16) {
-                off0 -= s.raise[buf][hf];
-                off1 -= s.raise[buf][2 + hf];
-            }
-            float sum0 = 0.f, sum1 = 0.f;
+                for (int i = 0; i < 16; ++i) {
+                    e[i] = __builtin_amdgcn_exp2f(fmaf(x[kt][i], kc, -off));
+                    sum += e[i];
+                }
+                sum *= pscale;
+                // a sum up to 2^8 says that no probability is above; otherwise, and while a row has seen nothing, the
+                // reference moves to the maximum
+                if (__any(!(sum <= 256.f) || m == -INFINITY)) {
+                    float mx = x[kt][0];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                x[0][i] = __builtin_amdgcn_exp2f(fmaf(x[0][i], kc0, -off0));
-                x[1][i] = __builtin_amdgcn_exp2f(fmaf(x[1][i], kc1, -off1));
-                sum0 += x[0][i];
-                sum1 += x[1][i];
-            }
-            if constexpr (DT == PGN_F16) {
-                sum0 *= s.pscale[buf][hf];
-                sum1 *= s.pscale[buf][2 + hf];
-            }
-            l += sum0 + sum1;
+                    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, x[kt][i]);
+                    mx *= kc;
+                    mx = fmaxf(mx, __shfl_xor(mx, 32));
+                    const float m_new = fmaxf(m, mx);
+                    const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new);
+                    m = m_new;
+                    l *= alpha;
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
+                    for (int d = 0; d < DTILES; ++d)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
+                    off = (m == -INFINITY ? 0.f : m) - raise;
+                    sum = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        e[i] = __builtin_amdgcn_exp2f(fmaf(x[kt][i], kc, -off));
+                        sum += e[i];
+                    }
+                    sum *= pscale;
+                }
+                l += sum;
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     v8 p;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) p[j] = Mat<DT>::one(x[kt][8 * half + j]);
+                    for (int j = 0; j < 8; ++j) p[j] = Mat<DT>::one(e[8 * half + j]);
 #pragma unroll
                     for (int d = 0; d < DTILES; ++d) {
                         const unsigned short* vp = tile.v + (32 * d + col) * 64;
-                        o[d] = Mat<DT>::mfma32(*reinterpret_cast<const v8*>(vp + (((4 * kt + 2 * hf + half) ^ key_swizzle<64>(col)) * 8)), p, o[d]);
+                        o[d] = Mat<DT>::mfma32(
+                            *reinterpret_cast<const v8*>(vp + (((4 * kt + 2 * hf + half) ^ key_swizzle<64>(col)) * 8)), p, o[d]);
                     }
                 }
+            }
             if (s.nan[buf][0] | s.nan[buf][1] | s.nan[buf][2] | s.nan[buf][3]) {
                 for (int w = 0; w < 4; ++w) {
                     if (!s.nan[buf][w]) continue;
@@ -875,7 +881,6 @@ extern "C" int pgn_cached_attention(const void* q, int dtype, const void* k_page
     a.out_vec = pgn_aligned(out, 8) && o_st % 4 == 0 && o_sh % 4 == 0;
     a.c = scale * 1.4426950408889634f;
     hipStream_t s = (hipStream_t)stream;
-    const dim3 block(PGN_CA_THREADS);
 #define PGN_CA_KERNEL(kernel, lds, grid)                                                                               \
     do {                                                                                                               \
         if ((lds) > 64 * 1024 - 1024) {                                                                                \
@@ -883,7 +888,7 @@ extern "C" int pgn_cached_attention(const void* q, int dtype, const void* k_page
                                                hipFuncAttributeMaxDynamicSharedMemorySize, (int)(lds));                \
             if (e != hipSuccess) return (int)e;                                                                        \
         }                                                                                                              \
-        hipLaunchKernelGGL(kernel, grid, block, lds, s, a);                                                            \
+        hipLaunchKernelGGL(kernel, grid, dim3(PGN_CA_THREADS), lds, s, a);                                             \
         PGN_LAUNCH_CHECK();                                                                                            \
     } while (0)
 #define PGN_CA_LAUNCH(DT, D)                                                                                           \
@@ -893,7 +898,7 @@ extern "C" int pgn_cached_attention(const void* q, int dtype, const void* k_page
                           dim3(Hkv * p.big_tiles, p.big_nsplit));                                                      \
         PGN_CA_KERNEL((pgn_cached_rows16_kernel<DT, D>), (size_t)4 * 16 * D * 4, dim3(Hkv * p.tiles, p.nsplit));       \
         if (p.nsplit > 1)                                                                                              \
-            PGN_CA_KERNEL((pgn_cached_join_kernel<DT, D, 16>), 0, dim3(Hkv * p.tiles, 4));                          \
+            PGN_CA_KERNEL((pgn_cached_join_kernel<DT, D, 16>), 0, dim3(Hkv * p.tiles, 4));                             \
         if (p.big_nsplit > 1)                                                                                          \
             PGN_CA_KERNEL((pgn_cached_join_kernel<DT, D, 128>), 0, dim3(Hkv * p.big_tiles, 32));                       \
     } while (0)
