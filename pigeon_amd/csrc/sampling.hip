@@ -7,21 +7,29 @@
 // One order ranks the ids: larger logit first, lower index first among equal ones.  As a 64-bit key - the logit's bits
 // made monotone and complemented, then the index - "rank before" is "smaller key", and every filter keeps the ids up to
 // some key: top-k the one where k ids, top-p the one where the wanted weight is reached.  That key is found without
-// sorting the row: a histogram over the distance to the maximum (2048 bins, 32 to a factor of two of weight) says in
-// which bin it lies, the few ids of that bin are gathered and sorted in LDS.
+// sorting the row, by bins over the distance to the maximum (2048 bins, 32 to a factor of two of weight).
 //
-// One workgroup of 1024 threads takes a row and reads it two or three times: maximum, histogram (of ids for top-k, of
-// weights for top-p), then either the gathering of the few ids that are left (top-k) or the sums of kept weights by
-// stretches of the row, one of which holds the drawn id.  Only the first reading comes from HBM.
+// One workgroup of 1024 threads takes a row.  It is bound by the passes over the row, whose loads only the first time
+// come from HBM, and by what each id costs in them (a CU spends some 1.5 cycles a 64-id instruction), so:
+//   top-k   the k-th largest of the 1024 threads' own maxima, known after the first pass, is at most the k-th largest
+//           logit: one more pass gathers what is not below its bin, some 1.1 k ids, and the rest (k, p, min-p, draw) is
+//           done among those in LDS;
+//   top-p   a pass adds the weights to the bins (whole numbers: an fp32 addition in LDS takes seven times as long), which
+//           says in which bin the border is; the next pass gathers the ids of that bin, where the border is found by a
+//           sort, and sums what is kept by stretches of the row.  A bin with more ids than the list takes (thousands of
+//           equal logits) has its key searched for by digits;
+//   draw    the stretch that the random number falls into is summed again by one wave.
 #include "pgn_common.h"
 
 #define PGN_SAMPLE_THREADS 1024
 #define PGN_SAMPLE_WAVES (PGN_SAMPLE_THREADS / 64)
 #define PGN_SAMPLE_BINS 2048
 #define PGN_SAMPLE_BINS_PER_OCTAVE 32.0f
-#define PGN_SAMPLE_LIST 4096                                 // ids of one bin, or of a whole top-k, that are sorted in LDS
+#define PGN_SAMPLE_LIST 4096                                 // ids that are sorted in LDS
+#define PGN_SAMPLE_FEW 256                                   // ids that are compared each with each instead
 #define PGN_SAMPLE_TABLE 1024
 #define PGN_SAMPLE_BITS 45
+#define PGN_SAMPLE_AHEAD 4                                   // vectors of a row that a thread has in flight
 
 namespace {
 
@@ -42,11 +50,16 @@ struct SampleArgs {
 };
 
 struct SampleLds {
-    u64 hist[PGN_SAMPLE_BINS];
+    union {
+        u64 mass[PGN_SAMPLE_BINS];
+        unsigned ids[PGN_SAMPLE_BINS];
+        u64 digit[256];
+    } hist;
     u64 key[PGN_SAMPLE_LIST];                                // the gathered ids
     u64 weight[PGN_SAMPLE_LIST];
     u64 seg[PGN_SAMPLE_MAX_IDS / 256 + PGN_SAMPLE_WAVES];    // kept weight of each 64 vectors (4 or 8 ids each) of the row
     double table[PGN_SAMPLE_TABLE];                          // 2^(-j / 1024)
+    u64 kept[PGN_SAMPLE_WAVES][128];                         // of each wave: kept logits and their indexes, 64 at a time
     u64 part[PGN_SAMPLE_WAVES];
     u64 found, before;
     float fpart[PGN_SAMPLE_WAVES];
@@ -66,32 +79,78 @@ __device__ __forceinline__ u64 rank_key(float x, int i) { return ((u64)rank_bits
 // NaN counts as a logit of -inf; -0 as 0, so that the two tie as they compare
 __device__ __forceinline__ float clean(float x) { return x != x ? -INFINITY : x + 0.f; }
 
-// A row in 16-byte vectors.  It may begin at any element: vector 0 is the aligned one that holds its first element, and
-// vectors that reach over either end are put together from single loads.
+// A row in 16-byte vectors.  It may begin at any element: vector 0 is the aligned one that holds its first element.  The
+// vectors that reach over an end are put together from single loads, with -inf where there is no id.
 template <int DT>
 struct Row {
     typedef typename Cvt<DT>::storage S;
     static constexpr int E = 16 / (int)sizeof(S);
     const S* first;                                          // aligned, at most E - 1 elements before the row
-    int lead, V, vectors;
+    int lead, V, vectors, whole_lo, whole_hi;                // vectors [whole_lo, whole_hi) lie inside the row
     __device__ __forceinline__ Row(const void* p, int n) {
         lead = (int)(((uintptr_t)p & 15) / sizeof(S));
         first = reinterpret_cast<const S*>(p) - lead;
         V = n;
         vectors = (lead + n + E - 1) / E;
+        whole_lo = lead > 0;
+        whole_hi = (lead + n) / E;
     }
-    // elements of vector j; index of the first of them is j * E - lead
-    __device__ __forceinline__ void load(int j, float* x) const {
-        const int i0 = j * E - lead;
-        S v[E];
-        if (i0 >= 0 && i0 + E <= V) {
-            *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(first + (int64_t)j * E);
+    __device__ __forceinline__ float one(int i) const { return clean(Cvt<DT>::to_f32(first[lead + i])); }
+    // index of element e of vector j
+    __device__ __forceinline__ int index(int j, int e) const { return j * E - lead + e; }
+    static __device__ __forceinline__ void unpack(const uint4& r, float* x) {
+        const unsigned w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-            for (int e = 0; e < E; ++e) x[e] = clean(Cvt<DT>::to_f32(v[e]));
-        } else {
+        for (int e = 0; e < E; ++e) {
+            if constexpr (DT == PGN_F32)
+                x[e] = clean(__uint_as_float(w[e]));
+            else
+                x[e] = clean(Cvt<DT>::to_f32((unsigned short)(e & 1 ? w[e / 2] >> 16 : w[e / 2] & 0xffffu)));
+        }
+    }
+    // any vector, one element at a time
+    __device__ __forceinline__ void pick(int j, float* x) const {
 #pragma unroll
-            for (int e = 0; e < E; ++e)
-                x[e] = i0 + e >= 0 && i0 + e < V ? clean(Cvt<DT>::to_f32(first[(int64_t)j * E + e])) : -INFINITY;
+        for (int e = 0; e < E; ++e) {
+            const int i = index(j, e);
+            x[e] = j < vectors && i >= 0 && i < V ? one(i) : -INFINITY;
+        }
+    }
+    // f(j, x[E]) for every vector of the row, in all threads equally often, some with vectors that hold nothing.  Vector j
+    // is thread j % 1024's.  The loads are free of branches and four of them are in flight.
+    template <typename F>
+    __device__ __forceinline__ void each(F f) const {
+        const int tid = threadIdx.x;
+        if (whole_hi > whole_lo) {
+            const auto load = [&](int j) {
+                return *reinterpret_cast<const uint4*>(first + (int64_t)min(max(j, whole_lo), whole_hi - 1) * E);
+            };
+            uint4 r[PGN_SAMPLE_AHEAD];
+#pragma unroll
+            for (int u = 0; u < PGN_SAMPLE_AHEAD; ++u) r[u] = load(u * PGN_SAMPLE_THREADS + tid);
+            for (int j0 = 0; j0 < whole_hi; j0 += PGN_SAMPLE_AHEAD * PGN_SAMPLE_THREADS) {
+#pragma unroll
+                for (int u = 0; u < PGN_SAMPLE_AHEAD; ++u) {
+                    const int j1 = j0 + u * PGN_SAMPLE_THREADS, j = j1 + tid;
+                    if (j1 < whole_hi) {
+                        float x[E];
+                        unpack(r[u], x);
+                        r[u] = load(j + PGN_SAMPLE_AHEAD * PGN_SAMPLE_THREADS);
+                        if (j < whole_lo || j >= whole_hi) {
+#pragma unroll
+                            for (int e = 0; e < E; ++e) x[e] = -INFINITY;
+                        }
+                        f(j, x);
+                    }
+                }
+            }
+        }
+        if (whole_lo > 0 || whole_hi < vectors) {            // at most two vectors: the ends
+            const int last = vectors - 1;
+            const int j = tid == 0 && whole_lo > 0 ? 0 : tid == 1 && whole_hi < vectors && (last > 0 || whole_lo == 0) ? last : vectors;
+            float x[E];
+            pick(j, x);
+            f(j, x);
         }
     }
 };
@@ -99,14 +158,13 @@ struct Row {
 struct Weights {
     double max, c;                                           // c: 1024 log2(e) / temperature
     float fmax, fc;                                          // fc: bins per unit of distance
-    bool infinite;                                           // the maximum is +inf: only its equals weigh anything
     const double* table;
     // w 2^45, nearest whole number.  2^-(t / 1024) with t = k + f, k whole, |f| <= 1/2: a table of 2^-(k % 1024 / 1024),
-    // an exponent, and e^-(f ln2 / 1024) as its series up to the third power (the fourth is 2^-50).
+    // an exponent, and e^-(f ln2 / 1024) as its series up to the third power (the fourth is 2^-50).  Beyond 2^-47 the
+    // result is 0 by itself; an infinite maximum leaves only its equals.
     __device__ __forceinline__ u64 fixed(float x) const {
-        if (infinite) return x == INFINITY ? 1ull << PGN_SAMPLE_BITS : 0;
-        const double t = (max - (double)x) * c;
-        if (!(t < 1024.0 * (PGN_SAMPLE_BITS + 2))) return x == fmax ? 1ull << PGN_SAMPLE_BITS : 0;
+        const double dx = x == fmax ? 0.0 : max - (double)x;
+        const double t = fmin(dx * c, 1024.0 * (PGN_SAMPLE_BITS + 2));       // a NaN (inf * 0) too
         const double d = t + 0x1.8p52;
         const int k = (int)(unsigned)(u64)__double_as_longlong(d);
         const double f = t - (d - 0x1.8p52);
@@ -117,91 +175,90 @@ struct Weights {
     }
     // monotone in x: 32 bins to a factor of two, everything from 2^-64 on in the last
     __device__ __forceinline__ int bin(float x) const {
-        const float y = x == fmax ? 0.f : (fmax - x) * fc;
-        return (int)fminf(y, (float)(PGN_SAMPLE_BINS - 1));
+        return (int)fminf(x == fmax ? 0.f : (fmax - x) * fc, (float)(PGN_SAMPLE_BINS - 1));
     }
 };
 
-__device__ u64 block_sum(u64 v, u64* part) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
-    __syncthreads();
-    u64 s = 0;
-#pragma unroll
-    for (int w = 0; w < PGN_SAMPLE_WAVES; ++w) s += part[w];
-    return s;
+// inclusive prefix sum over the wave, by lane shifts within rows of 16 and two broadcasts across them
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp0(int v) {
+    return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
 }
-
-__device__ __forceinline__ u64 wave_scan(u64 v) {            // inclusive
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const u64 o = __shfl_up(v, off);
-        if (lane >= off) v += o;
-    }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 dpp0(u64 v) {
+    const unsigned lo = (unsigned)dpp0<CTRL, ROWS>((int)(unsigned)v), hi = (unsigned)dpp0<CTRL, ROWS>((int)(unsigned)(v >> 32));
+    return ((u64)hi << 32) | lo;
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned dpp0(unsigned v) { return (unsigned)dpp0<CTRL, ROWS>((int)v); }
+template <typename T>
+__device__ __forceinline__ T wave_scan(T v) {
+    v += dpp0<0x111, 0xf>(v);
+    v += dpp0<0x112, 0xf>(v);
+    v += dpp0<0x114, 0xf>(v);
+    v += dpp0<0x118, 0xf>(v);
+    v += dpp0<0x142, 0xa>(v);
+    v += dpp0<0x143, 0xc>(v);
     return v;
 }
 
-__device__ u64 block_scan(u64 v, u64* part, u64& total) {    // inclusive
+// inclusive prefix sum over the workgroup, and the sum of all
+template <typename T>
+__device__ T block_scan(T v, void* scratch, T& total) {
+    T* part = reinterpret_cast<T*>(scratch);
     const int wid = threadIdx.x >> 6;
     v = wave_scan(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 63) part[wid] = v;
     __syncthreads();
-    u64 before = 0, all = 0;
+    T before = 0, all = 0;
 #pragma unroll
     for (int w = 0; w < PGN_SAMPLE_WAVES; ++w) {
-        const u64 p = part[w];
+        const T p = part[w];
         before += w < wid ? p : 0;
         all += p;
     }
     total = all;
     return v + before;
 }
+__device__ __forceinline__ u64 block_sum(u64 v, u64* part) {
+    u64 total;
+    block_scan(v, part, total);
+    return total;
+}
 
-// hist[b] += v in one lane for the whole wave where all its lanes add to one bin (equal logits), else lane by lane
-__device__ __forceinline__ void hist_add(u64* hist, int b, u64 v, bool on) {
-    const uint64_t lanes = __ballot(on);
+// hist[b] += v in one lane for the whole wave where all its lanes add to one place (equal logits), else lane by lane
+__device__ __forceinline__ void digit_add(u64* hist, int b, u64 v) {
+    const uint64_t lanes = __ballot(v > 0);
     if (lanes == 0) return;
     const int leader = __builtin_ctzll(lanes), b0 = __shfl(b, leader);
-    if (__popcll(lanes) > 1 && __all(!on || b == b0)) {
-        u64 s = on ? v : 0;
-#pragma unroll
-        for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off);
-        if ((int)(threadIdx.x & 63) == leader) atomicAdd(&hist[b0], s);
-    } else if (on) {
+    if (__popcll(lanes) > 1 && __all(v == 0 || b == b0)) {
+        const u64 s = wave_scan(v);
+        if ((threadIdx.x & 63) == 63) atomicAdd(&hist[b0], s);
+    } else if (v > 0) {
         atomicAdd(&hist[b], v);
     }
 }
 
-// The key up to which the ids (of keys up to `limit`) hold `target` together, by eight bits of the key at a time over the
-// whole row: for bins with more ids than the list takes.
+// The key up to which the ids (of keys up to `limit`) hold `target` together, ids counted or weights summed, by eight bits
+// of the key at a time over the whole row.
 template <int DT>
 __device__ u64 select_key(SampleLds& s, const Row<DT>& row, const Weights& w, bool by_weight, u64 target, u64 limit) {
     u64 prefix = 0, before = 0;
     const int tid = threadIdx.x;
     for (int shift = 48; shift >= 0; shift -= 8) {
         __syncthreads();
-        for (int b = tid; b < 256; b += PGN_SAMPLE_THREADS) s.hist[b] = 0;
+        for (int b = tid; b < 256; b += PGN_SAMPLE_THREADS) s.hist.digit[b] = 0;
         __syncthreads();
-        for (int j0 = 0; j0 < row.vectors; j0 += PGN_SAMPLE_THREADS) {
-            float x[Row<DT>::E];
-            const bool in = j0 + tid < row.vectors;
-            if (in) row.load(j0 + tid, x);
-#pragma unroll 1
-            for (int e = 0; e < Row<DT>::E; ++e) {
-                const float xe = in ? x[e] : -INFINITY;
-                const u64 key = rank_key(xe, (j0 + tid) * Row<DT>::E - row.lead + e);
-                const bool on = xe > -INFINITY && key <= limit && (key >> (shift + 8)) == prefix;
-                const u64 v = !on ? 0 : by_weight ? w.fixed(xe) : 1;
-                hist_add(s.hist, (int)(key >> shift) & 255, v, on && v > 0);
-            }
+        for (int i0 = 0; i0 < row.V; i0 += PGN_SAMPLE_THREADS) {
+            const float x = i0 + tid < row.V ? row.one(i0 + tid) : -INFINITY;
+            const u64 key = rank_key(x, i0 + tid);
+            const bool on = x > -INFINITY && key <= limit && (key >> (shift + 8)) == prefix;
+            digit_add(s.hist.digit, (int)(key >> shift) & 255, !on ? 0 : by_weight ? w.fixed(x) : 1);
         }
         __syncthreads();
         u64 total;
-        const u64 v = tid < 256 ? s.hist[tid] : 0;
+        const u64 v = tid < 256 ? s.hist.digit[tid] : 0;
         const u64 c = before + block_scan(v, s.part, total);
         if (tid < 256 && v > 0 && c - v < target && c >= target) {
             s.found = (prefix << 8) | (unsigned)tid;
@@ -214,26 +271,31 @@ __device__ u64 select_key(SampleLds& s, const Row<DT>& row, const Weights& w, bo
     return prefix;
 }
 
-// Bin in which the running sum over the histogram reaches `target` (it does), and the sum before it.
-__device__ int find_bin(SampleLds& s, u64 target, u64& before) {
+// Bin in which the running sum over the histogram reaches `target`, and the sum before it; the last bin if none does.
+template <typename T>
+__device__ int find_bin(SampleLds& s, const T* hist, T target, T& before) {
     constexpr int PER = PGN_SAMPLE_BINS / PGN_SAMPLE_THREADS;
-    u64 v[PER], sum = 0, total;
+    T v[PER], sum = 0, total;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        v[i] = s.hist[threadIdx.x * PER + i];
+        v[i] = hist[threadIdx.x * PER + i];
         sum += v[i];
     }
-    u64 c = block_scan(sum, s.part, total) - sum;
+    if (threadIdx.x == 0) s.at = PGN_SAMPLE_BINS - 1;
+    T c = block_scan(sum, s.part, total) - sum;
+    T* out = reinterpret_cast<T*>(&s.before);
+    if (threadIdx.x == 0) *out = total - hist[PGN_SAMPLE_BINS - 1];
+    __syncthreads();
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
         if (c < target && c + v[i] >= target) {
             s.at = threadIdx.x * PER + i;
-            s.before = c;
+            *out = c;
         }
         c += v[i];
     }
     __syncthreads();
-    before = s.before;
+    before = *out;
     const int b = s.at;
     __syncthreads();
     return b;
@@ -270,7 +332,7 @@ __device__ int pad_list(SampleLds& s, int n) {
     return m;
 }
 
-// First place of the list at which the running sum of weights reaches `target`; n - 1 if none.  n <= 4 per thread.
+// First place of the list at which the running sum of weights reaches `target`; n - 1 if none.
 __device__ int find_place(SampleLds& s, int n, u64 target, u64& total) {
     constexpr int PER = PGN_SAMPLE_LIST / PGN_SAMPLE_THREADS;
     u64 v[PER], sum = 0;
@@ -307,6 +369,67 @@ __device__ __forceinline__ u64 nucleus_target(float p, u64 z) {
     return t < z ? t : z;
 }
 
+// The rest of a top-k among the n ids of the list, the first k in rank among them: top-p, min-p and the draw.  `least`:
+// min-p as a weight.  A few ids compare each with each (ranks and running sums without a sort, three rounds); more are
+// sorted by rank, then by index.
+__device__ void finish_list(SampleLds& s, const Weights& w, int n, int k, float p, double least, float u, int64_t* id) {
+    const int tid = threadIdx.x;
+    const u64 one = 1ull << PGN_SAMPLE_BITS;
+    u64 z;
+    if (n <= PGN_SAMPLE_FEW) {
+        u64 key = 0, v = 0;
+        if (tid < n) {
+            key = s.key[tid];
+            int rank = 0;
+            for (int j = 0; j < n; ++j) rank += s.key[j] < key;
+            v = rank < k ? w.fixed(rank_value((unsigned)(key >> 24))) : 0;
+            s.weight[tid] = v;
+        }
+        const u64 all = block_sum(v, s.part);
+        if (p < 1.f) {
+            const u64 target = nucleus_target(p, all);
+            if (tid < n) {
+                u64 before = 0;
+                for (int j = 0; j < n; ++j) before += s.key[j] < key ? s.weight[j] : 0;
+                v = before < target ? v : 0;
+            }
+        }
+        if (!((double)v >= least || v == one)) v = 0;
+        __syncthreads();
+        if (tid < n) s.weight[tid] = v;
+        if (tid == 0) s.found = ~0ull;
+        z = block_sum(v, s.part);
+        if (tid < n && v > 0) {
+            const unsigned i = (unsigned)key & 0xffffff;
+            u64 upto = 0;
+            for (int j = 0; j < n; ++j) upto += ((unsigned)s.key[j] & 0xffffff) <= i ? s.weight[j] : 0;
+            if (upto >= draw_target(u, z)) atomicMin(&s.found, (u64)i);
+        }
+        __syncthreads();
+        if (tid == 0) *id = (int64_t)s.found;
+        return;
+    }
+    sort_list(s, pad_list(s, n));
+    int kept = k < n ? k : n;
+    u64 all = 0;
+    for (int i = tid; i < kept; i += PGN_SAMPLE_THREADS) all += s.weight[i] = w.fixed(rank_value((unsigned)(s.key[i] >> 24)));
+    all = block_sum(all, s.part);
+    if (p < 1.f) kept = find_place(s, kept, nucleus_target(p, all), z) + 1;
+    const int padded = pad_list(s, kept);
+    u64 sum = 0;
+    for (int i = tid; i < kept; i += PGN_SAMPLE_THREADS) {
+        const u64 v = s.weight[i];
+        const bool on = (double)v >= least || v == one;
+        s.weight[i] = on ? v : 0;
+        s.key[i] &= 0xffffff;                                // by index now
+        sum += on ? v : 0;
+    }
+    z = block_sum(sum, s.part);
+    sort_list(s, padded);
+    const int at = find_place(s, kept, draw_target(u, z), z);
+    if (tid == 0) *id = (int64_t)s.key[at];
+}
+
 template <int DT>
 __global__ __launch_bounds__(PGN_SAMPLE_THREADS) void pgn_sample_tokens_kernel(const SampleArgs a) {
     extern __shared__ unsigned char smem[];
@@ -318,17 +441,17 @@ __global__ __launch_bounds__(PGN_SAMPLE_THREADS) void pgn_sample_tokens_kernel(c
     const int k = a.top_k ? a.top_k[b] : a.top_k_all;
     const float p = a.top_p ? a.top_p[b] : a.top_p_all;
     const float min_p = a.min_p ? a.min_p[b] : a.min_p_all;
+    const float u = a.u[b];
 
-    float m = -INFINITY;
-    for (int j = tid; j < row.vectors; j += PGN_SAMPLE_THREADS) {
-        float x[E];
-        row.load(j, x);
+    float mine = -INFINITY;                                  // the thread's own maximum
+    row.each([&](int, const float* x) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) m = fmaxf(m, x[e]);
-    }
-    for (int i = tid; i < PGN_SAMPLE_BINS; i += PGN_SAMPLE_THREADS) s.hist[i] = 0;
+        for (int e = 0; e < E; ++e) mine = fmaxf(mine, x[e]);
+    });
+    for (int i = tid; i < PGN_SAMPLE_BINS; i += PGN_SAMPLE_THREADS) s.hist.ids[i] = 0;
     s.table[tid] = exp2((double)tid * (-1.0 / PGN_SAMPLE_TABLE));
     if (tid == 0) s.count = 0;
+    float m = mine;
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
     if (lane == 0) s.fpart[wid] = m;
@@ -341,12 +464,10 @@ __global__ __launch_bounds__(PGN_SAMPLE_THREADS) void pgn_sample_tokens_kernel(c
     }
     if (!(t > 0.f) || p <= 0.f || k == 1) {                  // the first in rank: the lowest index of the largest logit
         int at = V;
-        for (int j = tid; j < row.vectors; j += PGN_SAMPLE_THREADS) {
-            float x[E];
-            row.load(j, x);
+        row.each([&](int j, const float* x) {
 #pragma unroll
-            for (int e = E - 1; e >= 0; --e) at = x[e] == m ? min(at, j * E - row.lead + e) : at;
-        }
+            for (int e = E - 1; e >= 0; --e) at = x[e] == m ? min(at, row.index(j, e)) : at;
+        });
 #pragma unroll
         for (int off = 32; off > 0; off >>= 1) at = min(at, __shfl_xor(at, off));
         if (lane == 0) s.part[wid] = (u64)at;
@@ -361,169 +482,192 @@ __global__ __launch_bounds__(PGN_SAMPLE_THREADS) void pgn_sample_tokens_kernel(c
     Weights w;
     w.max = m;
     w.fmax = m;
-    w.infinite = m == INFINITY;
     w.c = PGN_SAMPLE_TABLE * 1.44269504088896340736 / (double)t;
     w.fc = (float)(PGN_SAMPLE_BINS_PER_OCTAVE * 1.44269504088896340736 / (double)t);
     w.table = s.table;
+    const double least = (double)min_p * (double)(1ull << PGN_SAMPLE_BITS);
     u64 limit = ~0ull;                                       // keys up to it are kept
 
-    if (k > 0 && k < V) {
-        for (int j0 = 0; j0 < row.vectors; j0 += PGN_SAMPLE_THREADS) {
-            float x[E];
-            const bool in = j0 + tid < row.vectors;
-            if (in) row.load(j0 + tid, x);
+    // gathers the ids of bins [from, to]; how many there are (the list takes PGN_SAMPLE_LIST of them)
+    const auto gather = [&](int from, int to) {
+        __syncthreads();
+        if (tid == 0) s.count = 0;
+        __syncthreads();
+        row.each([&](int j, const float* x) {
+            unsigned in = 0;
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                const float xe = in ? x[e] : -INFINITY;
-                hist_add(s.hist, w.bin(xe), 1, xe > -INFINITY);
+                const int bin = w.bin(x[e]);
+                in |= x[e] > -INFINITY && bin >= from && bin <= to ? 1u << e : 0u;
             }
-        }
-        __syncthreads();
-        u64 sum = 0;
-        for (int i = tid; i < PGN_SAMPLE_BINS; i += PGN_SAMPLE_THREADS) sum += s.hist[i];
-        if (block_sum(sum, s.part) > (u64)k) {
-            u64 before;
-            const int cut = find_bin(s, (u64)k, before);
-            const u64 inside = s.hist[cut];
-            const bool all = before + inside <= PGN_SAMPLE_LIST;
-            if (all || inside <= PGN_SAMPLE_LIST) {          // all ids up to the bin's end, or those of the bin alone
-                for (int j = tid; j < row.vectors; j += PGN_SAMPLE_THREADS) {
-                    float x[E];
-                    row.load(j, x);
+#pragma unroll 1
+            for (; __any(in != 0); in &= in - 1) {           // one id a lane at a time
+                const int e = in ? __builtin_ctz(in) : 0;
+                float xe = x[0];
 #pragma unroll
-                    for (int e = 0; e < E; ++e) {
-                        const int bin = w.bin(x[e]);
-                        if (x[e] > -INFINITY && (bin == cut || (all && bin < cut))) {
-                            const int at = atomicAdd(&s.count, 1);
-                            s.key[at] = rank_key(x[e], j * E - row.lead + e);
-                            s.weight[at] = 0;
-                        }
-                    }
+                for (int n = 1; n < E; ++n) xe = e == n ? x[n] : xe;
+                if (in) {
+                    const int at = atomicAdd(&s.count, 1);
+                    if (at < PGN_SAMPLE_LIST) s.key[at] = rank_key(xe, row.index(j, e));
                 }
-                __syncthreads();
-                const int n = s.count;
-                const int padded = pad_list(s, n);
-                sort_list(s, padded);
-                if (!all) {
-                    limit = s.key[k - (int)before - 1];
-                } else {                                     // the k ids are here: the rest is done in the list
-                    for (int i = tid; i < k; i += PGN_SAMPLE_THREADS) s.weight[i] = w.fixed(rank_value((unsigned)(s.key[i] >> 24)));
-                    __syncthreads();
-                    int kept = k;
-                    u64 z;
-                    if (p < 1.f) {
-                        u64 sum_k = 0;
-                        for (int i = tid; i < k; i += PGN_SAMPLE_THREADS) sum_k += s.weight[i];
-                        sum_k = block_sum(sum_k, s.part);
-                        kept = find_place(s, k, nucleus_target(p, sum_k), z) + 1;
-                    }
-                    const int again = pad_list(s, kept);
-                    const double least = (double)min_p * (double)(1ull << PGN_SAMPLE_BITS);
-                    for (int i = tid; i < kept; i += PGN_SAMPLE_THREADS) {
-                        const bool on = (double)s.weight[i] >= least || s.weight[i] == 1ull << PGN_SAMPLE_BITS;
-                        s.weight[i] = on ? s.weight[i] : 0;
-                        s.key[i] &= 0xffffff;                // by index now
-                    }
-                    sort_list(s, again);
-                    u64 zero = 0;
-                    for (int i = tid; i < kept; i += PGN_SAMPLE_THREADS) zero += s.weight[i];
-                    z = block_sum(zero, s.part);
-                    const int at = find_place(s, kept, draw_target(a.u[b], z), z);
-                    if (tid == 0) a.ids[b] = (int64_t)s.key[at];
+            }
+        });
+        __syncthreads();
+        return s.count;
+    };
+
+    if (k > 0 && k < V) {
+        unsigned before, total;
+        if (k <= PGN_SAMPLE_THREADS) {
+            if (mine > -INFINITY) atomicAdd(&s.hist.ids[w.bin(mine)], 1u);
+            __syncthreads();
+            const int cut = find_bin(s, s.hist.ids, (unsigned)k, before);      // the last bin too if there are fewer maxima
+            if (cut < PGN_SAMPLE_BINS - 1) {
+                const int n = gather(0, cut);
+                if (n <= PGN_SAMPLE_LIST) {
+                    finish_list(s, w, n, k, p, least, u, a.ids + b);
                     return;
                 }
+            }
+            __syncthreads();
+            for (int i = tid; i < PGN_SAMPLE_BINS; i += PGN_SAMPLE_THREADS) s.hist.ids[i] = 0;
+            __syncthreads();
+        }
+        // all ids by bins; the last bin, which may hold most of a row, is counted in registers
+        unsigned last = 0;
+        row.each([&](int, const float* x) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const int bin = w.bin(x[e]);
+                const bool is = x[e] > -INFINITY;
+                if (is && bin < PGN_SAMPLE_BINS - 1) atomicAdd(&s.hist.ids[bin], 1u);
+                last += is && bin == PGN_SAMPLE_BINS - 1;
+            }
+        });
+        block_scan(last, s.part, total);
+        if (tid == 0) s.hist.ids[PGN_SAMPLE_BINS - 1] = total;
+        __syncthreads();
+        unsigned sum = 0;
+        for (int i = tid; i < PGN_SAMPLE_BINS; i += PGN_SAMPLE_THREADS) sum += s.hist.ids[i];
+        block_scan(sum, s.part, total);
+        if (total > (unsigned)k) {
+            const int cut = find_bin(s, s.hist.ids, (unsigned)k, before);
+            const unsigned inside = s.hist.ids[cut];
+            if (before + inside <= PGN_SAMPLE_LIST) {
+                const int n = gather(0, cut);
+                finish_list(s, w, n, k, p, least, u, a.ids + b);
+                return;
+            }
+            if (inside <= PGN_SAMPLE_LIST) {                 // many ids are kept: only the border is looked for in the list
+                const int n = gather(cut, cut);
+                sort_list(s, pad_list(s, n));
+                limit = s.key[k - (int)before - 1];
             } else {
                 limit = select_key<DT>(s, row, w, false, (u64)k, limit);
             }
         }
         __syncthreads();
-        for (int i = tid; i < PGN_SAMPLE_BINS; i += PGN_SAMPLE_THREADS) s.hist[i] = 0;
-        if (tid == 0) s.count = 0;
-        __syncthreads();
     }
 
     int cut = PGN_SAMPLE_BINS;                               // bins before it are kept whole (as far as `limit` goes)
     u64 target_p = 0, inside_target = 0;
-    bool listed = false;
     if (p < 1.f) {
-        for (int j0 = 0; j0 < row.vectors; j0 += PGN_SAMPLE_THREADS) {
-            float x[E];
-            const bool in = j0 + tid < row.vectors;
-            if (in) row.load(j0 + tid, x);
+        for (int i = tid; i < PGN_SAMPLE_BINS; i += PGN_SAMPLE_THREADS) s.hist.mass[i] = 0;
+        if (tid == 0) s.count = 0;
+        __syncthreads();
+        row.each([&](int j, const float* x) {
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                const float xe = in ? x[e] : -INFINITY;
-                const u64 v = rank_key(xe, (j0 + tid) * E - row.lead + e) <= limit ? w.fixed(xe) : 0;
-                hist_add(s.hist, w.bin(xe), v, v > 0);
+                u64 v = w.fixed(x[e]);
+                if (limit != ~0ull) v = rank_key(x[e], row.index(j, e)) <= limit ? v : 0;
+                if (v > 0) atomicAdd(&s.hist.mass[w.bin(x[e])], v);
             }
-        }
+        });
         __syncthreads();
         u64 sum = 0, before;
-        for (int i = tid; i < PGN_SAMPLE_BINS; i += PGN_SAMPLE_THREADS) sum += s.hist[i];
+        for (int i = tid; i < PGN_SAMPLE_BINS; i += PGN_SAMPLE_THREADS) sum += s.hist.mass[i];
         target_p = nucleus_target(p, block_sum(sum, s.part));
-        cut = find_bin(s, target_p, before);
+        cut = find_bin(s, s.hist.mass, target_p, before);
         inside_target = target_p - before;
-        listed = true;
     }
 
     // weights of what is kept, by stretches of 64 vectors; the ids of the bin with the border go to the list
-    const double least = (double)min_p * (double)(1ull << PGN_SAMPLE_BITS);
     const int segs = (row.vectors + 63) >> 6;
+    bool listed = p < 1.f;
     for (;;) {
-        for (int g = wid; g < segs; g += PGN_SAMPLE_WAVES) {
-            const int j = g * 64 + lane;
-            u64 sum = 0;
-            if (j < row.vectors) {
-                float x[E];
-                row.load(j, x);
+        for (int i = tid; i < segs; i += PGN_SAMPLE_THREADS) s.seg[i] = 0;
+        __syncthreads();
+        // Few ids may be kept, and a weight is dear: every wave collects kept logits until it has 64 to weigh.
+        u64* kept = s.kept[wid];
+        int held = 0;
+        const auto weigh = [&](bool on, u64 entry) {
+            const u64 v = on ? w.fixed(__uint_as_float((unsigned)entry)) : 0;
+            if (on && ((double)v >= least || v == 1ull << PGN_SAMPLE_BITS))
+                atomicAdd(&s.seg[((int)(entry >> 32) + row.lead) / (64 * E)], v);
+        };
+        row.each([&](int j, const float* x) {
+            unsigned in = 0, at_edge = 0;
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const u64 key = rank_key(x[e], j * E - row.lead + e);
-                    const int bin = w.bin(x[e]);
-                    if (x[e] > -INFINITY && bin <= cut && key <= limit) {
-                        const u64 v = w.fixed(x[e]);
-                        if (listed && bin == cut) {
-                            const int at = atomicAdd(&s.count, 1);
-                            if (at < PGN_SAMPLE_LIST) {
-                                s.key[at] = key;
-                                s.weight[at] = v;
-                            }
-                        } else if ((double)v >= least || x[e] == m) {
-                            sum += v;
-                        }
-                    }
+            for (int e = 0; e < E; ++e) {
+                const int bin = w.bin(x[e]);
+                const bool on = x[e] > -INFINITY && (limit == ~0ull || rank_key(x[e], row.index(j, e)) <= limit);
+                in |= on && bin < cut ? 1u << e : 0u;
+                at_edge |= on && bin == cut ? 1u << e : 0u;
+            }
+            in |= at_edge << 8;
+#pragma unroll 1
+            for (; __any(in != 0); in &= in - 1) {           // one id a lane at a time
+                const int bit = in ? __builtin_ctz(in) : 31, e = bit & 7, i = row.index(j, e);
+                float xe = x[0];
+#pragma unroll
+                for (int n = 1; n < E; ++n) xe = e == n ? x[n] : xe;
+                if (bit >= 8 && bit < 16) {
+                    const int at = atomicAdd(&s.count, 1);
+                    if (at < PGN_SAMPLE_LIST) s.key[at] = rank_key(xe, i);
+                }
+                const uint64_t lanes = __ballot(bit < 8);
+                if (bit < 8) kept[held + __popcll(lanes & ((1ull << lane) - 1))] = ((u64)(unsigned)i << 32) | __float_as_uint(xe);
+                held += __popcll(lanes);
+                if (held >= 64) {
+                    __builtin_amdgcn_wave_barrier();
+                    weigh(true, kept[lane]);
+                    held -= 64;
+                    const u64 rest = kept[64 + lane];
+                    __builtin_amdgcn_wave_barrier();
+                    if (lane < held) kept[lane] = rest;
                 }
             }
-#pragma unroll
-            for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off);
-            if (lane == 0) s.seg[g] = sum;
-        }
+        });
+        __builtin_amdgcn_wave_barrier();
+        weigh(lane < held, kept[lane]);
         __syncthreads();
-        if (!listed || s.count <= PGN_SAMPLE_LIST) break;
-        limit = select_key<DT>(s, row, w, true, target_p, limit);    // too many ids in the border's bin
+        if (!listed) break;
+        const int n = s.count;
+        if (n <= PGN_SAMPLE_LIST) {
+            u64 total;
+            for (int i = tid; i < n; i += PGN_SAMPLE_THREADS) s.weight[i] = w.fixed(rank_value((unsigned)(s.key[i] >> 24)));
+            sort_list(s, pad_list(s, n));
+            const int last = find_place(s, n, inside_target, total);
+            limit = min(limit, s.key[last]);
+            for (int i = tid; i <= last; i += PGN_SAMPLE_THREADS) {
+                const u64 v = s.weight[i];
+                if ((double)v >= least || v == 1ull << PGN_SAMPLE_BITS)
+                    atomicAdd(&s.seg[((int)(s.key[i] & 0xffffff) + row.lead) / (64 * E)], v);
+            }
+            __syncthreads();
+            break;
+        }
+        limit = select_key<DT>(s, row, w, true, target_p, limit);
         cut = PGN_SAMPLE_BINS;
         listed = false;
-    }
-    if (listed) {
-        const int n = s.count, padded = pad_list(s, n);
-        sort_list(s, padded);
-        u64 total;
-        const int last = find_place(s, n, inside_target, total);
-        limit = min(limit, s.key[last]);
-        for (int i = tid; i <= last; i += PGN_SAMPLE_THREADS) {
-            const u64 v = s.weight[i];
-            if ((double)v >= least || v == 1ull << PGN_SAMPLE_BITS)
-                atomicAdd(&s.seg[((int)(s.key[i] & 0xffffff) + row.lead) / (64 * E)], v);
-        }
         __syncthreads();
     }
     if (wid != 0) return;
 
     u64 z = 0;
     for (int g = lane; g < segs; g += 64) z += s.seg[g];
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) z += __shfl_xor(z, off);
-    const u64 target = draw_target(a.u[b], z);
+    z = __shfl(wave_scan(z), 63);
+    const u64 target = draw_target(u, z);
     u64 before = 0;
     int g0 = 0;
     for (; g0 < segs; g0 += 64) {
@@ -540,21 +684,18 @@ __global__ __launch_bounds__(PGN_SAMPLE_THREADS) void pgn_sample_tokens_kernel(c
     const int j = g0 * 64 + lane;
     u64 v[E], sum = 0;
     float x[E];
-    if (j < row.vectors) row.load(j, x);
+    row.pick(j, x);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-        v[e] = 0;
-        if (j < row.vectors && x[e] > -INFINITY && rank_key(x[e], j * E - row.lead + e) <= limit) {
-            const u64 f = w.fixed(x[e]);
-            if ((double)f >= least || x[e] == m) v[e] = f;
-        }
+        const u64 f = x[e] > -INFINITY && rank_key(x[e], row.index(j, e)) <= limit ? w.fixed(x[e]) : 0;
+        v[e] = (double)f >= least || x[e] == m ? f : 0;
         sum += v[e];
     }
     u64 c = before + wave_scan(sum) - sum;
     int hit = -1;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-        if (hit < 0 && c < target && c + v[e] >= target) hit = j * E - row.lead + e;
+        if (hit < 0 && c < target && c + v[e] >= target) hit = row.index(j, e);
         c += v[e];
     }
     const uint64_t any = __ballot(hit >= 0);

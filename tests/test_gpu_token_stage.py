@@ -533,6 +533,26 @@ def test_sampling_more_equal_logits_than_a_list_holds():
     _check_sample(far, u[:2], top_k=5000, top_p=0.9999, temperature=200.0)
 
 
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_sampling_wide_nuclei_and_large_top_k(dt):
+    """Borders deep in the tail: top-p near 1, top-k beyond the threads' own maxima and beyond the list, the largest
+    logits all in one thread's share."""
+    x, u = _logits(6, 60000, dt, seed=11)
+    for p in (0.999, 0.9999, 0.999999, 1.0 - 2.0 ** -24, 1e-6, 1e-30):
+        _check_sample(x, u, top_p=p)
+        _check_sample(x, u, top_p=p, temperature=3.0, min_p=1e-4)
+    for k in (256, 257, 1000, 1024, 1025, 4095, 4096, 4097, 30000, 59999, 60000, 2 ** 31 - 1):
+        _check_sample(x, u, top_k=k)
+        _check_sample(x, u, top_k=k, top_p=0.97, temperature=2.0)
+    y = torch.full((2, 40000), -5.0, device=DEV)                    # ids 0 .. 7 and 4096 .. 4103: few threads see them all
+    y[:, :8] = torch.linspace(3, 4, 8, device=DEV)
+    y[:, 4096:4104] = 3.5
+    y[1, 9000:9600] = 3.75
+    for k in (2, 9, 12, 500, 620):
+        _check_sample(y.to(dt), u[:2], top_k=k)
+        _check_sample(y.to(dt), u[2:4], top_k=k, top_p=0.8)
+
+
 def test_sampling_masked_and_infinite_logits():
     g = torch.Generator().manual_seed(0)
     x = torch.randn(10, 500, generator=g)
