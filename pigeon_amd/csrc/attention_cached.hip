@@ -201,23 +201,45 @@ __global__ __launch_bounds__(PGN_CA_THREADS) void pgn_cached_rows16_kernel(const
 
     const int* table = a.table + t.r * a.table_stride;
     const int P = 1 << a.shift;
-    for (int base = kb + wid * 64; base < kend; base += 256) {
-        // pages: of the key rows that this lane loads, and of the keys that it owns
-        const int kkey = base + 16 * (col >> 2) + (col & 3), okey = base + 16 * g;
-        const int kpage = table[min(kkey >> a.shift, a.W - 1)], opage = table[min(okey >> a.shift, a.W - 1)];
-        const bool kgood = kkey < t.len && (unsigned)kpage < (unsigned)a.N;
-        const bool ogood = okey < hi && okey + 16 > lo && (unsigned)opage < (unsigned)a.N;
-        const unsigned char* kp = a.k_pages + (((int64_t)(kgood ? kpage : 0) * a.Hkv + h) * P + (kkey & (P - 1))) * D + g * 16;
-        const unsigned char* vp = a.v_pages + (((int64_t)(ogood ? opage : 0) * a.Hkv + h) * D + col) * P + (okey & (P - 1));
-        uint4 kw[4][DB], vw[DTILES];
+    // Bytes of 64 keys: asked for while the 64 before are worked on - keys when their scores are done, values when their
+    // product is - and their pages, of the key rows that this lane loads and of the keys that it owns, one round earlier.
+    uint4 kw[4][DB], vw[DTILES];
+    float ks = 0.f, vs = 0.f;
+    bool ogood = false;
+    int kpage = 0, opage = 0;
+    const auto look_up = [&](int base) {
+        kpage = table[min((base + 16 * (col >> 2)) >> a.shift, a.W - 1)];
+        opage = table[min((base + 16 * g) >> a.shift, a.W - 1)];
+    };
+    const auto load_keys = [&](int base, int page) {
+        const int key = base + 16 * (col >> 2) + (col & 3);
+        const bool good = key < t.len && (unsigned)page < (unsigned)a.N;
+        const unsigned char* kp = a.k_pages + (((int64_t)(good ? page : 0) * a.Hkv + h) * P + (key & (P - 1))) * D + g * 16;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int s = 0; s < DB; ++s) kw[i][s] = *reinterpret_cast<const uint4*>(kp + i * 4 * D + s * 64);
+    };
+    const auto load_values = [&](int base, int page) {
+        const int key = base + 16 * g;
+        ogood = key < hi && key + 16 > lo && (unsigned)page < (unsigned)a.N;
+        const int64_t at = (int64_t)(ogood ? page : 0) * a.Hkv + h;
+        const unsigned char* vp = a.v_pages + (at * D + col) * P + (key & (P - 1));
 #pragma unroll
         for (int d = 0; d < DTILES; ++d) vw[d] = *reinterpret_cast<const uint4*>(vp + (int64_t)d * 16 * P);
-        const float ks = ogood ? a.k_scale[(int64_t)opage * a.Hkv + h] * a.c : 0.f;
-        const float vs = ogood ? a.v_scale[(int64_t)opage * a.Hkv + h] : 0.f;
+        ks = ogood ? a.k_scale[at] * a.c : 0.f;
+        vs = ogood ? a.v_scale[at] : 0.f;
+    };
+    if (kb + wid * 64 < kend) {
+        look_up(kb + wid * 64);
+        load_keys(kb + wid * 64, kpage);
+        load_values(kb + wid * 64, opage);
+        look_up(kb + wid * 64 + 256);
+    }
+    for (int base = kb + wid * 64; base < kend; base += 256) {
+        const int okey = base + 16 * g;
+        const bool more = base + 256 < kend;
+        const int next_page = opage;
 
         f32x4_t x[4];
 #pragma unroll
@@ -229,6 +251,10 @@ __global__ __launch_bounds__(PGN_CA_THREADS) void pgn_cached_rows16_kernel(const
                 x[i] = Mat<DT>::mfma16(widen8<DT>(kw[i][s].z, kw[i][s].w, 1.f), qf[2 * s + 1], x[i]);
             }
             x[i] *= ks;
+        }
+        if (more) {
+            load_keys(base + 256, kpage);
+            look_up(base + 512);
         }
         // (a conversion reads only its scale's exponent: a scale of 0 has to clear the bytes instead)
         const bool ogive = ogood && vs != 0.f;
@@ -334,6 +360,7 @@ __global__ __launch_bounds__(PGN_CA_THREADS) void pgn_cached_rows16_kernel(const
             o[d] = Mat<DT>::mfma16(widen8<DT>(vw[d].x, vw[d].y, vmul), p[0], o[d]);
             o[d] = Mat<DT>::mfma16(widen8<DT>(vw[d].z, vw[d].w, vmul), p[1], o[d]);
         }
+        if (more) load_values(base + 256, next_page);
     }
 
     l += __shfl_xor(l, 16);
@@ -778,7 +805,9 @@ struct CachedPlan {
     int big_tiles, big_nsplit, big_split_keys;               // 128-row kernel; no tiles: not launched
 };
 
-// Splits of the keys so that `want` workgroups are there, each with `least` keys or more.
+// Splits of the keys so that `want` workgroups are there, each with `least` keys or more (256: one round of the 16-row
+// kernel's four waves).  Wanted are 512, which is what the CUs hold at a time: 143 us for 4 requests of up to 131072 keys
+// and 8 KV heads, against 146 with twice and 155 with four times as many and their larger join.
 static void split_keys(int64_t wgs, int64_t want, int64_t max_keys, int least, int* nsplit, int* keys) {
     const int64_t most = (max_keys + least - 1) / least;
     int64_t n = (want + wgs - 1) / wgs;
@@ -793,7 +822,7 @@ static CachedPlan cached_plan(int T, int R, bool packed, int G, int Hkv, int64_t
     const int few = packed ? (PGN_CA_FEW_ROWS < (int64_t)T * G ? PGN_CA_FEW_ROWS : T * G) : G;
     p.tiles_per_request = (few + 15) / 16;
     p.tiles = R * p.tiles_per_request;
-    split_keys((int64_t)(packed ? R : p.tiles) * Hkv, 1024, max_keys, 256, &p.nsplit, &p.split_keys);
+    split_keys((int64_t)(packed ? R : p.tiles) * Hkv, 512, max_keys, 256, &p.nsplit, &p.split_keys);
     p.big_tiles = packed && (int64_t)T * G > PGN_CA_FEW_ROWS ? (int)((int64_t)T * G / 128 + R) : 0;
     p.big_nsplit = 1;
     p.big_split_keys = 0;
