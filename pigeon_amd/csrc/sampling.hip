@@ -271,9 +271,10 @@ __device__ u64 select_key(SampleLds& s, const Row<DT>& row, const Weights& w, bo
     return prefix;
 }
 
-// Bin in which the running sum over the histogram reaches `target`, and the sum before it; the last bin if none does.
-template <typename T>
-__device__ int find_bin(SampleLds& s, const T* hist, T target, T& before) {
+// Bin in which the running sum over the histogram reaches target(sum of all), and the sum before it; the last bin if none
+// does.
+template <typename T, typename F>
+__device__ int find_bin(SampleLds& s, const T* hist, F target_of, T& before) {
     constexpr int PER = PGN_SAMPLE_BINS / PGN_SAMPLE_THREADS;
     T v[PER], sum = 0, total;
 #pragma unroll
@@ -283,6 +284,7 @@ __device__ int find_bin(SampleLds& s, const T* hist, T target, T& before) {
     }
     if (threadIdx.x == 0) s.at = PGN_SAMPLE_BINS - 1;
     T c = block_scan(sum, s.part, total) - sum;
+    const T target = target_of(total);
     T* out = reinterpret_cast<T*>(&s.before);
     if (threadIdx.x == 0) *out = total - hist[PGN_SAMPLE_BINS - 1];
     __syncthreads();
@@ -521,7 +523,7 @@ __global__ __launch_bounds__(PGN_SAMPLE_THREADS) void pgn_sample_tokens_kernel(c
         if (k <= PGN_SAMPLE_THREADS) {
             if (mine > -INFINITY) atomicAdd(&s.hist.ids[w.bin(mine)], 1u);
             __syncthreads();
-            const int cut = find_bin(s, s.hist.ids, (unsigned)k, before);      // the last bin too if there are fewer maxima
+            const int cut = find_bin(s, s.hist.ids, [&](unsigned) { return (unsigned)k; }, before);      // the last bin too if there are fewer maxima
             if (cut < PGN_SAMPLE_BINS - 1) {
                 const int n = gather(0, cut);
                 if (n <= PGN_SAMPLE_LIST) {
@@ -551,7 +553,7 @@ __global__ __launch_bounds__(PGN_SAMPLE_THREADS) void pgn_sample_tokens_kernel(c
         for (int i = tid; i < PGN_SAMPLE_BINS; i += PGN_SAMPLE_THREADS) sum += s.hist.ids[i];
         block_scan(sum, s.part, total);
         if (total > (unsigned)k) {
-            const int cut = find_bin(s, s.hist.ids, (unsigned)k, before);
+            const int cut = find_bin(s, s.hist.ids, [&](unsigned) { return (unsigned)k; }, before);
             const unsigned inside = s.hist.ids[cut];
             if (before + inside <= PGN_SAMPLE_LIST) {
                 const int n = gather(0, cut);
@@ -584,10 +586,8 @@ __global__ __launch_bounds__(PGN_SAMPLE_THREADS) void pgn_sample_tokens_kernel(c
             }
         });
         __syncthreads();
-        u64 sum = 0, before;
-        for (int i = tid; i < PGN_SAMPLE_BINS; i += PGN_SAMPLE_THREADS) sum += s.hist.mass[i];
-        target_p = nucleus_target(p, block_sum(sum, s.part));
-        cut = find_bin(s, s.hist.mass, target_p, before);
+        u64 before;
+        cut = find_bin(s, s.hist.mass, [&](u64 z) { return target_p = nucleus_target(p, z); }, before);
         inside_target = target_p - before;
     }
 
@@ -643,6 +643,24 @@ __global__ __launch_bounds__(PGN_SAMPLE_THREADS) void pgn_sample_tokens_kernel(c
         __syncthreads();
         if (!listed) break;
         const int n = s.count;
+        if (n <= PGN_SAMPLE_FEW) {                           // compared each with each
+            u64 key = 0, v = 0;
+            if (tid < n) s.weight[tid] = v = w.fixed(rank_value((unsigned)((key = s.key[tid]) >> 24)));
+            if (tid == 0) s.found = 0;
+            __syncthreads();
+            if (tid < n) {
+                u64 before = 0;
+                for (int j = 0; j < n; ++j) before += s.key[j] < key ? s.weight[j] : 0;
+                if (before < inside_target) {
+                    atomicMax(&s.found, key);
+                    if ((double)v >= least || v == 1ull << PGN_SAMPLE_BITS)
+                        atomicAdd(&s.seg[((int)(key & 0xffffff) + row.lead) / (64 * E)], v);
+                }
+            }
+            __syncthreads();
+            limit = min(limit, s.found);
+            break;
+        }
         if (n <= PGN_SAMPLE_LIST) {
             u64 total;
             for (int i = tid; i < n; i += PGN_SAMPLE_THREADS) s.weight[i] = w.fixed(rank_value((unsigned)(s.key[i] >> 24)));
