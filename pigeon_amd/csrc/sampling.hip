@@ -29,7 +29,6 @@
 #define PGN_SAMPLE_FEW 256                                   // ids that are compared each with each instead
 #define PGN_SAMPLE_TABLE 1024
 #define PGN_SAMPLE_BITS 45
-#define PGN_SAMPLE_AHEAD 4                                   // vectors of a row that a thread has in flight
 
 namespace {
 
@@ -59,7 +58,7 @@ struct SampleLds {
     u64 weight[PGN_SAMPLE_LIST];
     u64 seg[PGN_SAMPLE_MAX_IDS / 256 + PGN_SAMPLE_WAVES];    // kept weight of each 64 vectors (4 or 8 ids each) of the row
     double table[PGN_SAMPLE_TABLE];                          // 2^(-j / 1024)
-    u64 kept[PGN_SAMPLE_WAVES][128];                         // of each wave: kept logits and their indexes, 64 at a time
+    u64 pile[PGN_SAMPLE_WAVES][128];                         // of each wave: kept logits and their indexes, 64 at a time
     u64 part[PGN_SAMPLE_WAVES];
     u64 found, before;
     float fpart[PGN_SAMPLE_WAVES];
@@ -117,41 +116,56 @@ struct Row {
         }
     }
     // f(j, x[E]) for every vector of the row, in all threads equally often, some with vectors that hold nothing.  Vector j
-    // is thread j % 1024's.  The loads are free of branches and four of them are in flight.
-    template <typename F>
+    // is thread j % 1024's.  The loads are free of branches and AHEAD of them are in flight: four where the work on a vector
+    // is short, one where it hides the next load (every copy of the body is instructions to fetch, once a launch).
+    template <int AHEAD, typename F>
     __device__ __forceinline__ void each(F f) const {
         const int tid = threadIdx.x;
+        const auto load = [&](int j) {
+            return *reinterpret_cast<const uint4*>(first + (int64_t)min(max(j, whole_lo), whole_hi - 1) * E);
+        };
+        uint4 r[AHEAD];
         if (whole_hi > whole_lo) {
-            const auto load = [&](int j) {
-                return *reinterpret_cast<const uint4*>(first + (int64_t)min(max(j, whole_lo), whole_hi - 1) * E);
-            };
-            uint4 r[PGN_SAMPLE_AHEAD];
 #pragma unroll
-            for (int u = 0; u < PGN_SAMPLE_AHEAD; ++u) r[u] = load(u * PGN_SAMPLE_THREADS + tid);
-            for (int j0 = 0; j0 < whole_hi; j0 += PGN_SAMPLE_AHEAD * PGN_SAMPLE_THREADS) {
+            for (int u = 0; u < AHEAD; ++u) r[u] = load(u * PGN_SAMPLE_THREADS + tid);
+        }
+        const int rounds = whole_hi > whole_lo ? (whole_hi + PGN_SAMPLE_THREADS - 1) / PGN_SAMPLE_THREADS : 0;
+        const int all = rounds + (whole_lo > 0 || whole_hi < vectors);       // one more for the ends, two vectors at most
+        const int last = vectors - 1;
+        const int end = tid == 0 && whole_lo > 0 ? 0 : tid == 1 && whole_hi < vectors && (last > 0 || whole_lo == 0) ? last : vectors;
+#pragma unroll 1
+        for (int i0 = 0; i0 < all; i0 += AHEAD) {
 #pragma unroll
-                for (int u = 0; u < PGN_SAMPLE_AHEAD; ++u) {
-                    const int j1 = j0 + u * PGN_SAMPLE_THREADS, j = j1 + tid;
-                    if (j1 < whole_hi) {
-                        float x[E];
-                        unpack(r[u], x);
-                        r[u] = load(j + PGN_SAMPLE_AHEAD * PGN_SAMPLE_THREADS);
-                        if (j < whole_lo || j >= whole_hi) {
+            for (int u = 0; u < AHEAD; ++u) {
+                const int i = i0 + u;
+                if (i >= all) break;
+                float x[E];
+                int j = i * PGN_SAMPLE_THREADS + tid;
+                if (i < rounds) {
+                    unpack(r[u], x);
+                    r[u] = load(j + AHEAD * PGN_SAMPLE_THREADS);
+                    if (j < whole_lo || j >= whole_hi) {
 #pragma unroll
-                            for (int e = 0; e < E; ++e) x[e] = -INFINITY;
-                        }
-                        f(j, x);
+                        for (int e = 0; e < E; ++e) x[e] = -INFINITY;
                     }
+                } else {
+                    j = end;
+                    pick(j, x);
                 }
+                f(j, x);
             }
         }
-        if (whole_lo > 0 || whole_hi < vectors) {            // at most two vectors: the ends
-            const int last = vectors - 1;
-            const int j = tid == 0 && whole_lo > 0 ? 0 : tid == 1 && whole_hi < vectors && (last > 0 || whole_lo == 0) ? last : vectors;
-            float x[E];
-            pick(j, x);
-            f(j, x);
-        }
+    }
+};
+
+// The ids that a filter keeps: those above a logit, and those of that logit up to an index.
+struct Kept {
+    float x;
+    int i;
+    __device__ __forceinline__ bool operator()(float y, int j) const { return y > x || (y == x && j <= i); }
+    __device__ __forceinline__ void upto(u64 k) {
+        x = rank_value((unsigned)(k >> 24));
+        i = (int)(k & 0xffffff);
     }
 };
 
@@ -204,7 +218,7 @@ __device__ __forceinline__ T wave_scan(T v) {
 
 // inclusive prefix sum over the workgroup, and the sum of all
 template <typename T>
-__device__ T block_scan(T v, void* scratch, T& total) {
+__device__ __forceinline__ T block_scan(T v, void* scratch, T& total) {
     T* part = reinterpret_cast<T*>(scratch);
     const int wid = threadIdx.x >> 6;
     v = wave_scan(v);
@@ -240,10 +254,11 @@ __device__ __forceinline__ void digit_add(u64* hist, int b, u64 v) {
     }
 }
 
-// The key up to which the ids (of keys up to `limit`) hold `target` together, ids counted or weights summed, by eight bits
+// The key up to which the kept ids hold `target` together, ids counted or weights summed, by eight bits
 // of the key at a time over the whole row.
 template <int DT>
-__device__ u64 select_key(SampleLds& s, const Row<DT>& row, const Weights& w, bool by_weight, u64 target, u64 limit) {
+__device__ __forceinline__ u64 select_key(SampleLds& s, const Row<DT>& row, const Weights& w, bool by_weight, u64 target,
+                                          const Kept& kept) {
     u64 prefix = 0, before = 0;
     const int tid = threadIdx.x;
     for (int shift = 48; shift >= 0; shift -= 8) {
@@ -253,7 +268,7 @@ __device__ u64 select_key(SampleLds& s, const Row<DT>& row, const Weights& w, bo
         for (int i0 = 0; i0 < row.V; i0 += PGN_SAMPLE_THREADS) {
             const float x = i0 + tid < row.V ? row.one(i0 + tid) : -INFINITY;
             const u64 key = rank_key(x, i0 + tid);
-            const bool on = x > -INFINITY && key <= limit && (key >> (shift + 8)) == prefix;
+            const bool on = kept(x, i0 + tid) && (key >> (shift + 8)) == prefix;
             digit_add(s.hist.digit, (int)(key >> shift) & 255, !on ? 0 : by_weight ? w.fixed(x) : 1);
         }
         __syncthreads();
@@ -274,7 +289,7 @@ __device__ u64 select_key(SampleLds& s, const Row<DT>& row, const Weights& w, bo
 // Bin in which the running sum over the histogram reaches target(sum of all), and the sum before it; the last bin if none
 // does.
 template <typename T, typename F>
-__device__ int find_bin(SampleLds& s, const T* hist, F target_of, T& before) {
+__device__ __forceinline__ int find_bin(SampleLds& s, const T* hist, F target_of, T& before) {
     constexpr int PER = PGN_SAMPLE_BINS / PGN_SAMPLE_THREADS;
     T v[PER], sum = 0, total;
 #pragma unroll
@@ -304,7 +319,7 @@ __device__ int find_bin(SampleLds& s, const T* hist, F target_of, T& before) {
 }
 
 // Ascending sort of n keys (n a power of two, the list filled up to it), their weights with them.
-__device__ void sort_list(SampleLds& s, int n) {
+__device__ __forceinline__ void sort_list(SampleLds& s, int n) {
     for (int size = 2; size <= n; size <<= 1)
         for (int step = size >> 1; step > 0; step >>= 1) {
             __syncthreads();
@@ -324,7 +339,7 @@ __device__ void sort_list(SampleLds& s, int n) {
 }
 
 // Fills the list up to a power of two with what sorts last and weighs nothing.
-__device__ int pad_list(SampleLds& s, int n) {
+__device__ __forceinline__ int pad_list(SampleLds& s, int n) {
     int m = 2;
     while (m < n) m <<= 1;
     for (int i = n + threadIdx.x; i < m; i += PGN_SAMPLE_THREADS) {
@@ -335,7 +350,7 @@ __device__ int pad_list(SampleLds& s, int n) {
 }
 
 // First place of the list at which the running sum of weights reaches `target`; n - 1 if none.
-__device__ int find_place(SampleLds& s, int n, u64 target, u64& total) {
+__device__ __forceinline__ int find_place(SampleLds& s, int n, u64 target, u64& total) {
     constexpr int PER = PGN_SAMPLE_LIST / PGN_SAMPLE_THREADS;
     u64 v[PER], sum = 0;
 #pragma unroll
@@ -374,7 +389,7 @@ __device__ __forceinline__ u64 nucleus_target(float p, u64 z) {
 // The rest of a top-k among the n ids of the list, the first k in rank among them: top-p, min-p and the draw.  `least`:
 // min-p as a weight.  A few ids compare each with each (ranks and running sums without a sort, three rounds); more are
 // sorted by rank, then by index.
-__device__ void finish_list(SampleLds& s, const Weights& w, int n, int k, float p, double least, float u, int64_t* id) {
+__device__ __forceinline__ void finish_list(SampleLds& s, const Weights& w, int n, int k, float p, double least, float u, int64_t* id) {
     const int tid = threadIdx.x;
     const u64 one = 1ull << PGN_SAMPLE_BITS;
     u64 z;
@@ -383,6 +398,7 @@ __device__ void finish_list(SampleLds& s, const Weights& w, int n, int k, float 
         if (tid < n) {
             key = s.key[tid];
             int rank = 0;
+#pragma unroll 8
             for (int j = 0; j < n; ++j) rank += s.key[j] < key;
             v = rank < k ? w.fixed(rank_value((unsigned)(key >> 24))) : 0;
             s.weight[tid] = v;
@@ -392,6 +408,7 @@ __device__ void finish_list(SampleLds& s, const Weights& w, int n, int k, float 
             const u64 target = nucleus_target(p, all);
             if (tid < n) {
                 u64 before = 0;
+#pragma unroll 8
                 for (int j = 0; j < n; ++j) before += s.key[j] < key ? s.weight[j] : 0;
                 v = before < target ? v : 0;
             }
@@ -404,6 +421,7 @@ __device__ void finish_list(SampleLds& s, const Weights& w, int n, int k, float 
         if (tid < n && v > 0) {
             const unsigned i = (unsigned)key & 0xffffff;
             u64 upto = 0;
+#pragma unroll 8
             for (int j = 0; j < n; ++j) upto += ((unsigned)s.key[j] & 0xffffff) <= i ? s.weight[j] : 0;
             if (upto >= draw_target(u, z)) atomicMin(&s.found, (u64)i);
         }
@@ -446,7 +464,7 @@ __global__ __launch_bounds__(PGN_SAMPLE_THREADS) void pgn_sample_tokens_kernel(c
     const float u = a.u[b];
 
     float mine = -INFINITY;                                  // the thread's own maximum
-    row.each([&](int, const float* x) {
+    row.template each<4>([&](int, const float* x) {
 #pragma unroll
         for (int e = 0; e < E; ++e) mine = fmaxf(mine, x[e]);
     });
@@ -466,7 +484,7 @@ __global__ __launch_bounds__(PGN_SAMPLE_THREADS) void pgn_sample_tokens_kernel(c
     }
     if (!(t > 0.f) || p <= 0.f || k == 1) {                  // the first in rank: the lowest index of the largest logit
         int at = V;
-        row.each([&](int j, const float* x) {
+        row.template each<1>([&](int j, const float* x) {
 #pragma unroll
             for (int e = E - 1; e >= 0; --e) at = x[e] == m ? min(at, row.index(j, e)) : at;
         });
@@ -488,27 +506,30 @@ __global__ __launch_bounds__(PGN_SAMPLE_THREADS) void pgn_sample_tokens_kernel(c
     w.fc = (float)(PGN_SAMPLE_BINS_PER_OCTAVE * 1.44269504088896340736 / (double)t);
     w.table = s.table;
     const double least = (double)min_p * (double)(1ull << PGN_SAMPLE_BITS);
-    u64 limit = ~0ull;                                       // keys up to it are kept
+    Kept kept = {-INFINITY, -1};                             // everything that can be drawn
 
-    // gathers the ids of bins [from, to]; how many there are (the list takes PGN_SAMPLE_LIST of them)
-    const auto gather = [&](int from, int to) {
+    // a logit that no id of a bin up to `bin` is under (1 % of a bin and an ulp cover the rounding of the places)
+    const auto lowest = [&](int bin) {
+        const float x = (float)(w.max - (bin + 1.01) / (double)w.fc);
+        if (bin >= PGN_SAMPLE_BINS - 1 || x != x) return -INFINITY;      // the last bin has no end; inf - inf
+        return fabsf(x) < INFINITY ? x - fabsf(x) * 0x1p-23f : x;
+    };
+    // gathers the ids from `low` up, of all bins or of one; how many there are (the list takes PGN_SAMPLE_LIST of them)
+    const auto gather = [&](float low, int only) {
         __syncthreads();
         if (tid == 0) s.count = 0;
         __syncthreads();
-        row.each([&](int j, const float* x) {
+        row.template each<4>([&](int j, const float* x) {
             unsigned in = 0;
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const int bin = w.bin(x[e]);
-                in |= x[e] > -INFINITY && bin >= from && bin <= to ? 1u << e : 0u;
-            }
+            for (int e = 0; e < E; ++e) in |= x[e] >= low ? 1u << e : 0u;
 #pragma unroll 1
             for (; __any(in != 0); in &= in - 1) {           // one id a lane at a time
                 const int e = in ? __builtin_ctz(in) : 0;
                 float xe = x[0];
 #pragma unroll
                 for (int n = 1; n < E; ++n) xe = e == n ? x[n] : xe;
-                if (in) {
+                if (in && xe > -INFINITY && (only < 0 || w.bin(xe) == only)) {
                     const int at = atomicAdd(&s.count, 1);
                     if (at < PGN_SAMPLE_LIST) s.key[at] = rank_key(xe, row.index(j, e));
                 }
@@ -519,13 +540,40 @@ __global__ __launch_bounds__(PGN_SAMPLE_THREADS) void pgn_sample_tokens_kernel(c
     };
 
     if (k > 0 && k < V) {
-        unsigned before, total;
-        if (k <= PGN_SAMPLE_THREADS) {
-            if (mine > -INFINITY) atomicAdd(&s.hist.ids[w.bin(mine)], 1u);
+        for (bool full = k > PGN_SAMPLE_THREADS;; full = true) {
+            unsigned total = 0, before;
+            if (!full) {
+                if (mine > -INFINITY) atomicAdd(&s.hist.ids[w.bin(mine)], 1u);
+            } else {                                         // the last bin may hold most of a row: counted in registers
+                unsigned last = 0;
+                row.template each<1>([&](int, const float* x) {
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        const int bin = w.bin(x[e]);
+                        const bool is = x[e] > -INFINITY;
+                        if (is && bin < PGN_SAMPLE_BINS - 1) atomicAdd(&s.hist.ids[bin], 1u);
+                        last += is && bin == PGN_SAMPLE_BINS - 1;
+                    }
+                });
+                block_scan(last, s.part, total);
+                if (tid == 0) s.hist.ids[PGN_SAMPLE_BINS - 1] = total;
+            }
             __syncthreads();
-            const int cut = find_bin(s, s.hist.ids, [&](unsigned) { return (unsigned)k; }, before);      // the last bin too if there are fewer maxima
-            if (cut < PGN_SAMPLE_BINS - 1) {
-                const int n = gather(0, cut);
+            const int cut = find_bin(s, s.hist.ids, [&](unsigned z) { total = z; return (unsigned)k; }, before);
+            if (full && total <= (unsigned)k) break;         // everything is among the first k
+            const unsigned inside = s.hist.ids[cut];
+            const bool alone = full && before + inside > PGN_SAMPLE_LIST;        // only the border is looked for in the list
+            if (alone && inside > PGN_SAMPLE_LIST) {
+                kept.upto(select_key<DT>(s, row, w, false, (u64)k, kept));
+                break;
+            }
+            if (full || cut < PGN_SAMPLE_BINS - 1) {         // else there are fewer maxima than k
+                const int n = gather(lowest(cut), alone ? cut : -1);
+                if (alone) {
+                    sort_list(s, pad_list(s, n));
+                    kept.upto(s.key[k - (int)before - 1]);
+                    break;
+                }
                 if (n <= PGN_SAMPLE_LIST) {
                     finish_list(s, w, n, k, p, least, u, a.ids + b);
                     return;
@@ -535,54 +583,20 @@ __global__ __launch_bounds__(PGN_SAMPLE_THREADS) void pgn_sample_tokens_kernel(c
             for (int i = tid; i < PGN_SAMPLE_BINS; i += PGN_SAMPLE_THREADS) s.hist.ids[i] = 0;
             __syncthreads();
         }
-        // all ids by bins; the last bin, which may hold most of a row, is counted in registers
-        unsigned last = 0;
-        row.each([&](int, const float* x) {
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const int bin = w.bin(x[e]);
-                const bool is = x[e] > -INFINITY;
-                if (is && bin < PGN_SAMPLE_BINS - 1) atomicAdd(&s.hist.ids[bin], 1u);
-                last += is && bin == PGN_SAMPLE_BINS - 1;
-            }
-        });
-        block_scan(last, s.part, total);
-        if (tid == 0) s.hist.ids[PGN_SAMPLE_BINS - 1] = total;
-        __syncthreads();
-        unsigned sum = 0;
-        for (int i = tid; i < PGN_SAMPLE_BINS; i += PGN_SAMPLE_THREADS) sum += s.hist.ids[i];
-        block_scan(sum, s.part, total);
-        if (total > (unsigned)k) {
-            const int cut = find_bin(s, s.hist.ids, [&](unsigned) { return (unsigned)k; }, before);
-            const unsigned inside = s.hist.ids[cut];
-            if (before + inside <= PGN_SAMPLE_LIST) {
-                const int n = gather(0, cut);
-                finish_list(s, w, n, k, p, least, u, a.ids + b);
-                return;
-            }
-            if (inside <= PGN_SAMPLE_LIST) {                 // many ids are kept: only the border is looked for in the list
-                const int n = gather(cut, cut);
-                sort_list(s, pad_list(s, n));
-                limit = s.key[k - (int)before - 1];
-            } else {
-                limit = select_key<DT>(s, row, w, false, (u64)k, limit);
-            }
-        }
         __syncthreads();
     }
 
-    int cut = PGN_SAMPLE_BINS;                               // bins before it are kept whole (as far as `limit` goes)
+    int cut = PGN_SAMPLE_BINS;                               // bins before it are kept whole (as far as `kept` goes)
     u64 target_p = 0, inside_target = 0;
     if (p < 1.f) {
         for (int i = tid; i < PGN_SAMPLE_BINS; i += PGN_SAMPLE_THREADS) s.hist.mass[i] = 0;
         if (tid == 0) s.count = 0;
         __syncthreads();
-        row.each([&](int j, const float* x) {
+        row.template each<1>([&](int j, const float* x) {
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                u64 v = w.fixed(x[e]);
-                if (limit != ~0ull) v = rank_key(x[e], row.index(j, e)) <= limit ? v : 0;
-                if (v > 0) atomicAdd(&s.hist.mass[w.bin(x[e])], v);
+                const u64 v = w.fixed(x[e]);
+                if (v > 0 && kept(x[e], row.index(j, e))) atomicAdd(&s.hist.mass[w.bin(x[e])], v);
             }
         });
         __syncthreads();
@@ -598,19 +612,24 @@ __global__ __launch_bounds__(PGN_SAMPLE_THREADS) void pgn_sample_tokens_kernel(c
         for (int i = tid; i < segs; i += PGN_SAMPLE_THREADS) s.seg[i] = 0;
         __syncthreads();
         // Few ids may be kept, and a weight is dear: every wave collects kept logits until it has 64 to weigh.
-        u64* kept = s.kept[wid];
+        u64* pile = s.pile[wid];
         int held = 0;
         const auto weigh = [&](bool on, u64 entry) {
             const u64 v = on ? w.fixed(__uint_as_float((unsigned)entry)) : 0;
             if (on && ((double)v >= least || v == 1ull << PGN_SAMPLE_BITS))
                 atomicAdd(&s.seg[((int)(entry >> 32) + row.lead) / (64 * E)], v);
         };
-        row.each([&](int j, const float* x) {
+        const float low = cut < PGN_SAMPLE_BINS ? lowest(cut) : -INFINITY;
+        row.template each<1>([&](int j, const float* x) {
+            float largest = x[0];
+#pragma unroll
+            for (int e = 1; e < E; ++e) largest = fmaxf(largest, x[e]);
+            if (!__any(largest >= low)) return;
             unsigned in = 0, at_edge = 0;
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 const int bin = w.bin(x[e]);
-                const bool on = x[e] > -INFINITY && (limit == ~0ull || rank_key(x[e], row.index(j, e)) <= limit);
+                const bool on = kept(x[e], row.index(j, e));
                 in |= on && bin < cut ? 1u << e : 0u;
                 at_edge |= on && bin == cut ? 1u << e : 0u;
             }
@@ -626,20 +645,20 @@ __global__ __launch_bounds__(PGN_SAMPLE_THREADS) void pgn_sample_tokens_kernel(c
                     if (at < PGN_SAMPLE_LIST) s.key[at] = rank_key(xe, i);
                 }
                 const uint64_t lanes = __ballot(bit < 8);
-                if (bit < 8) kept[held + __popcll(lanes & ((1ull << lane) - 1))] = ((u64)(unsigned)i << 32) | __float_as_uint(xe);
+                if (bit < 8) pile[held + __popcll(lanes & ((1ull << lane) - 1))] = ((u64)(unsigned)i << 32) | __float_as_uint(xe);
                 held += __popcll(lanes);
                 if (held >= 64) {
                     __builtin_amdgcn_wave_barrier();
-                    weigh(true, kept[lane]);
+                    weigh(true, pile[lane]);
                     held -= 64;
-                    const u64 rest = kept[64 + lane];
+                    const u64 rest = pile[64 + lane];
                     __builtin_amdgcn_wave_barrier();
-                    if (lane < held) kept[lane] = rest;
+                    if (lane < held) pile[lane] = rest;
                 }
             }
         });
         __builtin_amdgcn_wave_barrier();
-        weigh(lane < held, kept[lane]);
+        weigh(lane < held, pile[lane]);
         __syncthreads();
         if (!listed) break;
         const int n = s.count;
@@ -650,6 +669,7 @@ __global__ __launch_bounds__(PGN_SAMPLE_THREADS) void pgn_sample_tokens_kernel(c
             __syncthreads();
             if (tid < n) {
                 u64 before = 0;
+#pragma unroll 8
                 for (int j = 0; j < n; ++j) before += s.key[j] < key ? s.weight[j] : 0;
                 if (before < inside_target) {
                     atomicMax(&s.found, key);
@@ -658,7 +678,7 @@ __global__ __launch_bounds__(PGN_SAMPLE_THREADS) void pgn_sample_tokens_kernel(c
                 }
             }
             __syncthreads();
-            limit = min(limit, s.found);
+            kept.upto(s.found);                              // under the top-k's border, if there is one
             break;
         }
         if (n <= PGN_SAMPLE_LIST) {
@@ -666,7 +686,7 @@ __global__ __launch_bounds__(PGN_SAMPLE_THREADS) void pgn_sample_tokens_kernel(c
             for (int i = tid; i < n; i += PGN_SAMPLE_THREADS) s.weight[i] = w.fixed(rank_value((unsigned)(s.key[i] >> 24)));
             sort_list(s, pad_list(s, n));
             const int last = find_place(s, n, inside_target, total);
-            limit = min(limit, s.key[last]);
+            kept.upto(s.key[last]);
             for (int i = tid; i <= last; i += PGN_SAMPLE_THREADS) {
                 const u64 v = s.weight[i];
                 if ((double)v >= least || v == 1ull << PGN_SAMPLE_BITS)
@@ -675,7 +695,7 @@ __global__ __launch_bounds__(PGN_SAMPLE_THREADS) void pgn_sample_tokens_kernel(c
             __syncthreads();
             break;
         }
-        limit = select_key<DT>(s, row, w, true, target_p, limit);
+        kept.upto(select_key<DT>(s, row, w, true, target_p, kept));
         cut = PGN_SAMPLE_BINS;
         listed = false;
         __syncthreads();
@@ -705,7 +725,7 @@ __global__ __launch_bounds__(PGN_SAMPLE_THREADS) void pgn_sample_tokens_kernel(c
     row.pick(j, x);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-        const u64 f = x[e] > -INFINITY && rank_key(x[e], row.index(j, e)) <= limit ? w.fixed(x[e]) : 0;
+        const u64 f = kept(x[e], row.index(j, e)) ? w.fixed(x[e]) : 0;
         v[e] = (double)f >= least || x[e] == m ? f : 0;
         sum += v[e];
     }
