@@ -409,7 +409,10 @@ __device__ __forceinline__ void finish_list(SampleLds& s, const Weights& w, int 
             if (tid < n) {
                 u64 before = 0;
 #pragma unroll 8
-                for (int j = 0; j < n; ++j) before += s.key[j] < key ? s.weight[j] : 0;
+                for (int j = 0; j < n; ++j) {
+                    const u64 other = s.key[j], weight = s.weight[j];        // both loads at once, not the one for the other
+                    before += other < key ? weight : 0;
+                }
                 v = before < target ? v : 0;
             }
         }
@@ -422,7 +425,10 @@ __device__ __forceinline__ void finish_list(SampleLds& s, const Weights& w, int 
             const unsigned i = (unsigned)key & 0xffffff;
             u64 upto = 0;
 #pragma unroll 8
-            for (int j = 0; j < n; ++j) upto += ((unsigned)s.key[j] & 0xffffff) <= i ? s.weight[j] : 0;
+            for (int j = 0; j < n; ++j) {
+                const u64 other = s.key[j], weight = s.weight[j];
+                upto += ((unsigned)other & 0xffffff) <= i ? weight : 0;
+            }
             if (upto >= draw_target(u, z)) atomicMin(&s.found, (u64)i);
         }
         __syncthreads();
@@ -670,7 +676,10 @@ __global__ __launch_bounds__(PGN_SAMPLE_THREADS) void pgn_sample_tokens_kernel(c
             if (tid < n) {
                 u64 before = 0;
 #pragma unroll 8
-                for (int j = 0; j < n; ++j) before += s.key[j] < key ? s.weight[j] : 0;
+                for (int j = 0; j < n; ++j) {
+                    const u64 other = s.key[j], weight = s.weight[j];
+                    before += other < key ? weight : 0;
+                }
                 if (before < inside_target) {
                     atomicMax(&s.found, key);
                     if ((double)v >= least || v == 1ull << PGN_SAMPLE_BITS)
