@@ -76,7 +76,7 @@ __device__ __forceinline__ float rank_value(unsigned r) {
 __device__ __forceinline__ u64 rank_key(float x, int i) { return ((u64)rank_bits(x) << 24) | (unsigned)i; }
 
 // NaN counts as a logit of -inf; -0 as 0, so that the two tie as they compare
-__device__ __forceinline__ float clean(float x) { return x != x ? -INFINITY : x + 0.f; }
+__device__ __forceinline__ float clean(float x) { return fmaxf(x + 0.f, -INFINITY); }
 
 // A row in 16-byte vectors.  It may begin at any element: vector 0 is the aligned one that holds its first element.  The
 // vectors that reach over an end are put together from single loads, with -inf where there is no id.
@@ -170,15 +170,14 @@ struct Kept {
 };
 
 struct Weights {
-    double max, c;                                           // c: 1024 log2(e) / temperature
+    double max, c;                                           // c: 1024 log2(e) / temperature, not 0
     float fmax, fc;                                          // fc: bins per unit of distance
     const double* table;
     // w 2^45, nearest whole number.  2^-(t / 1024) with t = k + f, k whole, |f| <= 1/2: a table of 2^-(k % 1024 / 1024),
     // an exponent, and e^-(f ln2 / 1024) as its series up to the third power (the fourth is 2^-50).  Beyond 2^-47 the
-    // result is 0 by itself; an infinite maximum leaves only its equals.
+    // result is 0 by itself; an infinite maximum leaves only its equals (inf - inf is a NaN, and fmax takes 0 for it).
     __device__ __forceinline__ u64 fixed(float x) const {
-        const double dx = x == fmax ? 0.0 : max - (double)x;
-        const double t = fmin(dx * c, 1024.0 * (PGN_SAMPLE_BITS + 2));       // a NaN (inf * 0) too
+        const double t = fmin(::fmax((max - (double)x) * c, 0.0), 1024.0 * (PGN_SAMPLE_BITS + 2));
         const double d = t + 0x1.8p52;
         const int k = (int)(unsigned)(u64)__double_as_longlong(d);
         const double f = t - (d - 0x1.8p52);
@@ -187,9 +186,9 @@ struct Weights {
         const double up = __hiloint2double((1023 + PGN_SAMPLE_BITS - (k >> 10)) << 20, 0);
         return (u64)__double_as_longlong(fma(e, up, 0x1p52)) & 0xfffffffffffffull;
     }
-    // monotone in x: 32 bins to a factor of two, everything from 2^-64 on in the last
+    // monotone in x > -inf: 32 bins to a factor of two, everything from 2^-64 on in the last; a NaN (inf - inf, 0 inf) is 0
     __device__ __forceinline__ int bin(float x) const {
-        return (int)fminf(x == fmax ? 0.f : (fmax - x) * fc, (float)(PGN_SAMPLE_BINS - 1));
+        return (int)fminf(fmaxf((fmax - x) * fc, 0.f), (float)(PGN_SAMPLE_BINS - 1));
     }
 };
 
@@ -508,7 +507,7 @@ __global__ __launch_bounds__(PGN_SAMPLE_THREADS) void pgn_sample_tokens_kernel(c
     Weights w;
     w.max = m;
     w.fmax = m;
-    w.c = PGN_SAMPLE_TABLE * 1.44269504088896340736 / (double)t;
+    w.c = fmax(PGN_SAMPLE_TABLE * 1.44269504088896340736 / (double)t, 1e-300);        // t may be infinite
     w.fc = (float)(PGN_SAMPLE_BINS_PER_OCTAVE * 1.44269504088896340736 / (double)t);
     w.table = s.table;
     const double least = (double)min_p * (double)(1ull << PGN_SAMPLE_BITS);
@@ -598,11 +597,12 @@ __global__ __launch_bounds__(PGN_SAMPLE_THREADS) void pgn_sample_tokens_kernel(c
         for (int i = tid; i < PGN_SAMPLE_BINS; i += PGN_SAMPLE_THREADS) s.hist.mass[i] = 0;
         if (tid == 0) s.count = 0;
         __syncthreads();
+        const bool filtered = kept.x > -INFINITY;
         row.template each<1>([&](int j, const float* x) {
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 const u64 v = w.fixed(x[e]);
-                if (v > 0 && kept(x[e], row.index(j, e))) atomicAdd(&s.hist.mass[w.bin(x[e])], v);
+                if (v > 0 && (!filtered || kept(x[e], row.index(j, e)))) atomicAdd(&s.hist.mass[w.bin(x[e])], v);
             }
         });
         __syncthreads();
@@ -627,31 +627,22 @@ __global__ __launch_bounds__(PGN_SAMPLE_THREADS) void pgn_sample_tokens_kernel(c
         };
         const float low = cut < PGN_SAMPLE_BINS ? lowest(cut) : -INFINITY;
         row.template each<1>([&](int j, const float* x) {
-            float largest = x[0];
+            unsigned in = 0;
 #pragma unroll
-            for (int e = 1; e < E; ++e) largest = fmaxf(largest, x[e]);
-            if (!__any(largest >= low)) return;
-            unsigned in = 0, at_edge = 0;
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const int bin = w.bin(x[e]);
-                const bool on = kept(x[e], row.index(j, e));
-                in |= on && bin < cut ? 1u << e : 0u;
-                at_edge |= on && bin == cut ? 1u << e : 0u;
-            }
-            in |= at_edge << 8;
+            for (int e = 0; e < E; ++e) in |= x[e] >= low ? 1u << e : 0u;
 #pragma unroll 1
             for (; __any(in != 0); in &= in - 1) {           // one id a lane at a time
-                const int bit = in ? __builtin_ctz(in) : 31, e = bit & 7, i = row.index(j, e);
+                const int e = in ? __builtin_ctz(in) : 0, i = row.index(j, e);
                 float xe = x[0];
 #pragma unroll
                 for (int n = 1; n < E; ++n) xe = e == n ? x[n] : xe;
-                if (bit >= 8 && bit < 16) {
+                const int bin = in && kept(xe, i) ? w.bin(xe) : PGN_SAMPLE_BINS + 1;
+                if (bin == cut) {
                     const int at = atomicAdd(&s.count, 1);
                     if (at < PGN_SAMPLE_LIST) s.key[at] = rank_key(xe, i);
                 }
-                const uint64_t lanes = __ballot(bit < 8);
-                if (bit < 8) pile[held + __popcll(lanes & ((1ull << lane) - 1))] = ((u64)(unsigned)i << 32) | __float_as_uint(xe);
+                const uint64_t lanes = __ballot(bin < cut);
+                if (bin < cut) pile[held + __popcll(lanes & ((1ull << lane) - 1))] = ((u64)(unsigned)i << 32) | __float_as_uint(xe);
                 held += __popcll(lanes);
                 if (held >= 64) {
                     __builtin_amdgcn_wave_barrier();
