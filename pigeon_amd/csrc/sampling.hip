@@ -599,11 +599,16 @@ __global__ __launch_bounds__(PGN_SAMPLE_THREADS) void pgn_sample_tokens_kernel(c
         __syncthreads();
         const bool filtered = kept.x > -INFINITY;
         row.template each<1>([&](int j, const float* x) {
+            u64 v[E];                                        // all of them before the first addition: chains side by side
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const u64 v = w.fixed(x[e]);
-                if (v > 0 && (!filtered || kept(x[e], row.index(j, e)))) atomicAdd(&s.hist.mass[w.bin(x[e])], v);
+            for (int e = 0; e < E; ++e) v[e] = w.fixed(x[e]);
+            if (filtered) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[e] = kept(x[e], row.index(j, e)) ? v[e] : 0;
             }
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (v[e] > 0) atomicAdd(&s.hist.mass[w.bin(x[e])], v[e]);
         });
         __syncthreads();
         u64 before;
