@@ -9,8 +9,10 @@
 // some key: top-k the one where k ids, top-p the one where the wanted weight is reached.  That key is found without
 // sorting the row, by bins over the distance to the maximum (2048 bins, 32 to a factor of two of weight).
 //
-// One workgroup of 1024 threads takes a row.  It is bound by the passes over the row, whose loads only the first time
-// come from HBM, and by what each id costs in them (a CU spends some 1.5 cycles a 64-id instruction), so:
+// One workgroup of 1024 threads takes a row.  It is bound by what each id costs in the passes over the row, in
+// instructions and in LDS, whose loads only the first time come from HBM, and for short rows by the steps between them, each
+// with its barriers (some 20 of 0.3 us).  256 bf16 rows of 131072 with top-p take 91 us, 14 of them for the first pass (67 MB at
+// 4.8 TB/s), 33 for the bins and 11 to 21 for the stretches; 64 rows of 48386 with a top-k of 50 19 us; one fp32 row 27 us.
 //   top-k   the k-th largest of the 1024 threads' own maxima, known after the first pass, is at most the k-th largest
 //           logit: one more pass gathers what is not below its bin, some 1.1 k ids, and the rest (k, p, min-p, draw) is
 //           done among those in LDS;
@@ -626,9 +628,15 @@ __global__ __launch_bounds__(PGN_SAMPLE_THREADS) void pgn_sample_tokens_kernel(c
         u64* pile = s.pile[wid];
         int held = 0;
         const auto weigh = [&](bool on, u64 entry) {
-            const u64 v = on ? w.fixed(__uint_as_float((unsigned)entry)) : 0;
-            if (on && ((double)v >= least || v == 1ull << PGN_SAMPLE_BITS))
-                atomicAdd(&s.seg[((int)(entry >> 32) + row.lead) / (64 * E)], v);
+            u64 v = on ? w.fixed(__uint_as_float((unsigned)entry)) : 0;
+            if (!((double)v >= least || v == 1ull << PGN_SAMPLE_BITS)) v = 0;
+            const int at = on ? ((int)(entry >> 32) + row.lead) / (64 * E) : 0;
+            if (__all(at == __builtin_amdgcn_readfirstlane(at))) {           // one stretch: summed here, not by 64 turns in LDS
+                v = wave_scan(v);
+                if (lane == 63) atomicAdd(&s.seg[at], v);
+            } else if (v > 0) {
+                atomicAdd(&s.seg[at], v);
+            }
         };
         const float low = cut < PGN_SAMPLE_BINS ? lowest(cut) : -INFINITY;
         row.template each<1>([&](int j, const float* x) {
