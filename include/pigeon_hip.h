@@ -412,7 +412,7 @@ int pgn_image_to_uint8(const void* x, int x_dtype, void* y, int N, int C, int H,
  * are: nobody who needs pages overtakes.  status int32 [R] is 0 otherwise.
  * starts int32 [R+1]: where each request's new tokens begin (prefix sums of add, at most num_slots); slots int64
  * [num_slots]: their slots, -1 behind the last.  lens becomes the tokens held after the step.  Table entries behind a
- * request's pages are left as they were.  One workgroup and, above 8192 slots, a second launch for the slot map. */
+ * request's pages are left as they were.  One workgroup and, above 4096 slots, a second launch for the slot map. */
 int pgn_page_advance(int32_t* lens, const int32_t* keep, const int32_t* add, int32_t* table, int64_t table_stride,
                      int32_t* free_pages, int32_t* free_count, int num_pages, int R, int W, int page_size,
                      int64_t num_slots, int64_t* slots, int32_t* starts, int32_t* status, void* stream);

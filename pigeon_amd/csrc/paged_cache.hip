@@ -18,11 +18,12 @@ namespace {
 // added, pages wanted) whose results every later step needs, 4 bytes a request.  The pages themselves are then moved
 // flat, one thread a page: a thread finds its request by bisection in the prefix sums, which lie in LDS.
 // A chain of short steps is bound by their latency, and a barrier of 16 waves is the longest of them, so a small call
-// runs in one wave or four.
+// runs in one wave or four (back to back on the GPU: 64 requests and slots 3.5 us in one wave, 4.0 in four, 5.5 in 16;
+// 512 slots 8.9, 6.4, 7.9; 256 requests and slots 15.0, 5.8, 7.9; 2048 slots 32, 11, 9).
 #define PGN_ADV_THREADS 1024
 // Up to this many slots the bookkeeping workgroup fills the slot map itself (one launch); above it a second, wide launch
-// does.  At 8192 slots the workgroup's 8 rounds cost what the second launch would.
-#define PGN_ADV_FUSED_SLOTS 8192
+// does (2048 slots: 8.9 us against 10.1; 8192: 14.4 against 10.5; 16384: 22 against 11).
+#define PGN_ADV_FUSED_SLOTS 4096
 
 __device__ __forceinline__ int64_t adv_pages(int64_t tokens, int shift) {
     return (tokens + ((int64_t)1 << shift) - 1) >> shift;
@@ -230,7 +231,8 @@ __global__ __launch_bounds__(256) void pgn_page_slots_kernel(const int* __restri
 // A run is a stretch of consecutive tokens whose slots follow one another inside one page; the slot map makes at most
 // one run of a page in a call.  One workgroup takes the runs that begin among its `chunk` tokens, for one head and one
 // of the two halves, so it owns the (page, head) pairs that it writes: their scale is found, the older tokens of the
-// page are rescaled if it grew, and the new ones are stored, with no exchange between workgroups.
+// page are rescaled if it grew, and the new ones are stored, with no exchange between workgroups.  Its four waves share
+// a run of more than 16 tokens and take shorter ones each for itself.
 //
 // A wave keeps 16 rows in registers between finding the largest magnitude and storing, so a run of up to 64 tokens is
 // read once.  Keys: 8 consecutive dims a lane, 16 bytes in and 8 out.  Values: the 16 page rows by D / 64 consecutive
@@ -296,58 +298,65 @@ __device__ __forceinline__ CwVec<N> cw_load(const unsigned short* p, bool vec) {
     return v;
 }
 
-// The largest pattern over the workgroup.
-template <int NW>
-__device__ __forceinline__ unsigned cw_block_max(unsigned amax, unsigned* wave_max) {
+#define PGN_CW_WAVES 4
+
+// The waves that work on a run together: all of the workgroup, or one.
+struct CwTeam {
+    int all, tid, threads;
+    unsigned* wave_max;
+};
+
+// The largest pattern over the team.
+__device__ __forceinline__ unsigned cw_team_max(unsigned amax, const CwTeam& g) {
     amax = max(amax & 0xffffu, amax >> 16);
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) amax = max(amax, (unsigned)__shfl_xor((int)amax, off));
-    if constexpr (NW > 1) {
+    if (g.all) {
         __syncthreads();                                     // what was there before has been read
-        if ((threadIdx.x & 63) == 0) wave_max[threadIdx.x >> 6] = amax;
+        if ((g.tid & 63) == 0) g.wave_max[g.tid >> 6] = amax;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < NW; ++w) amax = max(amax, wave_max[w]);
+        for (int w = 0; w < PGN_CW_WAVES; ++w) amax = max(amax, g.wave_max[w]);
     }
     return amax;
 }
 
-// Tokens x[0 .. count) of one head, for rows row0 .. row0 + count of the page half at dst.  NW waves.
-template <int DT, int D, int NW>
+// Tokens x[0 .. count) of one head, for rows row0 .. row0 + count of the page half at dst.
+template <int DT, int D>
 __device__ __forceinline__ void cw_keys(const unsigned short* x, int64_t x_st, bool vec, int row0, int count,
-                                        unsigned char* dst, float* scale, unsigned* wave_max) {
+                                        unsigned char* dst, float* scale, const CwTeam& g) {
     constexpr int PER_ROW = D / 8, KEEP = PER_ROW / 4;       // 16 rows a wave in registers
-    const int tid = threadIdx.x, n = count * PER_ROW;
+    const int tid = g.tid, n = count * PER_ROW;
     const auto load = [&](int e) { return cw_load<8>(x + (int64_t)(e / PER_ROW) * x_st + (e % PER_ROW) * 8, vec); };
     CwVec<8> v[KEEP];
 #pragma unroll
-    for (int i = 0; i < KEEP; ++i) v[i] = load(min(tid + i * NW * 64, n - 1));
+    for (int i = 0; i < KEEP; ++i) v[i] = load(min(tid + i * g.threads, n - 1));
     const float old = row0 > 0 ? *scale : 0.f;
     unsigned amax = 0;
 #pragma unroll
     for (int i = 0; i < KEEP; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) amax = cw_max2(amax, v[i].w[j]);
-    for (int e = tid + KEEP * NW * 64; e < n; e += NW * 64) {            // a longer run: read again below
+    for (int e = tid + KEEP * g.threads; e < n; e += g.threads) {            // a longer run: read again below
         const CwVec<8> u = load(e);
 #pragma unroll
         for (int j = 0; j < 4; ++j) amax = cw_max2(amax, u.w[j]);
     }
-    unsigned top = cw_block_max<NW>(amax, wave_max);
+    unsigned top = cw_team_max(amax, g);
     const bool odd = top >= CwInf<DT>::bits;                 // infinities or NaN: they do not count
     if (odd) {
         amax = 0;
-        for (int e = tid; e < n; e += NW * 64) {
+        for (int e = tid; e < n; e += g.threads) {
             const CwVec<8> u = load(e);
 #pragma unroll
             for (int j = 0; j < 4; ++j) amax = cw_max2(amax, cw_finite2<DT>(u.w[j]));
         }
-        top = cw_block_max<NW>(amax, wave_max);
+        top = cw_team_max(amax, g);
     }
     const float s = fmaxf(cw_scale(cw_lo<DT>(top)), old), inv = 1.0f / s;        // exact: s is a power of two
     if (old < s && row0 > 0) {                               // older tokens of the page, under the larger scale
         const float f = old * inv;
-        for (int e = tid; e < row0 * PER_ROW; e += NW * 64) {
+        for (int e = tid; e < row0 * PER_ROW; e += g.threads) {
             uint2 w = *reinterpret_cast<const uint2*>(dst + e * 8);
             w.x = pgn_fp8_rescale4(w.x, f);
             w.y = pgn_fp8_rescale4(w.y, f);
@@ -366,17 +375,17 @@ __device__ __forceinline__ void cw_keys(const unsigned short* x, int64_t x_st, b
     };
 #pragma unroll
     for (int i = 0; i < KEEP; ++i)
-        if (tid + i * NW * 64 < n) put(tid + i * NW * 64, v[i]);
-    for (int e = tid + KEEP * NW * 64; e < n; e += NW * 64) put(e, load(e));
-    if (NW > 1) __syncthreads();                             // every thread has read the old scale
+        if (tid + i * g.threads < n) put(tid + i * g.threads, v[i]);
+    for (int e = tid + KEEP * g.threads; e < n; e += g.threads) put(e, load(e));
+    if (g.all) __syncthreads();                             // every thread has read the old scale
     if (tid == 0) *scale = s;
 }
 
-template <int DT, int D, int NW>
+template <int DT, int D>
 __device__ __forceinline__ void cw_values(const unsigned short* x, int64_t x_st, bool vec, int row0, int count, int P,
-                                          unsigned char* dst, float* scale, unsigned* wave_max) {
+                                          unsigned char* dst, float* scale, const CwTeam& g) {
     constexpr int DV = D / 64, DW = (DV + 1) / 2;
-    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+    const int tid = g.tid, lane = tid & 63, wid = tid >> 6, waves = g.threads >> 6;
     const int slab0 = row0 >> 4, slabs = ((row0 + count + 15) >> 4) - slab0;     // slabs of 16 page rows that the run touches
     const auto row = [&](int slab, int j) { return (slab0 + slab) * 16 + j - row0; };    // token of the run, if in [0, count)
     const auto load = [&](int slab, CwVec<DV>* u) {
@@ -397,7 +406,7 @@ __device__ __forceinline__ void cw_values(const unsigned short* x, int64_t x_st,
     for (int j = 0; j < 16; ++j)
 #pragma unroll
         for (int d = 0; d < DW; ++d) amax = cw_max2(amax, v[j].w[d]);
-    for (int slab = wid + NW; slab < slabs; slab += NW) {    // a longer run: read again below
+    for (int slab = wid + waves; slab < slabs; slab += waves) {    // a longer run: read again below
         CwVec<DV> u[16];
         load(slab, u);
 #pragma unroll
@@ -405,11 +414,11 @@ __device__ __forceinline__ void cw_values(const unsigned short* x, int64_t x_st,
 #pragma unroll
             for (int d = 0; d < DW; ++d) amax = cw_max2(amax, u[j].w[d]);
     }
-    unsigned top = cw_block_max<NW>(amax, wave_max);
+    unsigned top = cw_team_max(amax, g);
     const bool odd = top >= CwInf<DT>::bits;
     if (odd) {
         amax = 0;
-        for (int slab = wid; slab < slabs; slab += NW) {
+        for (int slab = wid; slab < slabs; slab += waves) {
             CwVec<DV> u[16];
             load(slab, u);
 #pragma unroll
@@ -417,13 +426,13 @@ __device__ __forceinline__ void cw_values(const unsigned short* x, int64_t x_st,
 #pragma unroll
                 for (int d = 0; d < DW; ++d) amax = cw_max2(amax, cw_finite2<DT>(u[j].w[d]));
         }
-        top = cw_block_max<NW>(amax, wave_max);
+        top = cw_team_max(amax, g);
     }
     const float s = fmaxf(cw_scale(cw_lo<DT>(top)), old), inv = 1.0f / s;
     if (old < s && row0 > 0) {
         const float f = old * inv;
         const int words = (row0 + 3) >> 2;                   // the last word may hold tokens behind row0: bytes there
-        for (int e = threadIdx.x; e < D * words; e += NW * 64) {
+        for (int e = tid; e < D * words; e += g.threads) {
             const int d = e / words, w = e - d * words;
             unsigned char* p = dst + (int64_t)d * P + w * 4;
             const unsigned is = pgn_fp8_rescale4(*reinterpret_cast<const unsigned*>(p), f);
@@ -457,21 +466,21 @@ __device__ __forceinline__ void cw_values(const unsigned short* x, int64_t x_st,
         }
     };
     if (wid < slabs) put(wid, v);
-    for (int slab = wid + NW; slab < slabs; slab += NW) {
+    for (int slab = wid + waves; slab < slabs; slab += waves) {
         CwVec<DV> u[16];
         load(slab, u);
         put(slab, u);
     }
-    if (NW > 1) __syncthreads();
-    if (threadIdx.x == 0) *scale = s;
+    if (g.all) __syncthreads();
+    if (tid == 0) *scale = s;
 }
 
-template <int DT, int D, int NW>
-__global__ __launch_bounds__(NW * 64) void pgn_cache_write_kernel(
+template <int DT, int D>
+__global__ __launch_bounds__(PGN_CW_WAVES * 64) void pgn_cache_write_kernel(
     const unsigned short* __restrict__ k, const unsigned short* __restrict__ v, const int64_t* __restrict__ slots, int T,
     int H, int shift, int64_t N, int chunk, int64_t k_st, int64_t k_sh, int64_t v_st, int64_t v_sh, int k_vec, int v_vec,
     unsigned char* k_pages, unsigned char* v_pages, float* k_scale, float* v_scale) {
-    __shared__ unsigned wave_max[NW];
+    __shared__ unsigned wave_max[PGN_CW_WAVES];
     // Workgroups go round the 8 XCDs.  One XCD takes all heads of a chunk, one after another: a token's heads lie side by
     // side, and an XCD that read only every eighth of them would use few of its L2's channels.
     const int lane = threadIdx.x & 63, xcd = blockIdx.x & 7, j = blockIdx.x >> 3, h = j % H;
@@ -486,6 +495,7 @@ __global__ __launch_bounds__(NW * 64) void pgn_cache_write_kernel(
     if (lane == 0) my_before = t0 > 0 && t0 < T ? slots[t0 - 1] : -2;
     uint64_t runs = __ballot(lane < chunk && my_slot >= 0 && my_slot < limit &&
                              ((my_slot & (P - 1)) == 0 || my_before != my_slot - 1));
+    int turn = threadIdx.x >> 6;                             // short runs until the wave's next
     for (; runs != 0; runs &= runs - 1) {                    // every bound here is the same for the whole workgroup
         const int first = __builtin_ctzll(runs), t = t0 + first;
         const int64_t slot = __shfl(my_slot, first);
@@ -499,12 +509,18 @@ __global__ __launch_bounds__(NW * 64) void pgn_cache_write_kernel(
             count += on == 0 ? 64 : __builtin_ctzll(on);
         }
         const int64_t page = slot >> shift, half = (page * H + h) * (int64_t)P * D;
+        CwTeam g = {1, (int)threadIdx.x, PGN_CW_WAVES * 64, wave_max};
+        if (count <= 16) {
+            if (turn-- != 0) continue;
+            turn = PGN_CW_WAVES - 1;
+            g.all = 0, g.tid = lane, g.threads = 64;
+        }
         if (blockIdx.y == 0)
-            cw_keys<DT, D, NW>(k + (int64_t)t * k_st + h * k_sh, k_st, k_vec, row0, count, k_pages + half,
-                               k_scale + page * H + h, wave_max);
+            cw_keys<DT, D>(k + (int64_t)t * k_st + h * k_sh, k_st, k_vec, row0, count, k_pages + half,
+                           k_scale + page * H + h, g);
         else
-            cw_values<DT, D, NW>(v + (int64_t)t * v_st + h * v_sh, v_st, v_vec, row0, count, P, v_pages + half,
-                                 v_scale + page * H + h, wave_max);
+            cw_values<DT, D>(v + (int64_t)t * v_st + h * v_sh, v_st, v_vec, row0, count, P, v_pages + half,
+                             v_scale + page * H + h, g);
     }
 }
 
@@ -528,8 +544,8 @@ extern "C" int pgn_page_advance(int32_t* lens, const int32_t* keep, const int32_
 #define PGN_ADV_LAUNCH(NT)                                                                                             \
     hipLaunchKernelGGL((pgn_page_advance_kernel<NT>), dim3(1), dim3(NT), 0, s, lens, keep, add, table, table_stride,   \
                        free_pages, free_count, num_pages, R, W, shift, T, fused, slots, starts, status)
-    if (R <= 64 && T <= 512) PGN_ADV_LAUNCH(64);
-    else if (R <= 256 && T <= 2048) PGN_ADV_LAUNCH(256);
+    if (R <= 64 && T <= 128) PGN_ADV_LAUNCH(64);
+    else if (R <= 256 && T <= 1024) PGN_ADV_LAUNCH(256);
     else PGN_ADV_LAUNCH(PGN_ADV_THREADS);
 #undef PGN_ADV_LAUNCH
     PGN_LAUNCH_CHECK();
@@ -561,32 +577,27 @@ extern "C" int pgn_cache_write(const void* k, const void* v, int dtype, const in
     const int k_vec = pgn_aligned(k, 16) && k_st % 8 == 0 && k_sh % 8 == 0;
     const int v_vec = pgn_aligned(v, 2 * dv) && v_st % dv == 0 && v_sh % dv == 0;
     const int T = (int)num_tokens;
-    // A decoding step (every token a run of its own, latency counts): one token and one wave a workgroup.  Above that,
-    // four waves and 16 tokens, or 64 where that still makes 1024 workgroups: most tokens lie inside a run that began
-    // before, and a workgroup without a run costs its look at the slot map all the same.
-    const bool few = T <= 2048;
-    const int chunk = few ? 1 : ((int64_t)T * kv_heads >= 64 * 1024 ? 64 : 16);
+    // Few tokens, for decoding: each a run of its own, one for each wave (64 tokens of 8 heads by 128: 5.9 us, 15.0 with
+    // 16 tokens a workgroup, 51 with 64).  Many, for prompts: most lie inside a run that began before, and a workgroup
+    // without a run costs its look at the slot map all the same (2048 tokens: 18.6, 10.8 and 5.1 us; as many runs of one
+    // token: 42, 48 and 59 us).
+    const int chunk = T <= 512 ? 4 : T <= 1024 ? 16 : 64;
     const int64_t wgs = (int64_t)(((T + chunk - 1) / chunk + 7) / 8 * 8) * kv_heads;
     if (wgs > 0x7fffffff) return PGN_ERR_UNSUPPORTED;
     const dim3 grid((unsigned)wgs, 2);
     hipStream_t s = (hipStream_t)stream;
-#define PGN_CW_LAUNCH(DT, D, NW)                                                                                       \
-    hipLaunchKernelGGL((pgn_cache_write_kernel<DT, D, NW>), grid, dim3(NW * 64), 0, s, (const unsigned short*)k,       \
+#define PGN_CW_LAUNCH(DT, D)                                                                                           \
+    hipLaunchKernelGGL((pgn_cache_write_kernel<DT, D>), grid, dim3(PGN_CW_WAVES * 64), 0, s, (const unsigned short*)k, \
                        (const unsigned short*)v, slots, T, kv_heads, shift, (int64_t)num_pages, chunk, k_st, k_sh, v_st, \
                        v_sh, k_vec, v_vec, (unsigned char*)k_pages, (unsigned char*)v_pages, k_scale, v_scale)
-#define PGN_CW_DIMS(DT, NW)                                                                                            \
+#define PGN_CW_DIMS(DT)                                                                                                \
     do {                                                                                                               \
-        if (head_dim == 64) PGN_CW_LAUNCH(DT, 64, NW);                                                                 \
-        else if (head_dim == 128) PGN_CW_LAUNCH(DT, 128, NW);                                                          \
-        else PGN_CW_LAUNCH(DT, 256, NW);                                                                               \
+        if (head_dim == 64) PGN_CW_LAUNCH(DT, 64);                                                                     \
+        else if (head_dim == 128) PGN_CW_LAUNCH(DT, 128);                                                              \
+        else PGN_CW_LAUNCH(DT, 256);                                                                                   \
     } while (0)
-    if (dtype == PGN_BF16) {
-        if (few) PGN_CW_DIMS(PGN_BF16, 1);
-        else PGN_CW_DIMS(PGN_BF16, 4);
-    } else {
-        if (few) PGN_CW_DIMS(PGN_F16, 1);
-        else PGN_CW_DIMS(PGN_F16, 4);
-    }
+    if (dtype == PGN_BF16) PGN_CW_DIMS(PGN_BF16);
+    else PGN_CW_DIMS(PGN_F16);
 #undef PGN_CW_DIMS
 #undef PGN_CW_LAUNCH
     PGN_LAUNCH_CHECK();

@@ -836,7 +836,8 @@ def page_advance(lens: torch.Tensor, add: torch.Tensor, table: torch.Tensor, fre
 def cache_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                 k_scale: torch.Tensor, v_scale: torch.Tensor) -> None:
     """Stores k, v [T, kv_heads, head_dim] (bf16 / fp16, any strides with a contiguous last dim) at slots int64 [T] of one
-    layer's cache, in e4m3 with a power-of-two scale per page and head (pgn_cache_write).  Slots below 0 are left out."""
+    layer's cache, in e4m3 with a power-of-two scale per page and head (pgn_cache_write).  Slots below 0 are left out; the tokens of one page stand together, in ascending
+    slots, as page_advance lists them."""
     lib = _lib.load()
     dev = _on(k, v, slots, k_pages, v_pages, k_scale, v_scale)
     N, H, P, D = _check_pages(k_pages, v_pages, k_scale, v_scale)

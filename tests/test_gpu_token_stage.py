@@ -86,6 +86,32 @@ def test_page_advance_slot_map_sizes(T):
     assert got["slots"].cpu().tolist() == want[4] and got["starts"].tolist() == want[5] and dl.tolist() == want[0]
 
 
+@pytest.mark.parametrize("R,T", [(1, 128), (64, 128), (64, 129), (65, 128), (256, 1024), (256, 1025), (257, 1024),
+                                 (63, 4096), (300, 4097)])
+def test_page_advance_at_the_borders_of_its_launches(R, T):
+    """Requests and slots on both sides of where the bookkeeping takes more waves, with refusals and tokens left over."""
+    P, W, r = 16, 1 + T // 16, random.Random(R * T)
+    adds = [T // R] * R
+    adds[r.randrange(R)] += T % R
+    if R > 2:
+        adds[R // 2] = 0
+        adds[R - 1] += 9                                          # ends behind the slots: refused
+    pages = sum(-(-a // P) for a in adds) - (1 if R > 2 else 0)
+    lens, table, free, count = [r.randrange(P) for _ in range(R)], [[-1] * W for _ in range(R)], list(range(pages)), pages
+    keep = [r.choice([h, 0]) for h in lens]
+    for h, row in zip(lens, table):                               # their pages are outside the stack
+        if h:
+            row[0] = pages
+            pages += 1
+    free += [-1] * (pages - len(free))
+    dl, dt, df, dc = i32(lens), i32(table), i32(free), i32([count])
+    want = ref.page_advance_ref(lens, keep, adds, table, free, count, P, T)
+    got = ops.page_advance(dl, i32(adds), dt, df, dc, P, T, keep=i32(keep))
+    for name, a, b in (("lens", dl, want[0]), ("table", dt, want[1]), ("free", df, want[2]), ("count", dc, [want[3]]),
+                       ("slots", got["slots"], want[4]), ("starts", got["starts"], want[5]), ("status", got["status"], want[6])):
+        assert a.cpu().tolist() == b, name
+
+
 def test_page_advance_stays_inside_its_arrays_on_wrong_counts():
     """A stack height, lengths and additions that cannot be: nothing outside the arrays is touched."""
     R, W, N = 4, 2, 6
@@ -213,6 +239,31 @@ def test_cache_write_leaves_out_slots_that_are_none():
     g = torch.Generator().manual_seed(1)
     k, v = torch.randn(2, 10, H, D, generator=g).to(torch.float16).to(DEV)
     _check_write(k, v, slots, _cache(N, H, P, D))
+
+
+@pytest.mark.parametrize("T", [511, 512, 513, 1024, 1025])
+@pytest.mark.parametrize("P,D", [(16, 64), (128, 128), (64, 256)])
+def test_cache_write_short_and_long_runs_side_by_side(T, P, D):
+    """Runs of one wave and of the whole workgroup in any order, up to both sides of 16 and 64 tokens, slots that are none
+    between them."""
+    H, r = 2, random.Random(T * P + D)
+    runs, left, pages = [], T, list(range(T + 9))
+    r.shuffle(pages)
+    while left:
+        n = min(left, P, r.choice([1, 1, 2, 15, 16, 17, 18, 33, 63, 64, 65, 128]))
+        runs.append((pages.pop(), r.randint(0, P - n), n))
+        left -= n
+    slots = _slots(runs, P)
+    slots[::37] = -1
+    seen, last = set(), None                                      # a run that was cut in two keeps its first part
+    for i, s in enumerate(slots.tolist()):
+        if s >= 0 and s // P in seen and (last is None or s != last + 1):
+            slots[i] = s = -1
+        if s >= 0:
+            seen.add(s // P)
+        last = s if s >= 0 else None
+    k, v = torch.randn(2, T, H, D, generator=torch.Generator().manual_seed(T)).to(torch.bfloat16).to(DEV)
+    _check_write(k, v, slots, _cache(T + 9, H, P, D))
 
 
 @pytest.mark.parametrize("T", [2047, 2048, 2049, 5000])
