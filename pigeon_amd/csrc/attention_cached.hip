@@ -100,7 +100,9 @@ __device__ __forceinline__ unsigned key_bytes(int first, int word, int lo, int h
 }
 
 // Requests of up to this many rows (a row: a token and a query head of the KV head's group) go to the 16-row kernel, the
-// others to the 128-row kernel, in one call if need be.
+// others to the 128-row kernel, in one call if need be.  At head dim 128: 4 requests of 64 rows over 4096 keys of 4 KV
+// heads take 28 us in the one and 41 in the other, 32 requests over 2048 keys 62 and 61; with 128 rows 40 and 45, and 103
+// and 83.  With 8 KV heads 64 rows take 39 and 43, 96 and 88; 128 rows 64 and 47, 148 and 89.
 #define PGN_CA_FEW_ROWS 64
 
 // The rows of a workgroup: consecutive rows of one request, ROWS to a tile.  16-row tiles: a fixed number for every
@@ -153,15 +155,28 @@ __device__ __forceinline__ bool many_rows_tile(const CachedArgs& a, int tile, Ti
     return true;
 }
 
+// First key that the window leaves a token at `pos` (which may be negative: more queries than keys).
+__device__ __forceinline__ int window_lo(const CachedArgs& a, int pos) {
+    return a.window && pos >= a.window ? pos - a.window + 1 : 0;
+}
+
 // Keys that any row of the tile sees: [lo, hi).
 __device__ __forceinline__ void key_range(const CachedArgs& a, const TileRows& t, int& lo, int& hi) {
     const int pos0 = t.len - t.n + t.first / a.G, pos1 = t.len - t.n + (t.first + t.count - 1) / a.G;
     hi = a.causal ? max(0, min(t.len, pos1 + 1)) : t.len;
-    lo = a.window ? max(0, pos0 - a.window + 1) : 0;
+    lo = window_lo(a, pos0);
 }
 
 #define PGN_CA_THREADS 256
 
+// The kernel for single tokens and short requests: 16 rows of a request, four waves that take 64 keys in turn and join
+// their maxima, sums and outputs at the end.
+//
+// What bounds it is the cache's bytes: a row has two operations for every byte of key or value, so nothing is staged and
+// no lane waits for another one inside the loop; loads go to registers in the order in which the matrix instructions take
+// them, one round ahead (75 us below, 88 without).  16 requests of 1 to 4096 keys, 32 heads by 128, one row each: 354 MB
+// in 75 us, 4.7 TB/s; 4 requests of up to 131072 keys of 8 KV heads: 738 MB in 142 us, 5.2 TB/s.  A kernel that only
+// reads that much reaches 6.0.  One request of 257 keys: 8 us, a launch and a few trips to memory one behind the other.
 template <int DT, int D>
 __global__ __launch_bounds__(PGN_CA_THREADS) void pgn_cached_rows16_kernel(const CachedArgs a) {
     typedef typename Mat<DT>::v8 v8;
@@ -170,7 +185,7 @@ __global__ __launch_bounds__(PGN_CA_THREADS) void pgn_cached_rows16_kernel(const
     __shared__ float lds_m[4][16], lds_l[4][16];
     const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
     const int g = lane >> 4, col = lane & 15;
-    // heads fastest: 88 us against 101 with all heads of a stretch of keys on one XCD (16 requests of up to 4096, 32 heads)
+    // heads fastest: 88 us against 101 with all heads of a stretch of keys on one XCD (before the loads went ahead)
     const int h = blockIdx.x % a.Hkv, split = blockIdx.y;
     TileRows t;
     if (!few_rows_tile(a, blockIdx.x / a.Hkv, t)) return;
@@ -183,10 +198,10 @@ __global__ __launch_bounds__(PGN_CA_THREADS) void pgn_cached_rows16_kernel(const
     const int token = t.begin + row / a.G, head = h * a.G + row % a.G;
     const int pos = t.len - t.n + row / a.G;
     const int vis_hi = a.causal ? min(t.len, pos + 1) : t.len;
-    const int vis_lo = a.window ? max(0, pos - a.window + 1) : 0;
+    const int vis_lo = window_lo(a, pos);
     // keys that every row of the tile sees
     const int all_hi = a.causal ? min(t.len, t.len - t.n + t.first / a.G + 1) : t.len;
-    const int all_lo = a.window ? max(0, t.len - t.n + (t.first + t.count - 1) / a.G - a.window + 1) : 0;
+    const int all_lo = window_lo(a, t.len - t.n + (t.first + t.count - 1) / a.G);
 
     v8 qf[DB * 2];
     {
@@ -399,9 +414,12 @@ __global__ __launch_bounds__(PGN_CA_THREADS) void pgn_cached_rows16_kernel(const
 
 // The kernel for prompts: 128 rows of a request, 32 to a wave, 64 keys at a time.
 //
-// What bounds it is arithmetic: the two products take as many matrix cycles as the softmax takes vector cycles (32 keys
-// and 16 rows a lane: scaling, exp2, sum, maximum and rounding of 32 numbers against 32 matrix instructions at head
-// dim 128), so the bytes are widened ONCE per workgroup, on their way into LDS, not in every wave.  Tiles of 16-bit keys
+// What bounds it is arithmetic: the matrix units are busy for 35 % of the time and the vector units for 50 %, mostly with
+// the softmax (scaling, exp2, sum and rounding of 32 numbers a lane against 32 matrix instructions at head dim 128) and
+// the widening of bytes, which is done ONCE per workgroup, on the way into LDS, not in every wave.  4 prompts of 2048
+// tokens, 32 heads by 128: 520 us, 844 TFLOP/s (a library product of 16384^3 reaches 1346).  Taking 256 rows with 64 a wave
+// (1234 us, one wave a SIMD), 256 rows with eight waves (515, but 147 us for a batch of short requests that takes 76
+// here) or 32 keys at a time with three waves a SIMD (566) was not better.  Tiles of 16-bit keys
 // [64][D] and transposed values [D][64] are double buffered; while one is used, the next one's bytes are in flight
 // to registers.  Each wave fetches one 16-key chunk of a tile, which lies in one page.
 //
@@ -453,12 +471,12 @@ __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void pgn_cached_rows128_ke
     const int token = t.begin + row / a.G, head = h * a.G + row % a.G;
     const int pos = t.len - t.n + row / a.G;
     const int vis_hi = a.causal ? min(t.len, pos + 1) : t.len;
-    const int vis_lo = a.window ? max(0, pos - a.window + 1) : 0;
+    const int vis_lo = window_lo(a, pos);
     // keys that every row of the wave sees, and that any does
     const int pos0 = t.len - t.n + (t.first + min(wrow, t.count - 1)) / a.G;
     const int pos1 = t.len - t.n + (t.first + min(wrow + 31, t.count - 1)) / a.G;
     const int all_hi = a.causal ? min(t.len, pos0 + 1) : t.len, any_hi = a.causal ? min(t.len, pos1 + 1) : t.len;
-    const int all_lo = a.window ? max(0, pos1 - a.window + 1) : 0, any_lo = a.window ? max(0, pos0 - a.window + 1) : 0;
+    const int all_lo = window_lo(a, pos1), any_lo = window_lo(a, pos0);
 
     const bool flip = a.c < 0.f;                             // the maximum is taken before the scaling: c has to be positive
     const float c = fabsf(a.c);
@@ -865,7 +883,8 @@ extern "C" int pgn_cached_attention(const void* q, int dtype, const void* k_page
     if (dtype != PGN_BF16 && dtype != PGN_F16) return PGN_ERR_UNSUPPORTED;
     const int shift = cached_shift(page_size);
     if (shift < 0 || (head_dim != 64 && head_dim != 128 && head_dim != 256)) return PGN_ERR_UNSUPPORTED;
-    if (((int64_t)W << shift) > 0x7fffff00 - 65536 || Hkv > 65535 || R > (1 << 26) || (int64_t)num_tokens * (Hq / Hkv) > 0x7fffffff - 65536)
+    // positions are ints: the last split of the keys may begin at twice this and end at three times
+    if (((int64_t)W << shift) > PGN_CACHED_MAX_KEYS || Hkv > 65535 || R > (1 << 26) || (int64_t)num_tokens * (Hq / Hkv) > 0x7fffffff - 65536)
         return PGN_ERR_UNSUPPORTED;
     if (!pgn_aligned(q, 16) || q_st % 8 != 0 || q_sh % 8 != 0 || !pgn_aligned(k_pages, 16) || !pgn_aligned(v_pages, 16) ||
         !pgn_aligned(out, 2))

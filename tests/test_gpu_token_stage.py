@@ -376,6 +376,17 @@ def test_prompts_without_a_mask_and_with_more_queries_than_keys(causal, P):
     assert bool((got[43:] == 0).all()) and (not causal or bool((got[13:31] == 0).all()))
 
 
+@pytest.mark.parametrize("new", [[30, 12, 3], [90, 200, 70]])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 20, 7])
+def test_wide_windows_with_more_queries_than_keys(window, new):
+    """The first tokens stand at negative positions: no end of the window may wrap round."""
+    H, D, P = 2, 64, 32
+    lens = [9, 1, 68]
+    table, cache = _table(lens, P, 20), _cache(20, H, P, D)
+    starts = i32([0, new[0], new[0] + new[1], sum(new)])
+    _check_attention(_q(sum(new), 2 * H, D, torch.bfloat16), cache, table, i32(lens), starts, window=window)
+
+
 def test_rows_of_no_request_keep_what_out_held():
     new, lens = [3, 2], [40, 20]
     q = _q(12, 4, 64, torch.bfloat16)

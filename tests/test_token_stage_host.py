@@ -66,6 +66,16 @@ def test_entry_points_refuse_before_any_launch():
         assert sa(**k) == -2, k
 
 
+def test_attention_refuses_tables_beyond_the_positions_it_counts():
+    """W * P up to PGN_CACHED_MAX_KEYS passes the check of sizes (here it fails for its missing workspace, before any launch)."""
+    lib = _lib.load()
+    p, _keep = _p16()
+    call = lambda W, P: lib.pgn_cached_attention(p, 1, p, p, p, p, p, W, p, p, p, 2, 2, 4, 2, 64, 4, W, P, 256, 64, 256, 64, 0.1, 1, 0, None, 0,   # noqa: E731
+                                                 None)
+    for P in (16, 32, 64, 128):
+        assert call((1 << 28) // P, P) == -1 and call((1 << 28) // P + 1, P) == -2
+
+
 def test_workspace_is_zero_or_whole_and_grows_with_the_splits():
     f = _lib.load().pgn_cached_attention_workspace_bytes
     assert f(0, 1, 0, 1, 1, 64, 1, 16) == 0 and f(1, 1, 0, 3, 2, 64, 1, 16) == 0
