@@ -17,12 +17,15 @@ namespace {
 // One workgroup does the bookkeeping: it is a chain of three prefix sums over the requests (pages given back, tokens
 // added, pages wanted) whose results every later step needs, 4 bytes a request.  The pages themselves are then moved
 // flat, one thread a page: a thread finds its request by bisection in the prefix sums, which lie in LDS.
-// A chain of short steps is bound by their latency, and a barrier of 16 waves is the longest of them, so a small call
-// runs in one wave or four (back to back on the GPU: 64 requests and slots 3.5 us in one wave, 4.0 in four, 5.5 in 16;
-// 512 slots 8.9, 6.4, 7.9; 256 requests and slots 15.0, 5.8, 7.9; 2048 slots 32, 11, 9).
+// A chain of short steps is bound by their latency, and a barrier of 16 waves is the longest of them, so a call takes no
+// more waves than it has work for (us, back to back on the GPU, with 64, 256, 512 and 1024 threads):
+//   64 requests and slots  4.8  5.6  6.4  7.8        512 requests and slots       27  11   6.8  8.2
+//   64 and 512             8.9  6.4  6.4  7.9        512 and 4096                 63  21  12.5 10.9
+//   256 and 256            14   5.8  6.5  8.0        512 and 16384, two launches  31  14  10.7 12.0
+//   64 and 2048            23   11   9.0  8.9        16 and 8192, two launches   8.8 8.4   9.0 10.3
 #define PGN_ADV_THREADS 1024
 // Up to this many slots the bookkeeping workgroup fills the slot map itself (one launch); above it a second, wide launch
-// does (2048 slots: 8.9 us against 10.1; 8192: 14.4 against 10.5; 16384: 22 against 11).
+// does (512 requests, 4096 slots: 10.9 us against 10.5; 64 and 16384: 22 against 9.1).
 #define PGN_ADV_FUSED_SLOTS 4096
 
 __device__ __forceinline__ int64_t adv_pages(int64_t tokens, int shift) {
@@ -544,8 +547,11 @@ extern "C" int pgn_page_advance(int32_t* lens, const int32_t* keep, const int32_
 #define PGN_ADV_LAUNCH(NT)                                                                                             \
     hipLaunchKernelGGL((pgn_page_advance_kernel<NT>), dim3(1), dim3(NT), 0, s, lens, keep, add, table, table_stride,   \
                        free_pages, free_count, num_pages, R, W, shift, T, fused, slots, starts, status)
-    if (R <= 64 && T <= 128) PGN_ADV_LAUNCH(64);
-    else if (R <= 256 && T <= 1024) PGN_ADV_LAUNCH(256);
+    // requests, rounds over the slots, or (a few slots each) pages to hand out
+    const int per = fused ? T / 2 : T / 64, work = R > per ? R : per;
+    if (work <= 64) PGN_ADV_LAUNCH(64);
+    else if (work <= 256) PGN_ADV_LAUNCH(256);
+    else if (work <= 512) PGN_ADV_LAUNCH(512);
     else PGN_ADV_LAUNCH(PGN_ADV_THREADS);
 #undef PGN_ADV_LAUNCH
     PGN_LAUNCH_CHECK();

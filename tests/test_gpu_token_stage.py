@@ -87,7 +87,7 @@ def test_page_advance_slot_map_sizes(T):
 
 
 @pytest.mark.parametrize("R,T", [(1, 128), (64, 128), (64, 129), (65, 128), (256, 1024), (256, 1025), (257, 1024),
-                                 (63, 4096), (300, 4097)])
+                                 (63, 4096), (300, 4097), (512, 1024), (513, 1000), (512, 4200), (200, 20000), (3, 40000)])
 def test_page_advance_at_the_borders_of_its_launches(R, T):
     """Requests and slots on both sides of where the bookkeeping takes more waves, with refusals and tokens left over."""
     P, W, r = 16, 1 + T // 16, random.Random(R * T)
