@@ -174,7 +174,7 @@ __device__ __forceinline__ void key_range(const CachedArgs& a, const TileRows& t
 //
 // What bounds it is the cache's bytes: a row has two operations for every byte of key or value, so nothing is staged and
 // no lane waits for another one inside the loop; loads go to registers in the order in which the matrix instructions take
-// them, one round ahead (75 us below, 88 without).  16 requests of 1 to 4096 keys, 32 heads by 128, one row each: 354 MB
+// them, one round ahead (75 us below, 88 without).  16 requests of 900 to 4096 keys, 32 heads by 128, one row each: 354 MB
 // in 75 us, 4.7 TB/s; 4 requests of up to 131072 keys of 8 KV heads: 738 MB in 142 us, 5.2 TB/s.  A kernel that only
 // reads that much reaches 6.0.  One request of 257 keys: 8 us, a launch and a few trips to memory one behind the other.
 template <int DT, int D>
@@ -510,6 +510,11 @@ __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void pgn_cached_rows128_ke
     bool good = false;
     const auto page_at = [&](int key) { return table[min(key >> a.shift, a.W - 1)]; };
     int page = page_at(kb + 16 * chunk);                     // of the tile that is fetched next, looked up one tile ahead
+    int vpage[4];                                            // of all its chunks: fp16 needs the tile's largest scale
+    if constexpr (DT == PGN_F16) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) vpage[w] = page_at(kb + 16 * w);
+    }
 
     // bytes of the wave's chunk of the tile at `base`, and the scales of the tile
     auto fetch = [&](int base) {
@@ -527,7 +532,8 @@ __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void pgn_cached_rows128_ke
         if constexpr (DT == PGN_F16) {
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-                const int wkey = base + 16 * w, pw = page_at(wkey);
+                const int wkey = base + 16 * w, pw = vpage[w];
+                vpage[w] = page_at(wkey + 64);
                 const bool gw = wkey < hi && wkey + 16 > lo && (unsigned)pw < (unsigned)a.N;
                 vs[w] = gw ? a.v_scale[(int64_t)pw * a.Hkv + h] : 0.f;
             }

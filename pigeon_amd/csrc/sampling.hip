@@ -206,6 +206,10 @@ __device__ __forceinline__ u64 dpp0(u64 v) {
 }
 template <int CTRL, int ROWS>
 __device__ __forceinline__ unsigned dpp0(unsigned v) { return (unsigned)dpp0<CTRL, ROWS>((int)v); }
+__device__ __forceinline__ unsigned of_lane(unsigned v, int lane) { return (unsigned)__builtin_amdgcn_readlane((int)v, lane); }
+__device__ __forceinline__ u64 of_lane(u64 v, int lane) {
+    return ((u64)of_lane((unsigned)(v >> 32), lane) << 32) | of_lane((unsigned)v, lane);
+}
 template <typename T>
 __device__ __forceinline__ T wave_scan(T v) {
     v += dpp0<0x111, 0xf>(v);
@@ -221,20 +225,19 @@ __device__ __forceinline__ T wave_scan(T v) {
 template <typename T>
 __device__ __forceinline__ T block_scan(T v, void* scratch, T& total) {
     T* part = reinterpret_cast<T*>(scratch);
-    const int wid = threadIdx.x >> 6;
+    const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     v = wave_scan(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 63) part[wid] = v;
     __syncthreads();
-    T before = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < PGN_SAMPLE_WAVES; ++w) {
-        const T p = part[w];
-        before += w < wid ? p : 0;
-        all += p;
-    }
-    total = all;
-    return v + before;
+    static_assert(PGN_SAMPLE_WAVES == 16, "a row of 16 lanes scans the sums of the waves");
+    T p = part[threadIdx.x & 15];
+    p += dpp0<0x111, 0xf>(p);
+    p += dpp0<0x112, 0xf>(p);
+    p += dpp0<0x114, 0xf>(p);
+    p += dpp0<0x118, 0xf>(p);
+    total = of_lane(p, 15);
+    return v + (wid > 0 ? of_lane(p, wid - 1) : 0);
 }
 __device__ __forceinline__ u64 block_sum(u64 v, u64* part) {
     u64 total;
