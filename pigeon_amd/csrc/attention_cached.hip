@@ -506,44 +506,36 @@ __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void pgn_cached_rows128_ke
     const int P = 1 << a.shift;
     const int chunk = wid;                                   // of 16 keys of a tile, which the wave fetches
     uint4 kw[L], vw[L];
-    float ks = 0.f, vs[4];
-    bool good = false;
-    const auto page_at = [&](int key) { return table[min(key >> a.shift, a.W - 1)]; };
-    int page = page_at(kb + 16 * chunk);                     // of the tile that is fetched next, looked up one tile ahead
-    int vpage[4];                                            // of all its chunks: fp16 needs the tile's largest scale
-    if constexpr (DT == PGN_F16) {
-#pragma unroll
-        for (int w = 0; w < 4; ++w) vpage[w] = page_at(kb + 16 * w);
-    }
+    bool good = false;                                       // the wave's chunk lies on a page
+    // Pages and scales of the tile's chunks, chunk lane % 4 in each lane: scalar loads would be waited for together with the
+    // LDS reads of the tile that is worked on.  Pages are looked up one tile ahead.
+    const auto page_at = [&](int base) { return table[min((base + 16 * (lane & 3)) >> a.shift, a.W - 1)]; };
+    int page = page_at(kb);
+    float ks = 0.f, vs = 0.f;
+    bool on_page = false;
+    const auto of_chunk = [&](float v, int w) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), w)); };
 
     // bytes of the wave's chunk of the tile at `base`, and the scales of the tile
     auto fetch = [&](int base) {
-        const int key = base + 16 * chunk;
-        good = key < hi && key + 16 > lo && (unsigned)page < (unsigned)a.N;
-        const int64_t at = (int64_t)(good ? page : 0) * a.Hkv + h;
-        page = page_at(key + 64);
+        const int key = base + 16 * chunk, lkey = base + 16 * (lane & 3);
+        on_page = lkey < hi && lkey + 16 > lo && (unsigned)page < (unsigned)a.N;
+        const int own = __builtin_amdgcn_readlane(on_page ? page : -1, chunk);
+        good = own >= 0;
+        const int64_t at = (int64_t)(good ? own : 0) * a.Hkv + h, lat = (int64_t)(on_page ? page : 0) * a.Hkv + h;
         const unsigned char* kp = a.k_pages + (at * P + (key & (P - 1)) + (lane >> 2)) * D + (lane & 3) * 16;
 #pragma unroll
         for (int i = 0; i < L; ++i) kw[i] = *reinterpret_cast<const uint4*>(kp + i * 64);
-        ks = good ? a.k_scale[at] : 1.f;
         const unsigned char* vp = a.v_pages + (at * D + lane) * P + (key & (P - 1));
 #pragma unroll
         for (int i = 0; i < L; ++i) vw[i] = *reinterpret_cast<const uint4*>(vp + (int64_t)i * 64 * P);
-        if constexpr (DT == PGN_F16) {
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const int wkey = base + 16 * w, pw = vpage[w];
-                vpage[w] = page_at(wkey + 64);
-                const bool gw = wkey < hi && wkey + 16 > lo && (unsigned)pw < (unsigned)a.N;
-                vs[w] = gw ? a.v_scale[(int64_t)pw * a.Hkv + h] : 0.f;
-            }
-        } else {
-            vs[0] = good ? a.v_scale[at] : 0.f;
-        }
+        ks = a.k_scale[lat];
+        vs = a.v_scale[lat];
+        page = page_at(base + 64);
     };
     float store_ref = 0.f;
     auto store = [&](int base, int buf) {
         BigTile<DT, D>& tile = s.tile[buf];
+        const float kscale = of_chunk(ks, chunk), vlane = on_page ? vs : 0.f, vscale = of_chunk(vlane, chunk);
         const int key = lane >> 2, mrow = (key & 3) + 4 * (chunk & 1) + 8 * (key >> 2);
         unsigned short* kp = tile.k + (32 * (chunk >> 1) + mrow) * D;
 #pragma unroll
@@ -553,21 +545,18 @@ __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void pgn_cached_rows128_ke
             *reinterpret_cast<v8*>(kp + (((u + 1) ^ key_swizzle<D>(mrow)) * 8)) = widen8<DT>(kw[i].z, kw[i].w, 1.f);
         }
         if (lane == 0) {
-            s.ks[buf][chunk] = fmaxf(ks * c, 0x1p-126f); // 0 would turn a masked -inf into NaN
+            s.ks[buf][chunk] = fmaxf(good ? kscale * c : c, 0x1p-126f);      // 0 would turn a masked -inf into NaN
             s.live[buf][chunk] = good;
         }
-        float vmul = 1.f, raise = 0.f, pscale = 1.f, vscale;
+        float vmul = 1.f, raise = 0.f, pscale = 1.f;
         if constexpr (DT == PGN_F16) {                   // as in the 16-row kernel, raised by 2^7: probabilities reach 2^8
-            vscale = vs[0];
-#pragma unroll
-            for (int w = 1; w < 4; ++w) vscale = chunk == w ? vs[w] : vscale;
-            store_ref = fmaxf(store_ref, fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3])));
+            store_ref = fmaxf(store_ref, fmaxf(fmaxf(of_chunk(vlane, 0), of_chunk(vlane, 1)),
+                                               fmaxf(of_chunk(vlane, 2), of_chunk(vlane, 3))));
             const float ratio = good ? fmaxf(vscale / store_ref, 0x1p-60f) : 1.f;
             vmul = fmaxf(ratio, 0x1p-15f);
             pscale = 0x1p-7f * (vmul / ratio);
             raise = (float)(127 - (int)(__float_as_uint(pscale) >> 23));
         } else {
-            vscale = vs[0];
             vmul = good ? vscale : 1.f;
         }
         // bytes that no row sees may hold anything: they count as 0, as do those of a page whose scale is 0
