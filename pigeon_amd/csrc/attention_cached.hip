@@ -417,9 +417,9 @@ __global__ __launch_bounds__(PGN_CA_THREADS) void pgn_cached_rows16_kernel(const
 // What bounds it is arithmetic: the matrix units are busy for 35 % of the time and the vector units for 50 %, mostly with
 // the softmax (scaling, exp2, sum and rounding of 32 numbers a lane against 32 matrix instructions at head dim 128) and
 // the widening of bytes, which is done ONCE per workgroup, on the way into LDS, not in every wave.  4 prompts of 2048
-// tokens, 32 heads by 128: 520 us, 844 TFLOP/s (a library product of 16384^3 reaches 1346).  Taking 256 rows with 64 a wave
-// (1234 us, one wave a SIMD), 256 rows with eight waves (515, but 147 us for a batch of short requests that takes 76
-// here) or 32 keys at a time with three waves a SIMD (566) was not better.  Tiles of 16-bit keys
+// tokens, 32 heads by 128: 520 to 535 us, 820 to 844 TFLOP/s (a library product of 16384^3 reaches 1346); in fp16 562.
+// Taking 256 rows with 64 a wave (1234 us, one wave a SIMD), 256 rows with eight waves (515 against 517, but 147 against 80
+// for a batch of short requests) or 32 keys at a time with three waves a SIMD (566) was not better.  Tiles of 16-bit keys
 // [64][D] and transposed values [D][64] are double buffered; while one is used, the next one's bytes are in flight
 // to registers.  Each wave fetches one 16-key chunk of a tile, which lies in one page.
 //
