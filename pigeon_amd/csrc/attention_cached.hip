@@ -29,8 +29,10 @@ struct CachedArgs {
     const int* lens;
     const int* starts;
     unsigned short* out;
-    float* part_o;
+    float* part_o;                                           // of each split and row: unnormalised output, then maximum and sum
     float2* part_ml;
+    float* big_part_o;
+    float2* big_part_ml;
     int64_t table_stride, q_st, q_sh, o_st, o_sh;
     int T, R, Hq, Hkv, G, W, shift, N, causal, window;
     int split_keys, nsplit, tiles_per_request;               // of the 16-row kernel
@@ -137,6 +139,12 @@ __device__ __forceinline__ bool few_rows_tile(const CachedArgs& a, int tile, Til
     t.first = local * 16;
     t.count = min(16, rows - t.first);
     return t.count > 0;
+}
+
+// Rows of the 16-row kernel's tiles, and number `rr` of a tile's among them: the places of its partial results.
+__device__ __forceinline__ int64_t few_rows(const CachedArgs& a) { return (int64_t)a.R * a.tiles_per_request * 16 * a.Hkv; }
+__device__ __forceinline__ int64_t few_row(const CachedArgs& a, const TileRows& t, int rr, int h) {
+    return ((int64_t)t.r * a.tiles_per_request * 16 + t.first + rr) * a.Hkv + h;
 }
 
 template <int ROWS>
@@ -405,7 +413,7 @@ __global__ __launch_bounds__(PGN_CA_THREADS) void pgn_cached_rows16_kernel(const
         if (a.nsplit == 1) {
             a.out[tok * a.o_st + hd * a.o_sh + d] = Cvt<DT>::from_f32(den == 0.f ? 0.f : num / den);
         } else {
-            const int64_t at_row = ((int64_t)split * a.T + tok) * a.Hq + hd;
+            const int64_t at_row = split * few_rows(a) + few_row(a, t, rr, h);
             if (kb < kend) a.part_o[at_row * D + d] = num;
             if (d == 0) a.part_ml[at_row] = make_float2(big, den);
         }
@@ -757,10 +765,10 @@ __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void pgn_cached_rows128_ke
                     f32x4_t w;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) w[j] = o[d][4 * q + j] * unit;
-                    *reinterpret_cast<f32x4_t*>(a.part_o + at_row * D + d * 32 + q * 8 + hf * 4) = w;
+                    *reinterpret_cast<f32x4_t*>(a.big_part_o + at_row * D + d * 32 + q * 8 + hf * 4) = w;
                 }
         }
-        if (hf == 0) a.part_ml[at_row] = make_float2(m, l);
+        if (hf == 0) a.big_part_ml[at_row] = make_float2(m, l);
     }
 }
 
@@ -778,8 +786,10 @@ __global__ __launch_bounds__(PGN_CA_THREADS) void pgn_cached_join_kernel(const C
     if (rr >= t.count) return;
     const int nsplit = ROWS > 16 ? a.big_nsplit : a.nsplit;
     const int rw = t.first + rr, tok = t.begin + rw / a.G, hd = h * a.G + rw % a.G;
-    const int64_t row = (int64_t)tok * a.Hq + hd, step = (int64_t)a.T * a.Hq;
-    const float2 ml = lane < nsplit ? a.part_ml[lane * step + row] : make_float2(-INFINITY, 0.f);
+    const int64_t row = ROWS > 16 ? (int64_t)tok * a.Hq + hd : few_row(a, t, rr, h);
+    const int64_t step = ROWS > 16 ? (int64_t)a.T * a.Hq : few_rows(a);
+    const float2* part_ml = ROWS > 16 ? a.big_part_ml : a.part_ml;
+    const float2 ml = lane < nsplit ? part_ml[lane * step + row] : make_float2(-INFINITY, 0.f);
     float big = ml.x;
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) big = fmaxf(big, __shfl_xor(big, off));
@@ -791,7 +801,7 @@ __global__ __launch_bounds__(PGN_CA_THREADS) void pgn_cached_join_kernel(const C
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) den += __shfl_xor(den, off);
     float num[E] = {};
-    const float* part = a.part_o + row * D + lane;
+    const float* part = (ROWS > 16 ? a.big_part_o : a.part_o) + row * D + lane;
     while (seen) {
         float w[8], v[8][E];
 #pragma unroll
@@ -843,9 +853,12 @@ static CachedPlan cached_plan(int T, int R, bool packed, int G, int Hkv, int64_t
     return p;
 }
 
-static size_t cached_workspace(const CachedPlan& p, int64_t rows, int D) {
-    const int n = p.nsplit > p.big_nsplit ? p.nsplit : p.big_nsplit;
-    return n == 1 ? 0 : (size_t)n * rows * (D * 4 + 8);
+// Rows times splits of each kernel.  Splits end where there are 512 workgroups, so both are small (some 10^5) whatever
+// the number of tokens is.
+static int64_t few_parts(const CachedPlan& p, int Hkv) { return p.nsplit > 1 ? (int64_t)p.nsplit * p.tiles * 16 * Hkv : 0; }
+static int64_t big_parts(const CachedPlan& p, int64_t rows) { return p.big_nsplit > 1 ? p.big_nsplit * rows : 0; }
+static size_t cached_workspace(const CachedPlan& p, int64_t rows, int Hkv, int D) {
+    return (size_t)(few_parts(p, Hkv) + big_parts(p, rows)) * (D * 4 + 8);
 }
 
 }  // namespace
@@ -860,7 +873,7 @@ extern "C" size_t pgn_cached_attention_workspace_bytes(int num_tokens, int R, in
                                                        int W, int page_size) {
     if (!cached_sizes(num_tokens, R, Hq, Hkv, head_dim, W, page_size)) return 0;
     const CachedPlan p = cached_plan(num_tokens, R, packed != 0, Hq / Hkv, Hkv, (int64_t)W * page_size);
-    return cached_workspace(p, (int64_t)num_tokens * Hq, head_dim);
+    return cached_workspace(p, (int64_t)num_tokens * Hq, Hkv, head_dim);
 }
 
 extern "C" int pgn_cached_attention(const void* q, int dtype, const void* k_pages, const void* v_pages,
@@ -886,7 +899,7 @@ extern "C" int pgn_cached_attention(const void* q, int dtype, const void* k_page
         return PGN_ERR_INVALID;
     const CachedPlan p = cached_plan(num_tokens, R, starts != nullptr, Hq / Hkv, Hkv, (int64_t)W << shift);
     if ((int64_t)p.tiles * Hkv > 0x7fffffff || (int64_t)p.big_tiles * Hkv > 0x7fffffff) return PGN_ERR_UNSUPPORTED;
-    const size_t need = cached_workspace(p, (int64_t)num_tokens * Hq, head_dim);
+    const size_t need = cached_workspace(p, (int64_t)num_tokens * Hq, Hkv, head_dim);
     if (need > 0 && (workspace == nullptr || workspace_bytes < need || !pgn_aligned(workspace, 16))) return PGN_ERR_INVALID;
     CachedArgs a;
     a.q = (const unsigned short*)q;
@@ -898,8 +911,11 @@ extern "C" int pgn_cached_attention(const void* q, int dtype, const void* k_page
     a.lens = lens;
     a.starts = starts;
     a.out = (unsigned short*)out;
+    const int64_t few = few_parts(p, Hkv), big = big_parts(p, (int64_t)num_tokens * Hq);
     a.part_o = (float*)workspace;
-    a.part_ml = need ? (float2*)((char*)workspace + need / (head_dim * 4 + 8) * (head_dim * 4)) : nullptr;
+    a.big_part_o = a.part_o + few * head_dim;
+    a.part_ml = (float2*)(a.part_o + (few + big) * head_dim);
+    a.big_part_ml = a.part_ml + few;
     a.table_stride = table_stride;
     a.q_st = q_st;
     a.q_sh = q_sh;

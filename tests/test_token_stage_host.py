@@ -85,6 +85,17 @@ def test_workspace_is_zero_or_whole_and_grows_with_the_splits():
         assert n % (8 * (128 * 4 + 8)) == 0
 
 
+def test_workspace_does_not_grow_with_the_tokens_of_long_prompts():
+    """Few requests split their keys over many workgroups, but only as long as there are few rows: at most 512 workgroups
+    of 64 rows, and twice 512 of 128, each with head_dim + 2 numbers a row."""
+    f = _lib.load().pgn_cached_attention_workspace_bytes
+    for R in (1, 3, 40):
+        for T in (64, 1000, 8192, 100000, 1000000):
+            for Hq, Hkv in ((32, 32), (32, 8), (16, 1)):
+                for W in (16, 8192, 200000):
+                    assert f(T, R, 1, Hq, Hkv, 128, W, 16) <= (2 * 512 * 64 + 2 * 512 * 128) * (128 * 4 + 8), (R, T, Hq, Hkv, W)
+
+
 def test_cpu_tensors_raise():
     z = torch.zeros(2, dtype=torch.int32)
     with pytest.raises(RuntimeError, match="no CPU fallback"):
