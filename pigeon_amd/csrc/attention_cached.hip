@@ -35,8 +35,8 @@ struct CachedArgs {
     float2* big_part_ml;
     int64_t table_stride, q_st, q_sh, o_st, o_sh;
     int T, R, Hq, Hkv, G, W, shift, N, causal, window;
-    int split_keys, nsplit, tiles_per_request;               // of the 16-row kernel
-    int big_split_keys, big_nsplit, big_tiles;               // of the 128-row kernel
+    int nsplit, tiles_per_request;                           // of the 16-row kernel
+    int big_nsplit, big_tiles;                               // of the 128-row kernel
     int out_vec;                                             // rows of `out` begin on 8 bytes
     float c;                                                 // scale * log2(e)
 };
@@ -175,6 +175,20 @@ __device__ __forceinline__ void key_range(const CachedArgs& a, const TileRows& t
     lo = window_lo(a, pos0);
 }
 
+// Where a split of a tile's keys begins.  The launch says how many splits there are, from the width of the table; their
+// size goes by the keys that the tile sees, so that a wide table or a window leaves none of them idle (sizes by the table:
+// 103 us instead of 20 for one request of 16000 keys in a table for 10^6, 36 instead of 17 for 4 with a window of 4096; 142
+// instead of 146 for 4 requests that fill theirs by 46 to 100 %).  They have 512 keys at least: two rounds of the 16-row
+// kernel's four waves (256: 20.8 us against 16.2 for one request of 16000 keys, 10.4 against 8.2 for one of 257; 1024: 17.4),
+// 8 tiles of the 128-row kernel.
+#define PGN_CA_LEAST_KEYS 512
+__device__ __forceinline__ int split_begin(int lo, int hi, int nsplit, int split) {
+    const int from = lo & ~63;
+    if (nsplit == 1) return split == 0 ? from : 0x7fffffff;
+    const int units = ((hi - from + nsplit - 1) / nsplit + PGN_CA_LEAST_KEYS - 1) / PGN_CA_LEAST_KEYS;
+    return from + split * max(1, units) * PGN_CA_LEAST_KEYS;
+}
+
 #define PGN_CA_THREADS 256
 
 // The kernel for single tokens and short requests: 16 rows of a request, four waves that take 64 keys in turn and join
@@ -199,8 +213,8 @@ __global__ __launch_bounds__(PGN_CA_THREADS) void pgn_cached_rows16_kernel(const
     if (!few_rows_tile(a, blockIdx.x / a.Hkv, t)) return;
     int lo, hi;
     key_range(a, t, lo, hi);
-    const int kb = (lo & ~63) + split * a.split_keys;
-    const int kend = min(hi, kb + a.split_keys);
+    const int kb = split_begin(lo, hi, a.nsplit, split);
+    const int kend = min(hi, split_begin(lo, hi, a.nsplit, split + 1));
 
     const int row = t.first + min(col, t.count - 1);         // rows past the last repeat it and are not written
     const int token = t.begin + row / a.G, head = h * a.G + row % a.G;
@@ -470,8 +484,8 @@ __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void pgn_cached_rows128_ke
     if (!many_rows_tile<128>(a, a.big_tiles - 1 - (int)(blockIdx.x / a.Hkv), t)) return;     // a request's longest rows first
     int lo, hi;
     key_range(a, t, lo, hi);
-    const int kb = (lo & ~63) + split * a.big_split_keys;
-    const int kend = min(hi, kb + a.big_split_keys);
+    const int kb = split_begin(lo, hi, a.big_nsplit, split);
+    const int kend = min(hi, split_begin(lo, hi, a.big_nsplit, split + 1));
 
     const int wrow = wid * 32;                               // first row of the wave in the tile
     const int mine = min(wrow + col, t.count - 1);           // rows past the last repeat it and are not written
@@ -824,20 +838,17 @@ __global__ __launch_bounds__(PGN_CA_THREADS) void pgn_cached_join_kernel(const C
 }
 
 struct CachedPlan {
-    int tiles, tiles_per_request, nsplit, split_keys;        // 16-row kernel
-    int big_tiles, big_nsplit, big_split_keys;               // 128-row kernel; no tiles: not launched
+    int tiles, tiles_per_request, nsplit;                    // 16-row kernel
+    int big_tiles, big_nsplit;                               // 128-row kernel; no tiles: not launched
 };
 
-// Splits of the keys so that `want` workgroups are there, each with `least` keys or more (256: one round of the 16-row
-// kernel's four waves).  Wanted are 512, which is what the CUs hold at a time: 143 us for 4 requests of up to 131072 keys
-// and 8 KV heads, against 146 with twice and 155 with four times as many and their larger join.
-static void split_keys(int64_t wgs, int64_t want, int64_t max_keys, int least, int* nsplit, int* keys) {
-    const int64_t most = (max_keys + least - 1) / least;
-    int64_t n = (want + wgs - 1) / wgs;
+// Splits of the keys so that 512 workgroups are there, which is what the CUs hold at a time: 143 us for 4 requests of up to
+// 131072 keys and 8 KV heads, against 146 with twice and 155 with four times as many and their larger join.
+static int splits(int64_t wgs, int64_t max_keys) {
+    const int64_t most = (max_keys + PGN_CA_LEAST_KEYS - 1) / PGN_CA_LEAST_KEYS;
+    int64_t n = (512 + wgs - 1) / wgs;
     n = n < most ? n : most;
-    n = n < 1 ? 1 : (n > 64 ? 64 : n);
-    *keys = (int)(((max_keys + 64 + n - 1) / n + least - 1) / least * least);
-    *nsplit = (int)((max_keys + 64 + *keys - 1) / *keys);
+    return (int)(n < 1 ? 1 : (n > 64 ? 64 : n));
 }
 
 static CachedPlan cached_plan(int T, int R, bool packed, int G, int Hkv, int64_t max_keys) {
@@ -845,11 +856,9 @@ static CachedPlan cached_plan(int T, int R, bool packed, int G, int Hkv, int64_t
     const int few = packed ? (PGN_CA_FEW_ROWS < (int64_t)T * G ? PGN_CA_FEW_ROWS : T * G) : G;
     p.tiles_per_request = (few + 15) / 16;
     p.tiles = R * p.tiles_per_request;
-    split_keys((int64_t)(packed ? R : p.tiles) * Hkv, 512, max_keys, 256, &p.nsplit, &p.split_keys);
+    p.nsplit = splits((int64_t)(packed ? R : p.tiles) * Hkv, max_keys);
     p.big_tiles = packed && (int64_t)T * G > PGN_CA_FEW_ROWS ? (int)((int64_t)T * G / 128 + R) : 0;
-    p.big_nsplit = 1;
-    p.big_split_keys = 0;
-    if (p.big_tiles) split_keys((int64_t)p.big_tiles * Hkv, 512, max_keys, 512, &p.big_nsplit, &p.big_split_keys);
+    p.big_nsplit = p.big_tiles ? splits((int64_t)p.big_tiles * Hkv, max_keys) : 1;
     return p;
 }
 
@@ -891,7 +900,7 @@ extern "C" int pgn_cached_attention(const void* q, int dtype, const void* k_page
     if (dtype != PGN_BF16 && dtype != PGN_F16) return PGN_ERR_UNSUPPORTED;
     const int shift = cached_shift(page_size);
     if (shift < 0 || (head_dim != 64 && head_dim != 128 && head_dim != 256)) return PGN_ERR_UNSUPPORTED;
-    // positions are ints: the last split of the keys may begin at twice this and end at three times
+    // positions are ints, and 64 splits of 512 keys more than there are may be counted
     if (((int64_t)W << shift) > PGN_CACHED_MAX_KEYS || Hkv > 65535 || R > (1 << 26) || (int64_t)num_tokens * (Hq / Hkv) > 0x7fffffff - 65536)
         return PGN_ERR_UNSUPPORTED;
     if (!pgn_aligned(q, 16) || q_st % 8 != 0 || q_sh % 8 != 0 || !pgn_aligned(k_pages, 16) || !pgn_aligned(v_pages, 16) ||
@@ -931,10 +940,8 @@ extern "C" int pgn_cached_attention(const void* q, int dtype, const void* k_page
     a.N = num_pages;
     a.causal = causal != 0;
     a.window = window;
-    a.split_keys = p.split_keys;
     a.nsplit = p.nsplit;
     a.tiles_per_request = p.tiles_per_request;
-    a.big_split_keys = p.big_split_keys;
     a.big_nsplit = p.big_nsplit;
     a.big_tiles = p.big_tiles;
     a.out_vec = pgn_aligned(out, 8) && o_st % 4 == 0 && o_sh % 4 == 0;
