@@ -175,18 +175,25 @@ __device__ __forceinline__ void key_range(const CachedArgs& a, const TileRows& t
     lo = window_lo(a, pos0);
 }
 
-// Where a split of a tile's keys begins.  The launch says how many splits there are, from the width of the table; their
-// size goes by the keys that the tile sees, so that a wide table or a window leaves none of them idle (sizes by the table:
-// 103 us instead of 20 for one request of 16000 keys in a table for 10^6, 36 instead of 17 for 4 with a window of 4096; 142
-// instead of 146 for 4 requests that fill theirs by 46 to 100 %).  They have 512 keys at least: two rounds of the 16-row
-// kernel's four waves (256: 20.8 us against 16.2 for one request of 16000 keys, 10.4 against 8.2 for one of 257; 1024: 17.4),
-// 8 tiles of the 128-row kernel.
+// Keys of a split.  The launch says how many splits there are, from the width of the table; their size goes by the longest
+// request, or by the window, so that a wide table leaves none of them idle (sizes by the table: 103 us instead of 17 for
+// one request of 16000 keys in a table for 10^6, 36 instead of 17 for 4 with a window of 4096 in one for 131072) and all
+// workgroups have as much to do (sizes by each request's own length: 146 us instead of 143 for 4 requests of 60000 to
+// 131072).  They have 512 keys at least: two rounds of the 16-row kernel's four waves (256: 20.8 us against 16.2 for one
+// request of 16000 keys, 10.4 against 8.2 for one of 257; 1024: 17.4), 8 tiles of the 128-row kernel.
 #define PGN_CA_LEAST_KEYS 512
-__device__ __forceinline__ int split_begin(int lo, int hi, int nsplit, int split) {
-    const int from = lo & ~63;
-    if (nsplit == 1) return split == 0 ? from : 0x7fffffff;
-    const int units = ((hi - from + nsplit - 1) / nsplit + PGN_CA_LEAST_KEYS - 1) / PGN_CA_LEAST_KEYS;
-    return from + split * max(1, units) * PGN_CA_LEAST_KEYS;
+__device__ __forceinline__ int split_keys(const CachedArgs& a, int lo, int hi, int nsplit) {
+    int span = hi - (lo & ~63);
+    if (nsplit > 1 && a.R > 1) {                             // then R is under 512
+        int longest = 0;
+        for (int r = threadIdx.x & 63; r < a.R; r += 64) longest = max(longest, a.lens[r]);
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) longest = max(longest, __shfl_xor(longest, off));
+        longest = min(longest, a.W << a.shift);
+        span = max(span, a.window ? min(longest, a.window) : longest);
+    }
+    const int units = ((max(span, 1) + nsplit - 1) / nsplit + PGN_CA_LEAST_KEYS - 1) / PGN_CA_LEAST_KEYS;
+    return __builtin_amdgcn_readfirstlane(units * PGN_CA_LEAST_KEYS);
 }
 
 #define PGN_CA_THREADS 256
@@ -213,8 +220,7 @@ __global__ __launch_bounds__(PGN_CA_THREADS) void pgn_cached_rows16_kernel(const
     if (!few_rows_tile(a, blockIdx.x / a.Hkv, t)) return;
     int lo, hi;
     key_range(a, t, lo, hi);
-    const int kb = split_begin(lo, hi, a.nsplit, split);
-    const int kend = min(hi, split_begin(lo, hi, a.nsplit, split + 1));
+    const int keys = split_keys(a, lo, hi, a.nsplit), kb = (lo & ~63) + split * keys, kend = min(hi, kb + keys);
 
     const int row = t.first + min(col, t.count - 1);         // rows past the last repeat it and are not written
     const int token = t.begin + row / a.G, head = h * a.G + row % a.G;
@@ -484,8 +490,7 @@ __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void pgn_cached_rows128_ke
     if (!many_rows_tile<128>(a, a.big_tiles - 1 - (int)(blockIdx.x / a.Hkv), t)) return;     // a request's longest rows first
     int lo, hi;
     key_range(a, t, lo, hi);
-    const int kb = split_begin(lo, hi, a.big_nsplit, split);
-    const int kend = min(hi, split_begin(lo, hi, a.big_nsplit, split + 1));
+    const int keys = split_keys(a, lo, hi, a.big_nsplit), kb = (lo & ~63) + split * keys, kend = min(hi, kb + keys);
 
     const int wrow = wid * 32;                               // first row of the wave in the tile
     const int mine = min(wrow + col, t.count - 1);           // rows past the last repeat it and are not written

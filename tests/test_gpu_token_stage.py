@@ -515,6 +515,22 @@ def test_long_requests_are_split_and_joined(lens):
     _check_attention(_q(len(lens), 2, 64, torch.bfloat16), _cache(200, 1, P, 64), _table(lens, P, 200), i32(lens))
 
 
+@pytest.mark.parametrize("lens,new", [([700, 5100, 0, 2049], None), ([1], None), ([3300, 90, 1400], [3, 90, 70]), ([2600, 1500], [200, 1])])
+@pytest.mark.parametrize("window,causal", [(0, True), (600, True), (0, False)])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_splits_in_tables_much_wider_than_the_requests(lens, new, window, causal, dt):
+    """Room for 10^5 tokens a request, entries behind a request's pages that name no page or another's: splits
+    are sized by the longest request or the window."""
+    P, N, W = 32, 400, 3200
+    table = _table(lens, P, N)
+    wide = torch.full((len(lens), W), -5, dtype=torch.int32, device=DEV)
+    wide[:, 200:] = 3
+    wide[:, :table.shape[1]] = table
+    starts = None if new is None else i32(np.cumsum([0] + new).tolist())
+    T = len(lens) if new is None else sum(new)
+    _check_attention(_q(T, 4, 64, dt), _cache(N, 2, P, 64), wide, i32(lens), starts=starts, window=window, causal=causal)
+
+
 def test_offsets_beyond_32_bits():
     """A cache of 4.3 GB each for keys and values, the request on its last pages."""
     H, P, D = 8, 128, 256
