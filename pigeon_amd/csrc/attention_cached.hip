@@ -31,11 +31,12 @@ struct CachedArgs {
     unsigned short* out;
     float* part_o;                                           // of each split and row: unnormalised output, then maximum and sum
     float2* part_ml;
+    int4* plans;                                             // of each request with few rows: tiles, splits, first slot
     float* big_part_o;
     float2* big_part_ml;
     int64_t table_stride, q_st, q_sh, o_st, o_sh;
     int T, R, Hq, Hkv, G, W, shift, N, causal, window;
-    int nsplit, tiles_per_request;                           // of the 16-row kernel
+    int few_split, few_slots, tiles_per_request;             // of the 16-row kernel
     int big_nsplit, big_tiles;                               // of the 128-row kernel
     int out_vec;                                             // rows of `out` begin on 8 bytes
     float c;                                                 // scale * log2(e)
@@ -141,12 +142,6 @@ __device__ __forceinline__ bool few_rows_tile(const CachedArgs& a, int tile, Til
     return t.count > 0;
 }
 
-// Rows of the 16-row kernel's tiles, and number `rr` of a tile's among them: the places of its partial results.
-__device__ __forceinline__ int64_t few_rows(const CachedArgs& a) { return (int64_t)a.R * a.tiles_per_request * 16 * a.Hkv; }
-__device__ __forceinline__ int64_t few_row(const CachedArgs& a, const TileRows& t, int rr, int h) {
-    return ((int64_t)t.r * a.tiles_per_request * 16 + t.first + rr) * a.Hkv + h;
-}
-
 template <int ROWS>
 __device__ __forceinline__ bool many_rows_tile(const CachedArgs& a, int tile, TileRows& t) {
     int lo = 0, hi = a.R;
@@ -175,13 +170,12 @@ __device__ __forceinline__ void key_range(const CachedArgs& a, const TileRows& t
     lo = window_lo(a, pos0);
 }
 
-// Keys of a split.  The launch says how many splits there are, from the width of the table; their size goes by the longest
-// request, or by the window, so that a wide table leaves none of them idle (sizes by the table: 103 us instead of 17 for
-// one request of 16000 keys in a table for 10^6, 36 instead of 17 for 4 with a window of 4096 in one for 131072) and all
-// workgroups have as much to do (sizes by each request's own length: 146 us instead of 143 for 4 requests of 60000 to
-// 131072).  They have 512 keys at least: two rounds of the 16-row kernel's four waves (256: 20.8 us against 16.2 for one
-// request of 16000 keys, 10.4 against 8.2 for one of 257; 1024: 17.4), 8 tiles of the 128-row kernel.
+// Splits have this many keys at least: two rounds of the 16-row kernel's four waves (256: 20.8 us against 16.2 for one
+// request of 16000 keys of 8 heads, 10.4 against 8.2 for one of 257; 1024: 17.4), 8 tiles of the 128-row kernel.
 #define PGN_CA_LEAST_KEYS 512
+
+// Keys of a split of the 128-row kernel.  The launch says how many splits there are, from the width of the table; their size
+// goes by the longest request, or by the window, so that a wide table leaves none of them idle.
 __device__ __forceinline__ int split_keys(const CachedArgs& a, int lo, int hi, int nsplit) {
     int span = hi - (lo & ~63);
     if (nsplit > 1 && a.R > 1) {                             // then R is under 512
@@ -196,6 +190,100 @@ __device__ __forceinline__ int split_keys(const CachedArgs& a, int lo, int hi, i
     return __builtin_amdgcn_readfirstlane(units * PGN_CA_LEAST_KEYS);
 }
 
+// Splits of the 16-row kernel.  All have one size, under which the call's tiles make as many workgroups as the CUs hold at a
+// time, so that a long request among short ones gets its share of them (64 requests of 8 heads, one of 16367 keys, the
+// others of 500: 30 us instead of 111 without).  Nothing of this is known to the host: the launch has that many slots, or
+// one for each tile and that many, which is what any lengths can need, and every workgroup finds the tile and split of its
+// slot by a prefix sum over the requests.  That costs 1 us of a short call (4 requests of 2000 keys: 19 us).
+struct FewPlan {
+    int r, tiles, splits, first_slot, keys;                  // of a request: 16-row tiles, splits of each, its first slot
+};
+
+// tiles of request r and the keys that one of them can see, counted from a multiple of 64
+__device__ __forceinline__ void few_request(const CachedArgs& a, int r, int& tiles, int& span) {
+    TileRows t;
+    tiles = span = 0;
+    if (r >= a.R || !request_rows(a, r, t)) return;
+    const int rows = t.n * a.G;
+    if (a.starts != nullptr && rows > PGN_CA_FEW_ROWS) return;
+    tiles = (rows + 15) / 16;
+    span = t.len;
+    if (a.window && t.len > a.window)
+        span = t.n == 1 ? t.len - ((t.len - a.window) & ~63) : min(t.len, a.window + t.n) + 63;
+}
+
+// Workgroups of the 16-row kernel that the CUs hold at a time, by its registers.
+__host__ __device__ constexpr int few_resident(int D) { return D == 64 ? 768 : D == 128 ? 512 : 256; }
+
+// The plan of the request that owns a slot, by all lanes of a wave; false: there is none.  512 requests at most.
+template <int D>
+__device__ __forceinline__ bool few_plan(const CachedArgs& a, int slot, FewPlan& p) {
+    const int lane = threadIdx.x & 63, share = max(1, few_resident(D) / a.Hkv);
+    int tiles, span, longest = 0, all = 0;
+    int64_t total = 0;
+    for (int r0 = 0; r0 < a.R; r0 += 64) {
+        few_request(a, r0 + lane, tiles, span);
+        longest = max(longest, tiles > 0 ? span : 0);
+        total += (int64_t)tiles * span;
+        all += tiles;
+    }
+    for (int off = a.R > 32 ? 32 : a.R > 8 ? 16 : 4; off > 0 && a.R > 1; off >>= 1) {
+        longest = max(longest, __shfl_xor(longest, off));
+        total += __shfl_xor(total, off);
+        all += __shfl_xor(all, off);
+    }
+    all = __builtin_amdgcn_readfirstlane(all);
+    longest = __builtin_amdgcn_readfirstlane(longest);
+    total = ((int64_t)__builtin_amdgcn_readfirstlane((int)(total >> 32)) << 32) | (unsigned)__builtin_amdgcn_readfirstlane((int)total);
+    // where there are enough tiles, only one of twice the average is split; 64 splits at most (see the join)
+    const float mean = fminf((float)total * ((all >= share ? 2.f : 1.f) / (float)share), (float)longest);
+    p.keys = max(PGN_CA_LEAST_KEYS, (max((int)ceilf(mean), (longest + 63) / 64) + 255) / 256 * 256);
+    if (a.R <= 64 && all < share && p.keys < longest) {
+        // Rounded up for each request, the splits may be more than the share, and the last ones would run alone: the least size
+        // under which they are not, of 64, one in each lane (138 us instead of 168 for 4 requests of 60000 to 131072 keys).
+        const int step = max(256, p.keys / 64 / 256 * 256), size = p.keys + lane * step;
+        const float per = 1.f / (float)size;
+        int count = 0;
+        for (int r = 0; r < a.R; ++r) {
+            const int keys = __builtin_amdgcn_readlane(span, r), whole = (int)((float)keys * per), rest = keys - whole * size;
+            count += __builtin_amdgcn_readlane(tiles, r) * max(1, whole + (rest > 0) + (rest > size));     // exact: 64 at most
+        }
+        const uint64_t fit = __ballot(count <= share), one = __ballot(count * a.Hkv <= 256);
+        if (fit == 0) {
+            p.keys = longest;
+        } else {
+            // or a larger one with which no CU has two workgroups, if that leaves the busiest less to do
+            const int at = __builtin_ctzll(fit), last = one != 0 ? __builtin_ctzll(one) : at, first_keys = p.keys;
+            const int rounds = (__builtin_amdgcn_readlane(count, at) * a.Hkv + 255) / 256;
+            p.keys = first_keys + at * step;
+            if ((first_keys + last * step) * 1.15f < (float)p.keys * rounds) p.keys = first_keys + last * step;
+        }
+    }
+    p.first_slot = 0;
+    for (int r0 = 0; r0 < a.R; r0 += 64) {
+        if (a.R > 64) few_request(a, r0 + lane, tiles, span);
+        const int splits = max(1, (span + p.keys - 1) / p.keys), mine = tiles * splits;
+        int upto = mine;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            if (a.R <= off) break;
+            const int o = __shfl_up(upto, off);
+            if (lane >= off) upto += o;
+        }
+        const uint64_t has = __ballot(slot < p.first_slot + upto && mine > 0);
+        if (has != 0) {
+            const int at = __builtin_ctzll(has);
+            p.r = r0 + at;
+            p.tiles = __builtin_amdgcn_readlane(tiles, at);
+            p.splits = __builtin_amdgcn_readlane(splits, at);
+            p.first_slot += __builtin_amdgcn_readlane(upto - mine, at);
+            return true;
+        }
+        p.first_slot += __builtin_amdgcn_readlane(upto, 63);
+    }
+    return false;
+}
+
 #define PGN_CA_THREADS 256
 
 // The kernel for single tokens and short requests: 16 rows of a request, four waves that take 64 keys in turn and join
@@ -204,7 +292,7 @@ __device__ __forceinline__ int split_keys(const CachedArgs& a, int lo, int hi, i
 // What bounds it is the cache's bytes: a row has two operations for every byte of key or value, so nothing is staged and
 // no lane waits for another one inside the loop; loads go to registers in the order in which the matrix instructions take
 // them, one round ahead (75 us below, 88 without).  16 requests of 900 to 4096 keys, 32 heads by 128, one row each: 354 MB
-// in 75 us, 4.7 TB/s; 4 requests of up to 131072 keys of 8 KV heads: 738 MB in 142 us, 5.2 TB/s.  A kernel that only
+// in 75 us, 4.7 TB/s; 4 requests of 60000 to 131072 keys of 8 KV heads: 738 MB in 138 us, 5.4 TB/s.  A kernel that only
 // reads that much reaches 6.0.  One request of 257 keys: 8 us, a launch and a few trips to memory one behind the other.
 template <int DT, int D>
 __global__ __launch_bounds__(PGN_CA_THREADS) void pgn_cached_rows16_kernel(const CachedArgs a) {
@@ -215,12 +303,22 @@ __global__ __launch_bounds__(PGN_CA_THREADS) void pgn_cached_rows16_kernel(const
     const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
     const int g = lane >> 4, col = lane & 15;
     // heads fastest: 88 us against 101 with all heads of a stretch of keys on one XCD (before the loads went ahead)
-    const int h = blockIdx.x % a.Hkv, split = blockIdx.y;
+    const int h = blockIdx.x % a.Hkv, slot = blockIdx.x / a.Hkv;
     TileRows t;
-    if (!few_rows_tile(a, blockIdx.x / a.Hkv, t)) return;
+    FewPlan plan;
+    int split = 0;
+    if (a.few_split) {
+        if (!few_plan<D>(a, slot, plan) || !request_rows(a, plan.r, t)) return;
+        split = (slot - plan.first_slot) / plan.tiles;
+        if (slot == plan.first_slot && h == 0 && tid == 0) a.plans[plan.r] = int4{plan.tiles, plan.splits, plan.first_slot, 0};
+        t.first = (slot - plan.first_slot - split * plan.tiles) * 16;
+        t.count = min(16, t.n * a.G - t.first);
+    } else if (!few_rows_tile(a, slot, t)) {
+        return;
+    }
     int lo, hi;
     key_range(a, t, lo, hi);
-    const int keys = split_keys(a, lo, hi, a.nsplit), kb = (lo & ~63) + split * keys, kend = min(hi, kb + keys);
+    const int kb = (lo & ~63) + (a.few_split ? split * plan.keys : 0), kend = a.few_split ? min(hi, kb + plan.keys) : hi;
 
     const int row = t.first + min(col, t.count - 1);         // rows past the last repeat it and are not written
     const int token = t.begin + row / a.G, head = h * a.G + row % a.G;
@@ -430,10 +528,10 @@ __global__ __launch_bounds__(PGN_CA_THREADS) void pgn_cached_rows16_kernel(const
             num = fmaf(lds[(w * 16 + rr) * D + d], f, num);
         }
         const int rw = t.first + rr, tok = t.begin + rw / a.G, hd = h * a.G + rw % a.G;
-        if (a.nsplit == 1) {
+        if (!a.few_split || plan.splits == 1) {
             a.out[tok * a.o_st + hd * a.o_sh + d] = Cvt<DT>::from_f32(den == 0.f ? 0.f : num / den);
         } else {
-            const int64_t at_row = split * few_rows(a) + few_row(a, t, rr, h);
+            const int64_t at_row = ((int64_t)slot * 16 + rr) * a.Hkv + h;
             if (kb < kend) a.part_o[at_row * D + d] = num;
             if (d == 0) a.part_ml[at_row] = make_float2(big, den);
         }
@@ -803,10 +901,20 @@ __global__ __launch_bounds__(PGN_CA_THREADS) void pgn_cached_join_kernel(const C
     if (!(ROWS > 16 ? many_rows_tile<ROWS>(a, tile, t) : few_rows_tile(a, tile, t))) return;
     const int rr = blockIdx.y * 4 + wid;
     if (rr >= t.count) return;
-    const int nsplit = ROWS > 16 ? a.big_nsplit : a.nsplit;
+    int nsplit = a.big_nsplit;
+    int64_t row = 0, step = 0;
+    if constexpr (ROWS == 16) {
+        const int4 plan = a.plans[t.r];
+        nsplit = plan.y;
+        if (nsplit == 1) return;                             // is in `out` already
+        row = ((int64_t)(plan.z + t.first / 16) * 16 + rr) * a.Hkv + h;
+        step = (int64_t)plan.x * 16 * a.Hkv;
+    }
     const int rw = t.first + rr, tok = t.begin + rw / a.G, hd = h * a.G + rw % a.G;
-    const int64_t row = ROWS > 16 ? (int64_t)tok * a.Hq + hd : few_row(a, t, rr, h);
-    const int64_t step = ROWS > 16 ? (int64_t)a.T * a.Hq : few_rows(a);
+    if constexpr (ROWS > 16) {
+        row = (int64_t)tok * a.Hq + hd;
+        step = (int64_t)a.T * a.Hq;
+    }
     const float2* part_ml = ROWS > 16 ? a.big_part_ml : a.part_ml;
     const float2 ml = lane < nsplit ? part_ml[lane * step + row] : make_float2(-INFINITY, 0.f);
     float big = ml.x;
@@ -843,12 +951,11 @@ __global__ __launch_bounds__(PGN_CA_THREADS) void pgn_cached_join_kernel(const C
 }
 
 struct CachedPlan {
-    int tiles, tiles_per_request, nsplit;                    // 16-row kernel
+    int tiles, tiles_per_request, few_split, few_slots;      // 16-row kernel
     int big_tiles, big_nsplit;                               // 128-row kernel; no tiles: not launched
 };
 
-// Splits of the keys so that 512 workgroups are there, which is what the CUs hold at a time: 143 us for 4 requests of up to
-// 131072 keys and 8 KV heads, against 146 with twice and 155 with four times as many and their larger join.
+// Splits of the 128-row kernel's keys so that 512 workgroups are there, which is what the CUs hold at a time.
 static int splits(int64_t wgs, int64_t max_keys) {
     const int64_t most = (max_keys + PGN_CA_LEAST_KEYS - 1) / PGN_CA_LEAST_KEYS;
     int64_t n = (512 + wgs - 1) / wgs;
@@ -856,12 +963,17 @@ static int splits(int64_t wgs, int64_t max_keys) {
     return (int)(n < 1 ? 1 : (n > 64 ? 64 : n));
 }
 
-static CachedPlan cached_plan(int T, int R, bool packed, int G, int Hkv, int64_t max_keys) {
+static CachedPlan cached_plan(int T, int R, bool packed, int G, int Hkv, int D, int64_t max_keys) {
     CachedPlan p;
     const int few = packed ? (PGN_CA_FEW_ROWS < (int64_t)T * G ? PGN_CA_FEW_ROWS : T * G) : G;
     p.tiles_per_request = (few + 15) / 16;
     p.tiles = R * p.tiles_per_request;
-    p.nsplit = splits((int64_t)(packed ? R : p.tiles) * Hkv, max_keys);
+    // Enough tiles for all CUs are split only in wide tables, where one long request would go on alone (16 requests of 32
+    // heads, one of 65519 keys, the others of 500: 102 us instead of 476; all of 4000: 79 instead of 77), and not where
+    // there are so many that this matters little, or that adding them up would.
+    const int64_t tiles = (int64_t)p.tiles * Hkv, share = Hkv < few_resident(D) ? few_resident(D) / Hkv : 1;
+    p.few_split = max_keys > PGN_CA_LEAST_KEYS && (tiles < few_resident(D) || max_keys > 8192) && R <= 512 && tiles <= 4096;
+    p.few_slots = !p.few_split ? p.tiles : (int)(R <= 64 && p.tiles < share ? share : p.tiles + share);
     p.big_tiles = packed && (int64_t)T * G > PGN_CA_FEW_ROWS ? (int)((int64_t)T * G / 128 + R) : 0;
     p.big_nsplit = p.big_tiles ? splits((int64_t)p.big_tiles * Hkv, max_keys) : 1;
     return p;
@@ -869,10 +981,12 @@ static CachedPlan cached_plan(int T, int R, bool packed, int G, int Hkv, int64_t
 
 // Rows times splits of each kernel.  Splits end where there are 512 workgroups, so both are small (some 10^5) whatever
 // the number of tokens is.
-static int64_t few_parts(const CachedPlan& p, int Hkv) { return p.nsplit > 1 ? (int64_t)p.nsplit * p.tiles * 16 * Hkv : 0; }
+static int64_t few_parts(const CachedPlan& p, int Hkv) { return p.few_split ? (int64_t)p.few_slots * 16 * Hkv : 0; }
+// behind them, room for the plans: 512 times 16 bytes in the outputs of two slots of one head of 64
+static int64_t plan_parts(const CachedPlan& p, int Hkv) { return p.few_split ? 2 * 16 * (int64_t)Hkv : 0; }
 static int64_t big_parts(const CachedPlan& p, int64_t rows) { return p.big_nsplit > 1 ? p.big_nsplit * rows : 0; }
 static size_t cached_workspace(const CachedPlan& p, int64_t rows, int Hkv, int D) {
-    return (size_t)(few_parts(p, Hkv) + big_parts(p, rows)) * (D * 4 + 8);
+    return (size_t)(few_parts(p, Hkv) + plan_parts(p, Hkv) + big_parts(p, rows)) * (D * 4 + 8);
 }
 
 }  // namespace
@@ -886,7 +1000,7 @@ static bool cached_sizes(int T, int R, int Hq, int Hkv, int D, int W, int page_s
 extern "C" size_t pgn_cached_attention_workspace_bytes(int num_tokens, int R, int packed, int Hq, int Hkv, int head_dim,
                                                        int W, int page_size) {
     if (!cached_sizes(num_tokens, R, Hq, Hkv, head_dim, W, page_size)) return 0;
-    const CachedPlan p = cached_plan(num_tokens, R, packed != 0, Hq / Hkv, Hkv, (int64_t)W * page_size);
+    const CachedPlan p = cached_plan(num_tokens, R, packed != 0, Hq / Hkv, Hkv, head_dim, (int64_t)W * page_size);
     return cached_workspace(p, (int64_t)num_tokens * Hq, Hkv, head_dim);
 }
 
@@ -911,7 +1025,7 @@ extern "C" int pgn_cached_attention(const void* q, int dtype, const void* k_page
     if (!pgn_aligned(q, 16) || q_st % 8 != 0 || q_sh % 8 != 0 || !pgn_aligned(k_pages, 16) || !pgn_aligned(v_pages, 16) ||
         !pgn_aligned(out, 2))
         return PGN_ERR_INVALID;
-    const CachedPlan p = cached_plan(num_tokens, R, starts != nullptr, Hq / Hkv, Hkv, (int64_t)W << shift);
+    const CachedPlan p = cached_plan(num_tokens, R, starts != nullptr, Hq / Hkv, Hkv, head_dim, (int64_t)W << shift);
     if ((int64_t)p.tiles * Hkv > 0x7fffffff || (int64_t)p.big_tiles * Hkv > 0x7fffffff) return PGN_ERR_UNSUPPORTED;
     const size_t need = cached_workspace(p, (int64_t)num_tokens * Hq, Hkv, head_dim);
     if (need > 0 && (workspace == nullptr || workspace_bytes < need || !pgn_aligned(workspace, 16))) return PGN_ERR_INVALID;
@@ -927,8 +1041,9 @@ extern "C" int pgn_cached_attention(const void* q, int dtype, const void* k_page
     a.out = (unsigned short*)out;
     const int64_t few = few_parts(p, Hkv), big = big_parts(p, (int64_t)num_tokens * Hq);
     a.part_o = (float*)workspace;
-    a.big_part_o = a.part_o + few * head_dim;
-    a.part_ml = (float2*)(a.part_o + (few + big) * head_dim);
+    a.plans = (int4*)(a.part_o + few * head_dim);
+    a.big_part_o = a.part_o + (few + plan_parts(p, Hkv)) * head_dim;
+    a.part_ml = (float2*)(a.big_part_o + big * head_dim);
     a.big_part_ml = a.part_ml + few;
     a.table_stride = table_stride;
     a.q_st = q_st;
@@ -945,7 +1060,8 @@ extern "C" int pgn_cached_attention(const void* q, int dtype, const void* k_page
     a.N = num_pages;
     a.causal = causal != 0;
     a.window = window;
-    a.nsplit = p.nsplit;
+    a.few_split = p.few_split;
+    a.few_slots = p.few_slots;
     a.tiles_per_request = p.tiles_per_request;
     a.big_nsplit = p.big_nsplit;
     a.big_tiles = p.big_tiles;
@@ -967,8 +1083,8 @@ extern "C" int pgn_cached_attention(const void* q, int dtype, const void* k_page
         if (p.big_tiles)                                                                                               \
             PGN_CA_KERNEL((pgn_cached_rows128_kernel<DT, D>), sizeof(BigLds<DT, D>),                                   \
                           dim3(Hkv * p.big_tiles, p.big_nsplit));                                                      \
-        PGN_CA_KERNEL((pgn_cached_rows16_kernel<DT, D>), (size_t)4 * 16 * D * 4, dim3(Hkv * p.tiles, p.nsplit));       \
-        if (p.nsplit > 1)                                                                                              \
+        PGN_CA_KERNEL((pgn_cached_rows16_kernel<DT, D>), (size_t)4 * 16 * D * 4, dim3(Hkv * p.few_slots));       \
+        if (p.few_split)                                                                                              \
             PGN_CA_KERNEL((pgn_cached_join_kernel<DT, D, 16>), 0, dim3(Hkv * p.tiles, 4));                             \
         if (p.big_nsplit > 1)                                                                                          \
             PGN_CA_KERNEL((pgn_cached_join_kernel<DT, D, 128>), 0, dim3(Hkv * p.big_tiles, 32));                       \

@@ -531,6 +531,27 @@ def test_splits_in_tables_much_wider_than_the_requests(lens, new, window, causal
     _check_attention(_q(T, 4, 64, dt), _cache(N, 2, P, 64), wide, i32(lens), starts=starts, window=window, causal=causal)
 
 
+@pytest.mark.parametrize("D,Hkv,G", [(64, 1, 4), (128, 2, 20), (256, 1, 1), (64, 16, 1)])
+@pytest.mark.parametrize("R,long", [(3, 9000), (70, 5000), (300, 4000), (513, 3000)])
+@pytest.mark.parametrize("packed", [False, True])
+def test_one_long_request_among_many(R, long, packed, D, Hkv, G):
+    """The long request's keys go to many workgroups, whose slots are found by the lengths of all; more requests than are
+    added up; tables on both sides of the width from which a full launch is split."""
+    P, r = 64, random.Random(R + D)
+    lens = [r.choice([0, 1, r.randint(2, 90)]) for _ in range(R)]
+    lens[R // 3], lens[-1] = long, long // 2 + 17
+    new = [r.choice([0, 1, 1, 1, 3]) for _ in range(R)] if packed else [1] * R
+    new[R // 3], new[-1] = 1, 2 if packed else 1
+    lens = [max(h, n) for h, n in zip(lens, new)]
+    N = sum(-(-h // P) for h in lens) + 2
+    table = _table(lens, P, N)
+    if R % 2:
+        table = torch.cat([table, torch.full((R, 200), -1, dtype=torch.int32, device=DEV)], 1)
+    starts = i32(np.cumsum([0] + new).tolist()) if packed else None
+    _check_attention(_q(sum(new), Hkv * G, D, torch.bfloat16), _cache(N, Hkv, P, D), table, i32(lens), starts=starts,
+                     window=700 if R == 70 else 0)
+
+
 def test_offsets_beyond_32_bits():
     """A cache of 4.3 GB each for keys and values, the request on its last pages."""
     H, P, D = 8, 128, 256
