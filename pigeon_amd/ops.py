@@ -823,6 +823,8 @@ def page_advance(lens: torch.Tensor, add: torch.Tensor, table: torch.Tensor, fre
     slots = torch.empty(num_slots, dtype=torch.int64, device=dev)
     both = torch.empty(2 * R + 1, dtype=torch.int32, device=dev)
     starts, status = both[:R + 1], both[R + 1:]
+    if R == 0:
+        return {"slots": slots.fill_(-1), "starts": starts.zero_(), "status": status}
 
     def run():
         _call(dev, "pgn_page_advance", lib.pgn_page_advance, lens.data_ptr(), _ptr(keep), add.data_ptr(), table.data_ptr(),
@@ -887,8 +889,9 @@ def cached_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
         out = torch.empty(T, Hq, D, dtype=q.dtype, device=dev)
     elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
         raise ValueError("cached_attention: out must match q, with a contiguous last dim")
-    if T == 0:
+    if T == 0 or R == 0:
         return out
+    window = min(int(window), 2 ** 31 - 1)                     # as wide as any: the C argument would wrap
     if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
         q = q.contiguous()                                     # rows are read 16 bytes at a time
         if q.data_ptr() % 16:
@@ -902,7 +905,7 @@ def cached_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
         _call(dev, "pgn_cached_attention", lib.pgn_cached_attention, q.data_ptr(), _dt(q), k_pages.data_ptr(),
               v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), table.data_ptr(),
               table.stride(0) if R > 1 else W, lens.data_ptr(), _ptr(starts), out.data_ptr(), T, R, Hq, H, D, N, W, P,
-              q.stride(0), q.stride(1), out.stride(0), out.stride(1), scale, int(causal), int(window), _ptr(ws), nbytes)
+              q.stride(0), q.stride(1), out.stride(0), out.stride(1), scale, int(causal), window, _ptr(ws), nbytes)
 
     _launch("cached_attention", 4.0 * T * Hq * D, run)
     return out
@@ -918,6 +921,8 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, 
     if logits.dim() != 2:
         raise ValueError("sample_tokens expects logits [B, V]")
     B, V = logits.shape
+    if not isinstance(top_k, torch.Tensor):
+        top_k = min(max(int(top_k), 0), V)                     # the C argument would wrap
     tensors = [x if isinstance(x, torch.Tensor) else None for x in (temperature, top_k, top_p, min_p)]
     dev = _on(logits, uniform, *tensors)
     for t, dt, name in zip([uniform] + tensors, (torch.float32, torch.float32, torch.int32, torch.float32, torch.float32),
@@ -927,6 +932,8 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, 
     ids = torch.empty(B, dtype=torch.int64, device=dev)
     if B == 0:
         return ids
+    if V > 2 ** 31 - 1:
+        raise NotImplementedError("sample_tokens: too many ids")
     if logits.stride(1) != 1 and V > 1:
         logits = logits.contiguous()
     tt, kt, pt, mt = tensors

@@ -840,6 +840,25 @@ def test_two_runs_give_the_same_bits():
 
 
 # ------------------------------------------------------------------------------------------------ refusals
+def test_no_requests_and_arguments_wider_than_an_int():
+    none = i32([])
+    got = ops.page_advance(none, none, torch.empty(0, 3, dtype=torch.int32, device=DEV), i32([4, 5]), i32([2]), 16, 5)
+    assert got["slots"].tolist() == [-1] * 5 and got["starts"].tolist() == [0] and got["status"].numel() == 0
+    cache = _cache(4, 1, 16, 64)
+    out = torch.full((2, 1, 64), 7.0, dtype=torch.bfloat16, device=DEV)
+    ops.cached_attention(_q(2, 1, 64, torch.bfloat16), *cache, torch.empty(0, 3, dtype=torch.int32, device=DEV), none, starts=i32([0]), out=out)
+    assert bool((out == 7.0).all())
+    table, q = _table([30, 40], 16, 8), _q(2, 1, 64, torch.bfloat16)
+    cache = _cache(8, 1, 16, 64)
+    want = ops.cached_attention(q, *cache, table, i32([30, 40]))
+    for window in (2 ** 31, 2 ** 32 + 5, 2 ** 40):
+        assert torch.equal(ops.cached_attention(q, *cache, table, i32([30, 40]), window=window), want)
+    x, u = _logits(3, 500, torch.float32)
+    want = ops.sample_tokens(x, u)
+    for k in (2 ** 31, 2 ** 32 + 1, -1, -(2 ** 32) + 1):
+        assert torch.equal(ops.sample_tokens(x, u, top_k=k), want)
+
+
 def test_wrong_arguments_are_refused():
     cache, table, lens = _cache(4, 2, 16, 64), _table([20, 20], 16, 4, extra=0), i32([20, 20])
     kp, vp, ks, vs = cache
