@@ -830,6 +830,29 @@ def test_a_captured_step_replays_like_the_eager_one():
     assert torch.equal(graphed.cache[1].view(torch.uint8), eager.cache[1].view(torch.uint8))
 
 
+def test_a_captured_call_follows_the_lengths():
+    """Splits are planned from the lengths on the device: a graph captured at short ones replays at long ones."""
+    P, N, W, H = 32, 500, 300, 2
+    cache = _cache(N, H, P, 64)
+    table = i32([[random.Random(r * 1000 + j).randrange(N) for j in range(W)] for r in range(3)])
+    lens, q = i32([5, 1, 9]), _q(3, 4, 64, torch.float16)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        side.wait_stream(torch.cuda.default_stream())
+        ops.cached_attention(q, *cache, table, lens)
+    side.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = ops.cached_attention(q, *cache, table, lens)
+    for now in ([5, 1, 9], [7000, 3, 513], [0, 0, 0], [512, 9600, 9599], [1, 2, 3], [2000, 1500, 1000], [0, 0, 9000]):
+        lens.copy_(i32(now))
+        g.replay()
+        want = ops.cached_attention(q, *cache, table, lens)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), now
+        _check_attention(q, cache, table, lens)
+
+
 def test_two_runs_give_the_same_bits():
     lens = [3000, 700]
     cache, table = _cache(60, 2, 64, 128), _table([3000, 700], 64, 60)
