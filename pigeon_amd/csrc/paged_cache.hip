@@ -71,6 +71,17 @@ __device__ __forceinline__ int adv_find(const int* at, int n, int x) {
     return lo;
 }
 
+// the same of four numbers, in their places; n a power of two
+__device__ __forceinline__ void adv_find4(const int* at, int n, int* x) {
+    int lo[4] = {0, 0, 0, 0};
+    for (int step = n >> 1; step > 0; step >>= 1) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) lo[u] += at[lo[u] + step] <= x[u] ? step : 0;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) x[u] = lo[u];
+}
+
 struct AdvRequest {
     int64_t held, keep, add;
     int have, kept;
@@ -119,11 +130,20 @@ __global__ __launch_bounds__(NT) void pgn_page_advance_kernel(
             at[tid] = upto - mine;
             col[tid] = q.kept;
             __syncthreads();
-            for (int e = tid; e < total; e += NT) {
-                const int i = adv_find(at, NT, e);
-                const int64_t place = count + released - 1 - (done + e);
-                if (place < N)                               // more pages back than the pool holds: a caller's mistake
-                    free_pages[place] = table[(r0 + i) * table_stride + col[i] + (e - at[i])];
+            for (int e0 = tid; e0 < total; e0 += 4 * NT) {
+                int i[4], page[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) i[u] = min(e0 + u * NT, total - 1);
+                adv_find4(at, NT, i);
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    page[u] = table[(r0 + i[u]) * table_stride + col[i[u]] + (min(e0 + u * NT, total - 1) - at[i[u]])];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int64_t place = count + released - 1 - (done + e0 + u * NT);
+                    if (e0 + u * NT < total && place < N)    // more pages back than the pool holds: a caller's mistake
+                        free_pages[place] = page[u];
+                }
             }
             done += total;
             __syncthreads();
@@ -169,9 +189,20 @@ __global__ __launch_bounds__(NT) void pgn_page_advance_kernel(
             at[tid] = first;
             col[tid] = q.kept;
             __syncthreads();
-            for (int e = tid; e < total; e += NT) {
-                const int i = adv_find(at, NT, e);
-                table[(r0 + i) * table_stride + col[i] + (e - at[i])] = free_pages[top - 1 - popped - e];
+            for (int e0 = tid; e0 < total; e0 += 4 * NT) {
+                int i[4], page[4];                           // four at a time, so that their steps do not wait for one another
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int e = min(e0 + u * NT, total - 1);
+                    page[u] = free_pages[top - 1 - popped - e];
+                    i[u] = e;
+                }
+                adv_find4(at, NT, i);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int e = e0 + u * NT;
+                    if (e < total) table[(r0 + i[u]) * table_stride + col[i[u]] + (e - at[i[u]])] = page[u];
+                }
             }
             popped += total;
             __syncthreads();
