@@ -436,7 +436,8 @@ int pgn_cache_write(const void* k, const void* v, int dtype, const int64_t* slot
  * causal: a token sees the keys up to its own position, with window > 0 the last `window` of those; causal 0: every key
  * of its request (window must be 0).  A row that sees no key is zero.  Rows of no request (behind starts[R]) are left as
  * they were.  Table entries that name no page hide their keys.  Keys that a row does not see do not reach it, whatever
- * their bytes hold.  Sums are fp32 and divided at the end: values beyond 2^127 / (256 keys) may overflow.  W * P is at
+ * their bytes hold.  The same call gives the same bits; where a request's keys are split goes by the lengths of all, so
+ * its last bits may differ in other company.  Sums are fp32 and divided at the end: values beyond 2^127 / (256 keys) may overflow.  W * P is at
  * most PGN_CACHED_MAX_KEYS.  workspace: pgn_cached_attention_workspace_bytes bytes, 16-byte aligned, contents irrelevant. */
 #define PGN_CACHED_MAX_KEYS 268435456
 size_t pgn_cached_attention_workspace_bytes(int num_tokens, int R, int packed, int Hq, int Hkv, int head_dim, int W,

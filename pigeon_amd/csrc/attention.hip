@@ -323,20 +323,19 @@ __global__ __launch_bounds__(NWAVES * 64, MINW) void pgn_attn_fwd_kernel(AttnArg
 #pragma unroll
                 for (int r = 0; r < 16; r += 2) {
                     f32x2_t o2 = {oacc[d][r], oacc[d][r + 1]};
-                    o2 *= alpha2;   // v_pk_mul_f32
+                    o2 *= alpha2;
                     oacc[d][r] = o2[0];
                     oacc[d][r + 1] = o2[1];
                 }
             m_run = m_new;
         }
         const float mc = m_run * cm;
-        // packed fp32 math (v_pk_fma_f32 / v_pk_add_f32): two scores per VALU instruction.  Packed instructions do not
-        // issue underneath an MFMA (see pgn_attn_w64r_kernel); with this kernel's three waves per SIMD the plain form
-        // measured the same (+-0.5 %, profiles/r02_attention_32row_plain_valu_ab.txt) and costs a few spilled registers
-        // at the 168-VGPR cap, so the packed form stays here
+        // Written in float pairs, which the build turns into plain instructions (it has packed fp32 arithmetic off).  Packed
+        // ones do not issue underneath an MFMA (see pgn_attn_w64r_kernel); with this kernel's three waves per SIMD both
+        // measured the same (+-0.5 %, profiles/r02_attention_32row_plain_valu_ab.txt)
         const f32x2_t c2 = {HAS_BIAS ? 1.0f : a.c, HAS_BIAS ? 1.0f : a.c};
         const f32x2_t nmc2 = {-mc, -mc};
-        f32x2_t lsum2[2] = {{0.f, 0.f}, {0.f, 0.f}};   // two chains: no dependent back-to-back packed adds
+        f32x2_t lsum2[2] = {{0.f, 0.f}, {0.f, 0.f}};   // two chains: no dependent back-to-back adds
         u16x8_t pf[2][2];
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)

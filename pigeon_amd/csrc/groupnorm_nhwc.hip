@@ -111,8 +111,8 @@ __device__ __forceinline__ float nh_silu(float v) {
 
 // HAS_ADD (the per-(sample, channel) addend of ResnetBlock2D's norm2) and, in the apply kernel, ACT are compile-time:
 // as run-time flags they were if-converted into ~110 v_cndmask per loop body.  The per-element arithmetic is written on
-// float pairs so that it compiles to packed fp32 instructions (v_pk_add / v_pk_mul / v_pk_fma: two elements per issue
-// slot); the operations and their order are unchanged, results are bit-identical to the scalar form.
+// float pairs, which the build turns into plain fp32 instructions (it has packed arithmetic off); the operations and
+// their order are those of the scalar form, results are bit-identical to it.
 // one 16-byte vector of a lane's column into its pivot-shifted sums: shared by the statistics launch and by the
 // producer-side form (pgn_bias_res_stats_kernel), whose words must be the statistics launch's bit for bit
 template <int DT, bool HAS_ADD>
