@@ -524,8 +524,10 @@ __global__ __launch_bounds__(PGN_SAMPLE_THREADS) void pgn_sample_tokens_kernel(c
         if (bin >= PGN_SAMPLE_BINS - 1 || x != x) return -INFINITY;      // the last bin has no end; inf - inf
         return fabsf(x) < INFINITY ? x - fabsf(x) * 0x1p-23f : x;
     };
-    // gathers the ids from `low` up, of all bins or of one; how many there are (the list takes PGN_SAMPLE_LIST of them)
-    const auto gather = [&](float low, int only) {
+    // gathers the ids of the bins from `first` to `last`; how many there are (the list takes PGN_SAMPLE_LIST of them).  lowest()
+    // only keeps most of the others from being looked at: it has slack, so it must not be what decides.
+    const auto gather = [&](int first, int last) {
+        const float low = lowest(last);
         __syncthreads();
         if (tid == 0) s.count = 0;
         __syncthreads();
@@ -539,7 +541,8 @@ __global__ __launch_bounds__(PGN_SAMPLE_THREADS) void pgn_sample_tokens_kernel(c
                 float xe = x[0];
 #pragma unroll
                 for (int n = 1; n < E; ++n) xe = e == n ? x[n] : xe;
-                if (in && xe > -INFINITY && (only < 0 || w.bin(xe) == only)) {
+                const int bin = w.bin(xe);
+                if (in && xe > -INFINITY && bin >= first && bin <= last) {
                     const int at = atomicAdd(&s.count, 1);
                     if (at < PGN_SAMPLE_LIST) s.key[at] = rank_key(xe, row.index(j, e));
                 }
@@ -550,7 +553,7 @@ __global__ __launch_bounds__(PGN_SAMPLE_THREADS) void pgn_sample_tokens_kernel(c
     };
 
     if (k > 0 && k < V) {
-        for (bool full = k > PGN_SAMPLE_THREADS;; full = true) {
+        for (bool full = k > PGN_SAMPLE_THREADS;; full = true) {             // a full pass is the last
             unsigned total = 0, before;
             if (!full) {
                 if (mine > -INFINITY) atomicAdd(&s.hist.ids[w.bin(mine)], 1u);
@@ -578,13 +581,13 @@ __global__ __launch_bounds__(PGN_SAMPLE_THREADS) void pgn_sample_tokens_kernel(c
                 break;
             }
             if (full || cut < PGN_SAMPLE_BINS - 1) {         // else there are fewer maxima than k
-                const int n = gather(lowest(cut), alone ? cut : -1);
+                const int n = gather(alone ? cut : 0, cut);
                 if (alone) {
                     sort_list(s, pad_list(s, n));
                     kept.upto(s.key[k - (int)before - 1]);
                     break;
                 }
-                if (n <= PGN_SAMPLE_LIST) {
+                if (full || n <= PGN_SAMPLE_LIST) {          // full: n is before + inside
                     finish_list(s, w, n, k, p, least, u, a.ids + b);
                     return;
                 }

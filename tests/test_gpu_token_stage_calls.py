@@ -1,0 +1,74 @@
+"""Calls of the token stage's operators that their documentation allows and that once went wrong, on the GPU against
+oracle/token_stage_ref.py."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import token_stage_ref as ref
+from pigeon_amd import ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def _ids(x, u, temperature, k, p, q):
+    """The oracle's ids, with the numbers as the fp32 that the call makes of them."""
+    f32 = lambda v: float(np.float32(v))                            # noqa: E731
+    xn, un = x.cpu().double().numpy(), u.cpu().double().numpy()
+    return [ref.sample_tokens_ref(xn[b], un[b], f32(temperature), k, f32(p), f32(q)) for b in range(len(xn))]
+
+
+# ------------------------------------------------------------------------------------------------ top-k at a full list
+LIST = 4096                                                         # ids that the kernel sorts
+
+
+def _border(row, temperature, k):
+    """Of the bins over the distance to the maximum, 32 to a factor of two of weight, in fp32 as the kernel places
+    them: ids before the bin that holds rank k, ids in it, and the ids from its lower end with 1 % of a bin of slack."""
+    x, f32 = row.cpu().float().numpy(), np.float32
+    fc = f32(32 * 1.44269504088896340736 / float(f32(temperature)))
+    bins = np.minimum(np.maximum((x.max() - x) * fc, f32(0)), f32(2047)).astype(np.int64)
+    count = np.bincount(bins, minlength=2048)
+    upto = count.cumsum()
+    cut = int(np.searchsorted(upto, k))
+    low = f32(float(x.max()) - (cut + 1.01) / float(fc))
+    return int(upto[cut] - count[cut]), int(count[cut]), int((x >= low - abs(low) * f32(2.0 ** -23)).sum())
+
+
+def _two_levels(V, many, dt):
+    """`many` ids at 2.5 and the others 1/64 under it, which is 1.0019 bins at a temperature of 0.72."""
+    x = torch.full((4, V), 2.5 - 1.0 / 64)
+    x[:, V // 7:V // 7 + many] = 2.5
+    return x.to(dt).to(DEV)
+
+
+@pytest.mark.parametrize("filters", [(1.0, 0.0), (0.9, 0.0), (0.97, 0.3)])
+@pytest.mark.parametrize("case", ["normal", "levels", "few levels", "levels fp32"])
+def test_top_k_where_ids_just_behind_the_border_would_overfill_the_list(case, filters):
+    """The bins up to the border fit the list and the ids near its lower end do not: the pass over all ids, which is the
+    last, has to take the former alone."""
+    if case == "normal":
+        g = torch.Generator().manual_seed(1)
+        x = (torch.randn(131072, generator=g) * 0.5).to(torch.bfloat16).expand(4, -1).contiguous().to(DEV)
+        temperature, ks = 1.18, (3644, 3900, 4057)
+    else:
+        x = _two_levels(5000 if case == "few levels" else 48386, 3000, torch.float32 if case == "levels fp32" else torch.bfloat16)
+        temperature, ks = 0.72, (50, 1000, 1025, 2999, 3000)
+    u = torch.tensor([0.0, 0.3, 0.71, 0.9999], device=DEV)
+    p, q = filters
+    for k in ks:
+        before, inside, near = _border(x[0], temperature, k)
+        assert before + inside <= LIST < near, (before, inside, near)        # the state in question
+        got = ops.sample_tokens(x, u, temperature=temperature, top_k=k, top_p=p, min_p=q)
+        assert got.tolist() == _ids(x, u, temperature, k, p, q), (case, k)
+
+
+@pytest.mark.parametrize("many", [4095, 4096, 4097])
+def test_top_k_with_as_many_ids_as_the_list_takes(many):
+    """Both sides of the list's length, the border in its last bin and behind it."""
+    x, u = _two_levels(30000, many, torch.bfloat16), torch.tensor([0.0, 0.5, 0.8, 0.9999], device=DEV)
+    for k in (40, 1025, many - 1, many, many + 1, 9000):
+        for p in (1.0, 0.8):
+            assert ops.sample_tokens(x, u, temperature=0.72, top_k=k, top_p=p).tolist() == _ids(x, u, 0.72, k, p, 0.0), (k, p)
