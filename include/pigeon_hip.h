@@ -453,7 +453,8 @@ int pgn_cached_attention(const void* q, int dtype, const void* k_pages, const vo
  *   ids rank by (logit descending, index ascending); NaN logits count as -inf, and -inf is never drawn
  *   top_k >= 1 keeps the first top_k ids; w_i = exp((x_i - max) / temperature)
  *   top_p < 1 keeps the shortest run of first ids whose weight reaches top_p of all that top_k kept (one at least)
- *   min_p keeps the ids with w_i >= min_p (of the largest weight, 1)
+ *   min_p keeps the ids with w_i >= min_p (of the largest weight, 1), and the largest logits whatever min_p is: above 1,
+ *     or NaN, it keeps no others
  *   the id drawn is the first, in index order, whose running sum of kept weights exceeds u times their sum
  * temperature <= 0 or NaN takes the first id in rank; a row without any logit above -inf gives -1.  Weights are computed
  * in 64 bits and summed as integers of 2^-45: the same ids every time. */

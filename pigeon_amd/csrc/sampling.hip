@@ -173,6 +173,7 @@ struct Kept {
 
 struct Weights {
     double max, c;                                           // c: 1024 log2(e) / temperature, not 0
+    double least;                                            // min-p as a weight
     float fmax, fc;                                          // fc: bins per unit of distance
     const double* table;
     // w 2^45, nearest whole number.  2^-(t / 1024) with t = k + f, k whole, |f| <= 1/2: a table of 2^-(k % 1024 / 1024),
@@ -188,6 +189,9 @@ struct Weights {
         const double up = __hiloint2double((1023 + PGN_SAMPLE_BITS - (k >> 10)) << 20, 0);
         return (u64)__double_as_longlong(fma(e, up, 0x1p52)) & 0xfffffffffffffull;
     }
+    // min-p's rule, the same wherever weights are summed or drawn from: the largest logits stay whatever min-p is, above 1 or
+    // NaN, and of others only the weight counts.  (A weight of 1 need not be theirs: at a high temperature others round to it.)
+    __device__ __forceinline__ bool leaves(u64 v, float x) const { return (double)v >= least || x == fmax; }
     // monotone in x > -inf: 32 bins to a factor of two, everything from 2^-64 on in the last; a NaN (inf - inf, 0 inf) is 0
     __device__ __forceinline__ int bin(float x) const {
         return (int)fminf(fmaxf((fmax - x) * fc, 0.f), (float)(PGN_SAMPLE_BINS - 1));
@@ -390,12 +394,10 @@ __device__ __forceinline__ u64 nucleus_target(float p, u64 z) {
     return t < z ? t : z;
 }
 
-// The rest of a top-k among the n ids of the list, the first k in rank among them: top-p, min-p and the draw.  `least`:
-// min-p as a weight.  A few ids compare each with each (ranks and running sums without a sort, three rounds); more are
-// sorted by rank, then by index.
-__device__ __forceinline__ void finish_list(SampleLds& s, const Weights& w, int n, int k, float p, double least, float u, int64_t* id) {
+// The rest of a top-k among the n ids of the list, the first k in rank among them: top-p, min-p and the draw.  A few ids
+// compare each with each (ranks and running sums without a sort, three rounds); more are sorted by rank, then by index.
+__device__ __forceinline__ void finish_list(SampleLds& s, const Weights& w, int n, int k, float p, float u, int64_t* id) {
     const int tid = threadIdx.x;
-    const u64 one = 1ull << PGN_SAMPLE_BITS;
     u64 z;
     if (n <= PGN_SAMPLE_FEW) {
         u64 key = 0, v = 0;
@@ -420,7 +422,7 @@ __device__ __forceinline__ void finish_list(SampleLds& s, const Weights& w, int 
                 v = before < target ? v : 0;
             }
         }
-        if (!((double)v >= least || v == one)) v = 0;
+        if (!w.leaves(v, rank_value((unsigned)(key >> 24)))) v = 0;
         __syncthreads();
         if (tid < n) s.weight[tid] = v;
         if (tid == 0) s.found = ~0ull;
@@ -449,7 +451,7 @@ __device__ __forceinline__ void finish_list(SampleLds& s, const Weights& w, int 
     u64 sum = 0;
     for (int i = tid; i < kept; i += PGN_SAMPLE_THREADS) {
         const u64 v = s.weight[i];
-        const bool on = (double)v >= least || v == one;
+        const bool on = w.leaves(v, rank_value((unsigned)(s.key[i] >> 24)));
         s.weight[i] = on ? v : 0;
         s.key[i] &= 0xffffff;                                // by index now
         sum += on ? v : 0;
@@ -515,7 +517,7 @@ __global__ __launch_bounds__(PGN_SAMPLE_THREADS) void pgn_sample_tokens_kernel(c
     w.c = fmax(PGN_SAMPLE_TABLE * 1.44269504088896340736 / (double)t, 1e-300);        // t may be infinite
     w.fc = (float)(PGN_SAMPLE_BINS_PER_OCTAVE * 1.44269504088896340736 / (double)t);
     w.table = s.table;
-    const double least = (double)min_p * (double)(1ull << PGN_SAMPLE_BITS);
+    w.least = (double)min_p * (double)(1ull << PGN_SAMPLE_BITS);
     Kept kept = {-INFINITY, -1};                             // everything that can be drawn
 
     // a logit that no id of a bin up to `bin` is under (1 % of a bin and an ulp cover the rounding of the places)
@@ -588,7 +590,7 @@ __global__ __launch_bounds__(PGN_SAMPLE_THREADS) void pgn_sample_tokens_kernel(c
                     break;
                 }
                 if (full || n <= PGN_SAMPLE_LIST) {          // full: n is before + inside
-                    finish_list(s, w, n, k, p, least, u, a.ids + b);
+                    finish_list(s, w, n, k, p, u, a.ids + b);
                     return;
                 }
             }
@@ -634,8 +636,9 @@ __global__ __launch_bounds__(PGN_SAMPLE_THREADS) void pgn_sample_tokens_kernel(c
         u64* pile = s.pile[wid];
         int held = 0;
         const auto weigh = [&](bool on, u64 entry) {
-            u64 v = on ? w.fixed(__uint_as_float((unsigned)entry)) : 0;
-            if (!((double)v >= least || v == 1ull << PGN_SAMPLE_BITS)) v = 0;
+            const float xe = __uint_as_float((unsigned)entry);
+            u64 v = on ? w.fixed(xe) : 0;
+            if (!w.leaves(v, xe)) v = 0;
             const int at = on ? ((int)(entry >> 32) + row.lead) / (64 * E) : 0;
             if (__all(at == __builtin_amdgcn_readfirstlane(at))) {           // one stretch: summed here, not by 64 turns in LDS
                 v = wave_scan(v);
@@ -680,7 +683,8 @@ __global__ __launch_bounds__(PGN_SAMPLE_THREADS) void pgn_sample_tokens_kernel(c
         const int n = s.count;
         if (n <= PGN_SAMPLE_FEW) {                           // compared each with each
             u64 key = 0, v = 0;
-            if (tid < n) s.weight[tid] = v = w.fixed(rank_value((unsigned)((key = s.key[tid]) >> 24)));
+            float xe = -INFINITY;
+            if (tid < n) s.weight[tid] = v = w.fixed(xe = rank_value((unsigned)((key = s.key[tid]) >> 24)));
             if (tid == 0) s.found = 0;
             __syncthreads();
             if (tid < n) {
@@ -692,7 +696,7 @@ __global__ __launch_bounds__(PGN_SAMPLE_THREADS) void pgn_sample_tokens_kernel(c
                 }
                 if (before < inside_target) {
                     atomicMax(&s.found, key);
-                    if ((double)v >= least || v == 1ull << PGN_SAMPLE_BITS)
+                    if (w.leaves(v, xe))
                         atomicAdd(&s.seg[((int)(key & 0xffffff) + row.lead) / (64 * E)], v);
                 }
             }
@@ -708,7 +712,7 @@ __global__ __launch_bounds__(PGN_SAMPLE_THREADS) void pgn_sample_tokens_kernel(c
             kept.upto(s.key[last]);
             for (int i = tid; i <= last; i += PGN_SAMPLE_THREADS) {
                 const u64 v = s.weight[i];
-                if ((double)v >= least || v == 1ull << PGN_SAMPLE_BITS)
+                if (w.leaves(v, rank_value((unsigned)(s.key[i] >> 24))))
                     atomicAdd(&s.seg[((int)(s.key[i] & 0xffffff) + row.lead) / (64 * E)], v);
             }
             __syncthreads();
@@ -745,7 +749,7 @@ __global__ __launch_bounds__(PGN_SAMPLE_THREADS) void pgn_sample_tokens_kernel(c
 #pragma unroll
     for (int e = 0; e < E; ++e) {
         const u64 f = kept(x[e], row.index(j, e)) ? w.fixed(x[e]) : 0;
-        v[e] = (double)f >= least || x[e] == m ? f : 0;
+        v[e] = w.leaves(f, x[e]) ? f : 0;
         sum += v[e];
     }
     u64 c = before + wave_scan(sum) - sum;

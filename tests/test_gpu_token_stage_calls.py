@@ -72,3 +72,23 @@ def test_top_k_with_as_many_ids_as_the_list_takes(many):
     for k in (40, 1025, many - 1, many, many + 1, 9000):
         for p in (1.0, 0.8):
             assert ops.sample_tokens(x, u, temperature=0.72, top_k=k, top_p=p).tolist() == _ids(x, u, 0.72, k, p, 0.0), (k, p)
+
+
+# ------------------------------------------------------------------------------------------------ min-p above every weight
+@pytest.mark.parametrize("min_p", [0.5, 1.0, 1.5, 2.0, math.inf, math.nan])
+@pytest.mark.parametrize("temperature", [math.inf, 3e38, 1.0])
+@pytest.mark.parametrize("V,top_k", [(4, 0), (4, 3), (3001, 0), (3001, 40), (3001, 900), (40000, 0), (40000, 5000), (48386, 4000)])
+def test_min_p_leaves_the_same_ids_in_the_sums_and_in_the_draw(V, top_k, temperature, min_p):
+    """At a high temperature weights of ids under the maximum are 1 too: above 1, or NaN, min-p leaves the largest logits
+    alone, at 1 and below all of them.  Sums over more than the draw finds leave an id unwritten."""
+    x = -(torch.arange(V) % 1000).float() / 64
+    x = torch.stack([x, x.flip(0), torch.zeros(V), x.roll(V // 3)])
+    x[1, V // 2] = -math.inf
+    u = torch.tensor([0.9, 0.0, 0.6, 0.9999], device=DEV)
+    for dt in (torch.float32, torch.bfloat16):
+        y = x.to(dt).to(DEV)
+        for p in (1.0, 0.75):
+            want = _ids(y, u, temperature, top_k, p, min_p)
+            assert ops.sample_tokens(y, u, temperature=temperature, top_k=top_k, top_p=p, min_p=min_p).tolist() == want, (dt, p)
+            rows = torch.full((4,), min_p, device=DEV)
+            assert ops.sample_tokens(y, u, temperature=temperature, top_k=top_k, top_p=p, min_p=rows).tolist() == want, (dt, p)
