@@ -892,10 +892,10 @@ def cached_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     if T == 0 or R == 0:
         return out
     window = min(int(window), 2 ** 31 - 1)                     # as wide as any: the C argument would wrap
-    if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
-        q = q.contiguous()                                     # rows are read 16 bytes at a time
-        if q.data_ptr() % 16:
-            q = q.clone()
+    q_st, q_sh = (q.stride(0) if T > 1 else 0), (q.stride(1) if Hq > 1 else 0)      # that of a single token or head may be any
+    if q.stride(2) != 1 or q_st % 8 or q_sh % 8 or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)     # rows are read 16 bytes at a time
+        q_st, q_sh = Hq * D, D
     packed = starts is not None
     nbytes = _cached_attention_bytes(T, R, packed, Hq, H, D, W, P)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
@@ -905,7 +905,7 @@ def cached_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
         _call(dev, "pgn_cached_attention", lib.pgn_cached_attention, q.data_ptr(), _dt(q), k_pages.data_ptr(),
               v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), table.data_ptr(),
               table.stride(0) if R > 1 else W, lens.data_ptr(), _ptr(starts), out.data_ptr(), T, R, Hq, H, D, N, W, P,
-              q.stride(0), q.stride(1), out.stride(0), out.stride(1), scale, int(causal), window, _ptr(ws), nbytes)
+              q_st, q_sh, out.stride(0), out.stride(1), scale, int(causal), window, _ptr(ws), nbytes)
 
     _launch("cached_attention", 4.0 * T * Hq * D, run)
     return out

@@ -92,3 +92,34 @@ def test_min_p_leaves_the_same_ids_in_the_sums_and_in_the_draw(V, top_k, tempera
             assert ops.sample_tokens(y, u, temperature=temperature, top_k=top_k, top_p=p, min_p=min_p).tolist() == want, (dt, p)
             rows = torch.full((4,), min_p, device=DEV)
             assert ops.sample_tokens(y, u, temperature=temperature, top_k=top_k, top_p=p, min_p=rows).tolist() == want, (dt, p)
+
+
+# ------------------------------------------------------------------------------------------------ attention: layouts of q
+def _attention_inputs(T, H, D, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    P, N = 16, 12
+    cache = [torch.randn(N, H, P, D, generator=g).to(torch.float8_e4m3fn).to(DEV), torch.randn(N, H, D, P, generator=g).to(torch.float8_e4m3fn).to(DEV),
+             torch.ones(N, H, device=DEV), torch.ones(N, H, device=DEV)]
+    table = torch.randperm(N, generator=g)[:4 * min(T, 3)].view(-1, 4).to(torch.int32).to(DEV)
+    return cache, table, torch.full((len(table),), 61, dtype=torch.int32, device=DEV), g
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,Hq,D", [(1, 4, 64), (3, 1, 128), (1, 1, 64), (1, 2, 256)])
+@pytest.mark.parametrize("pitch,first", [(3, 0), (3, 2), (8, 8), (8, 4), (0, 1)])
+def test_queries_of_one_token_or_one_head_with_any_stride(T, Hq, D, pitch, first, dt):
+    """Slices of wider rows: torch calls a tensor contiguous whatever the stride of an axis of length 1 is."""
+    cache, table, lens, g = _attention_inputs(T, 1, D)
+    if T == 1:                                                      # a row of a [2, heads, D] tensor
+        q = torch.randn(2, Hq * D + pitch + first, generator=g).to(dt).to(DEV)[:, first:first + Hq * D].unflatten(1, (Hq, D))[:1]
+        assert q.is_contiguous() and q.stride(0) == Hq * D + pitch + first
+    else:                                                           # a head of a [2, T, D] tensor
+        q = torch.randn(2, T * D + pitch + first, generator=g).to(dt).to(DEV)[:, first:first + T * D].unflatten(1, (T, D)).transpose(0, 1)[:, :1]
+        assert q.is_contiguous() and q.stride(1) == T * D + pitch + first
+    starts = None if T == len(lens) else torch.tensor([0, T], dtype=torch.int32, device=DEV)
+    plain = torch.empty(T, Hq, D, dtype=dt, device=DEV)
+    plain.copy_(q)
+    want = ops.cached_attention(plain, *cache, table, lens, starts=starts)
+    assert torch.equal(ops.cached_attention(q, *cache, table, lens, starts=starts), want)
+    out = torch.empty(T, Hq, D + 3, dtype=dt, device=DEV)[:, :, 1:D + 1]
+    assert torch.equal(ops.cached_attention(q, *cache, table, lens, starts=starts, out=out), want)
