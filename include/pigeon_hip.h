@@ -401,7 +401,7 @@ int pgn_image_to_uint8(const void* x, int x_dtype, void* y, int N, int C, int H,
  *   v_pages  e4m3 [num_pages, kv_heads, D, P]     v_scale  fp32 [num_pages, kv_heads]
  * key = k_scale * byte, value = v_scale * byte; scales are powers of two.  Pages 16-byte aligned.
  * Requests: lens int32 [R] tokens held, table int32 [R, W] (row stride table_stride) pages in order; position p of
- * request r is token p % P of page table[r][p / P], slot page * P + p % P.
+ * request r is token p % P of page table[r][p / P], slot page * P + p % P.  num_pages, R and W are 1 at least.
  *
  * Page bookkeeping of a step, all on the device and in place.  keep (or NULL: all) says how many of its tokens each
  * request keeps (clamped to [0, lens]; 0 ends it, fewer than lens rolls it back); pages behind them go back on the

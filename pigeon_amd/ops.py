@@ -784,6 +784,11 @@ def _i32(t: torch.Tensor, shape, name: str):
         raise ValueError(f"{name} must be a contiguous int32 tensor of shape {tuple(shape)}")
 
 
+def _check_table(table, R):
+    if table.dim() != 2 or table.dtype != torch.int32 or table.shape[0] != R or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError("table must be int32 [R, W] with contiguous rows")
+
+
 def _check_pages(k_pages, v_pages, k_scale, v_scale):
     """(num_pages, kv_heads, page_size, head_dim) of one layer's cache."""
     if k_pages.dim() != 4 or k_pages.dtype != torch.float8_e4m3fn or v_pages.dtype != torch.float8_e4m3fn:
@@ -799,22 +804,33 @@ def _check_pages(k_pages, v_pages, k_scale, v_scale):
     return N, H, P, D
 
 
+def _some(N=1, H=1, W=1):
+    if N == 0 or H == 0:
+        raise ValueError("a cache must have a page and a head at least")
+    if W == 0:
+        raise ValueError("a table must have a column at least")
+
+
 def page_advance(lens: torch.Tensor, add: torch.Tensor, table: torch.Tensor, free_pages: torch.Tensor,
                  free_count: torch.Tensor, page_size: int, num_slots: int, keep: Optional[torch.Tensor] = None):
     """One step of the block tables (pgn_page_advance), in place on lens [R], table [R, W], the stack of free pages
-    free_pages [num_pages] and its height free_count [1], all int32.  `keep` [R]: tokens that each request keeps of those
-    it holds (None: all); `add` [R]: tokens that it gets.  num_slots: length of the slot map, sum(add) or more.
+    free_pages [num_pages] and its height free_count [1], all int32; W and num_pages are 1 at least.  `keep` [R]: tokens
+    that each request keeps of those it holds (None: all); `add` [R]: tokens that it gets.  num_slots: length of the slot
+    map, sum(add) or more.
     Returns dict(slots int64 [num_slots], starts int32 [R + 1], status int32 [R]: 1 where a request was refused).
     No host sync."""
     lib = _lib.load()
     dev = _on(lens, add, table, free_pages, free_count, keep)
     R = lens.numel()
-    if table.dim() != 2 or table.dtype != torch.int32 or table.shape[0] != R or (table.shape[1] > 1 and table.stride(1) != 1):
-        raise ValueError("table must be int32 [R, W] with contiguous rows")
+    _check_table(table, R)
     _i32(lens, (R,), "lens")
     _i32(add, (R,), "add")
     _i32(free_pages, (free_pages.numel(),), "free_pages")
     _i32(free_count, (1,), "free_count")
+    if R > 0:
+        _some(W=table.shape[1])
+        if free_pages.numel() == 0:
+            raise ValueError("free_pages must have room for a page at least")
     if keep is not None:
         _i32(keep, (R,), "keep")
     W = table.shape[1]
@@ -850,6 +866,7 @@ def cache_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_pages: 
         raise ValueError("cache_write: slots must be a contiguous int64 [T]")
     if T == 0:
         return
+    _some(N, H)
     k, v = (t if t.stride(2) == 1 else t.contiguous() for t in (k, v))
 
     def run():
@@ -869,17 +886,17 @@ def cached_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     starts int32 [R + 1]: request r owns tokens starts[r] .. starts[r + 1), the last of the lens[r] that it holds, itself
     among them; None: one token a request.  causal: a token sees keys up to its own position, the last `window` of them
     if window > 0.  A row that sees nothing is zero.  Rows behind starts[R] are not written: they keep what `out` held,
-    or stay unset in the tensor made here.  Returns [T, heads, head_dim]."""
+    or stay unset in the tensor made here.  The table has a column and the cache a page at least.  Returns
+    [T, heads, head_dim]."""
     lib = _lib.load()
     dev = _on(q, k_pages, v_pages, k_scale, v_scale, table, lens, starts, out)
     N, H, P, D = _check_pages(k_pages, v_pages, k_scale, v_scale)
-    if q.dim() != 3 or q.shape[2] != D or q.shape[1] % H:
+    if q.dim() != 3 or q.shape[2] != D or (q.shape[1] % H if H else q.shape[1]):
         raise ValueError("cached_attention: q must be [T, heads, head_dim] with heads a multiple of kv_heads")
     T, Hq, _ = q.shape
     R = lens.numel()
     _i32(lens, (R,), "lens")
-    if table.dim() != 2 or table.dtype != torch.int32 or table.shape[0] != R or (table.shape[1] > 1 and table.stride(1) != 1):
-        raise ValueError("table must be int32 [R, W] with contiguous rows")
+    _check_table(table, R)
     W = table.shape[1]
     if starts is not None:
         _i32(starts, (R + 1,), "starts")
@@ -891,6 +908,7 @@ def cached_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
         raise ValueError("cached_attention: out must match q, with a contiguous last dim")
     if T == 0 or R == 0:
         return out
+    _some(N, H, W)
     window = min(int(window), 2 ** 31 - 1)                     # as wide as any: the C argument would wrap
     q_st, q_sh = (q.stride(0) if T > 1 else 0), (q.stride(1) if Hq > 1 else 0)      # that of a single token or head may be any
     if q.stride(2) != 1 or q_st % 8 or q_sh % 8 or q.data_ptr() % 16:

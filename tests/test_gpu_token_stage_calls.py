@@ -123,3 +123,27 @@ def test_queries_of_one_token_or_one_head_with_any_stride(T, Hq, D, pitch, first
     assert torch.equal(ops.cached_attention(q, *cache, table, lens, starts=starts), want)
     out = torch.empty(T, Hq, D + 3, dtype=dt, device=DEV)[:, :, 1:D + 1]
     assert torch.equal(ops.cached_attention(q, *cache, table, lens, starts=starts, out=out), want)
+
+
+# ------------------------------------------------------------------------------------------------ refusals
+def test_tables_without_a_column_and_caches_without_a_page_are_refused_by_name():
+    cache, table, lens, g = _attention_inputs(2, 1, 64)
+    q = torch.randn(2, 1, 64, generator=g).to(torch.bfloat16).to(DEV)
+    i32 = lambda n: torch.zeros(n, dtype=torch.int32, device=DEV)                               # noqa: E731
+    empty = torch.empty(2, 0, dtype=torch.int32, device=DEV)
+    with pytest.raises(ValueError, match="column"):
+        ops.cached_attention(q, *cache, empty, i32(2))
+    with pytest.raises(ValueError, match="column"):
+        ops.page_advance(i32(2), i32(2), empty, i32(4), i32(1), 16, 2)
+    with pytest.raises(ValueError, match="room for a page"):
+        ops.page_advance(i32(2), i32(2), table, i32(0), i32(1), 16, 2)
+    none = [t[:0] for t in cache]
+    with pytest.raises(ValueError, match="page and a head"):
+        ops.cached_attention(q, *none, table, lens)
+    with pytest.raises(ValueError, match="page and a head"):
+        ops.cache_write(q, q, torch.zeros(2, dtype=torch.int64, device=DEV), *none)
+    # nothing to do is no error, whatever there is to do it with
+    assert ops.cached_attention(q, *cache, empty[:0], i32(0), starts=i32(1)).shape == q.shape
+    assert ops.cached_attention(q[:0], *none, empty, i32(2), starts=i32(3)).shape == (0, 1, 64)
+    ops.cache_write(q[:0], q[:0], torch.zeros(0, dtype=torch.int64, device=DEV), *none)
+    assert ops.page_advance(i32(0), i32(0), empty[:0], i32(0), i32(1), 16, 2)["slots"].tolist() == [-1, -1]
