@@ -779,6 +779,12 @@ def _cached_attention_bytes(*sizes) -> int:
     return _lib.load().pgn_cached_attention_workspace_bytes(*sizes)
 
 
+def _c_int(*sizes):
+    """ctypes cuts an int argument to 32 bits without a word: what does not fit is refused here."""
+    if max(sizes) >= 2 ** 31 or min(sizes) < -2 ** 31:
+        raise NotImplementedError(f"pigeon_amd: a size beyond 32 bits in {sizes}")
+
+
 def _i32(t: torch.Tensor, shape, name: str):
     if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor of shape {tuple(shape)}")
@@ -834,6 +840,7 @@ def page_advance(lens: torch.Tensor, add: torch.Tensor, table: torch.Tensor, fre
     if keep is not None:
         _i32(keep, (R,), "keep")
     W = table.shape[1]
+    _c_int(R, W, free_pages.numel(), page_size)
     if R > 1 and table.stride(0) < W:
         raise ValueError("the rows of table overlap")
     slots = torch.empty(num_slots, dtype=torch.int64, device=dev)
@@ -867,6 +874,7 @@ def cache_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_pages: 
     if T == 0:
         return
     _some(N, H)
+    _c_int(N)
     k, v = (t if t.stride(2) == 1 else t.contiguous() for t in (k, v))
 
     def run():
@@ -910,6 +918,9 @@ def cached_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
         return out
     _some(N, H, W)
     window = min(int(window), 2 ** 31 - 1)                     # as wide as any: the C argument would wrap
+    if window < 0:
+        raise ValueError("cached_attention: window must not be negative")
+    _c_int(T, R, W, N)
     q_st, q_sh = (q.stride(0) if T > 1 else 0), (q.stride(1) if Hq > 1 else 0)      # that of a single token or head may be any
     if q.stride(2) != 1 or q_st % 8 or q_sh % 8 or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)     # rows are read 16 bytes at a time
@@ -950,8 +961,7 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, 
     ids = torch.empty(B, dtype=torch.int64, device=dev)
     if B == 0:
         return ids
-    if V > 2 ** 31 - 1:
-        raise NotImplementedError("sample_tokens: too many ids")
+    _c_int(B, V)
     if logits.stride(1) != 1 and V > 1:
         logits = logits.contiguous()
     tt, kt, pt, mt = tensors

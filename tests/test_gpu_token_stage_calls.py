@@ -147,3 +147,16 @@ def test_tables_without_a_column_and_caches_without_a_page_are_refused_by_name()
     assert ops.cached_attention(q[:0], *none, empty, i32(2), starts=i32(3)).shape == (0, 1, 64)
     ops.cache_write(q[:0], q[:0], torch.zeros(0, dtype=torch.int64, device=DEV), *none)
     assert ops.page_advance(i32(0), i32(0), empty[:0], i32(0), i32(1), 16, 2)["slots"].tolist() == [-1, -1]
+
+
+def test_sizes_that_would_be_cut_to_32_bits_are_refused():
+    """2^32 + n must not pass for n, nor -2^32 + n."""
+    cache, table, lens, g = _attention_inputs(2, 1, 64)
+    q = torch.randn(2, 1, 64, generator=g).to(torch.bfloat16).to(DEV)
+    i32 = lambda n: torch.zeros(n, dtype=torch.int32, device=DEV)                               # noqa: E731
+    for window in (-1, -2 ** 31, -2 ** 32, -2 ** 32 + 5):
+        with pytest.raises(ValueError):
+            ops.cached_attention(q, *cache, table, lens, window=window)
+    for page_size in (2 ** 32 + 16, -2 ** 32 + 64, 2 ** 31, 0, -16):
+        with pytest.raises(NotImplementedError):
+            ops.page_advance(i32(2), i32(2), table, i32(4), i32(1), page_size, 2)
