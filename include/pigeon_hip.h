@@ -402,6 +402,8 @@ int pgn_image_to_uint8(const void* x, int x_dtype, void* y, int N, int C, int H,
  * key = k_scale * byte, value = v_scale * byte; scales are powers of two.  Pages 16-byte aligned.
  * Requests: lens int32 [R] tokens held, table int32 [R, W] (row stride table_stride) pages in order; position p of
  * request r is token p % P of page table[r][p / P], slot page * P + p % P.  num_pages, R and W are 1 at least.
+ * A call that needs 2^32 threads is refused before any launch (PGN_ERR_UNSUPPORTED): sampling from 2^22 rows on, attention
+ * where kv_heads times the requests and the tiles of rows that they need come to 2^24.
  *
  * Page bookkeeping of a step, all on the device and in place.  keep (or NULL: all) says how many of its tokens each
  * request keeps (clamped to [0, lens]; 0 ends it, fewer than lens rolls it back); pages behind them go back on the

@@ -1026,7 +1026,8 @@ extern "C" int pgn_cached_attention(const void* q, int dtype, const void* k_page
         !pgn_aligned(out, 2))
         return PGN_ERR_INVALID;
     const CachedPlan p = cached_plan(num_tokens, R, starts != nullptr, Hq / Hkv, Hkv, head_dim, (int64_t)W << shift);
-    if ((int64_t)p.tiles * Hkv > 0x7fffffff || (int64_t)p.big_tiles * Hkv > 0x7fffffff) return PGN_ERR_UNSUPPORTED;
+    const int64_t widest = p.few_slots > p.tiles ? p.few_slots : p.tiles;
+    if ((widest > p.big_tiles ? widest : p.big_tiles) * Hkv > PGN_MAX_GRID / PGN_CA_THREADS) return PGN_ERR_UNSUPPORTED;
     const size_t need = cached_workspace(p, (int64_t)num_tokens * Hq, Hkv, head_dim);
     if (need > 0 && (workspace == nullptr || workspace_bytes < need || !pgn_aligned(workspace, 16))) return PGN_ERR_INVALID;
     CachedArgs a;

@@ -620,7 +620,7 @@ extern "C" int pgn_cache_write(const void* k, const void* v, int dtype, const in
     // token: 42, 48 and 59 us).
     const int chunk = T <= 512 ? 4 : T <= 1024 ? 16 : 64;
     const int64_t wgs = (int64_t)(((T + chunk - 1) / chunk + 7) / 8 * 8) * kv_heads;
-    if (wgs > 0x7fffffff) return PGN_ERR_UNSUPPORTED;
+    if (wgs > PGN_MAX_GRID / (PGN_CW_WAVES * 64)) return PGN_ERR_UNSUPPORTED;
     const dim3 grid((unsigned)wgs, 2);
     hipStream_t s = (hipStream_t)stream;
 #define PGN_CW_LAUNCH(DT, D)                                                                                           \

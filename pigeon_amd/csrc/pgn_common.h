@@ -6,6 +6,7 @@
 #include "../../include/pigeon_hip.h"
 
 #define PGN_WAVE 64
+#define PGN_MAX_GRID 0xffffffffll /* threads that a launch may have along one axis */
 
 #define PGN_LAUNCH_CHECK()                          \
     do {                                            \

@@ -771,7 +771,7 @@ extern "C" int pgn_sample_tokens(const void* logits, int dtype, int64_t stride, 
                                  void* stream) {
     if (logits == nullptr || u == nullptr || ids == nullptr || B <= 0 || V <= 0 || stride < 0) return PGN_ERR_INVALID;
     if (dtype != PGN_F32 && dtype != PGN_BF16 && dtype != PGN_F16) return PGN_ERR_UNSUPPORTED;
-    if (V > PGN_SAMPLE_MAX_IDS) return PGN_ERR_UNSUPPORTED;
+    if (V > PGN_SAMPLE_MAX_IDS || B > PGN_MAX_GRID / PGN_SAMPLE_THREADS) return PGN_ERR_UNSUPPORTED;
     if (!pgn_aligned(logits, pgn_dtype_size(dtype))) return PGN_ERR_INVALID;
     SampleArgs a;
     a.logits = logits;
