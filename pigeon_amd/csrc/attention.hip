@@ -332,7 +332,9 @@ __global__ __launch_bounds__(NWAVES * 64, MINW) void pgn_attn_fwd_kernel(AttnArg
         const float mc = m_run * cm;
         // Written in float pairs, which the build turns into plain instructions (it has packed fp32 arithmetic off).  Packed
         // ones do not issue underneath an MFMA (see pgn_attn_w64r_kernel); with this kernel's three waves per SIMD both
-        // measured the same (+-0.5 %, profiles/r02_attention_32row_plain_valu_ab.txt)
+        // measured the same (+-0.5 %, profiles/r02_attention_32row_plain_valu_ab.txt).  Plain ones cost the forms without
+        // a key bias a few registers over their 168 (one spilled at full key tiles, five with a ragged tail, none of
+        // them in the loop over the full tiles)
         const f32x2_t c2 = {HAS_BIAS ? 1.0f : a.c, HAS_BIAS ? 1.0f : a.c};
         const f32x2_t nmc2 = {-mc, -mc};
         f32x2_t lsum2[2] = {{0.f, 0.f}, {0.f, 0.f}};   // two chains: no dependent back-to-back adds
@@ -650,13 +652,13 @@ __global__ __launch_bounds__(256, 2) void pgn_attn_w64_kernel(AttnArgs a) {
 // tile t+... i.e. two tile times later, before a raw s_barrier; the V fragment reads are inline asm (invisible to the
 // wait-count pass), issued early (block d = 0 between the two query blocks' softmax, d = 1 after it) and fenced by
 // counted lgkmcnt waits that take the fragment registers as in/out operands, so that no use can move above its wait.
-// Template parameters: the shipped instantiations are <DT, SUMCHK = true, PACKED = false, PIPE = 2, RAGGED = false / true>;
+// Template parameters: the shipped instantiations are <DT, SUMCHK = true, PIPE = 2, RAGGED = false / true>;
 //   SUMCHK  no row maximum on the common path (the lane's sum of its 32 probabilities is the overflow check)
-//   PACKED  softmax arithmetic in packed fp32 instructions (measurement build only: they do not issue under an MFMA)
 //   PIPE    0: per-block order + first-tile branch, 1: no first-tile branch, 2: both V fragment blocks read before the
 //           second query block's softmax and the first block's PV MFMAs placed between its exponentials and its check
-// (the earlier forms stay selectable in the measurement build so that every A/B in profiles/ can be repeated).
-template <int DT, bool SUMCHK, bool PACKED = false, int PIPE = 0, bool RAGGED = false>
+// (the earlier forms stay selectable in the measurement build so that the A/Bs in profiles/ can be repeated; not those
+// against softmax arithmetic in packed fp32 instructions, which the build no longer forms).
+template <int DT, bool SUMCHK, int PIPE = 0, bool RAGGED = false>
 __global__ __launch_bounds__(256, 2) void pgn_attn_w64r_kernel(AttnArgs a) {
     constexpr int DP = 64, QB = 2;
     constexpr int TILE_BYTES = ATT_BN * DP * 2;          // 8 KiB
@@ -750,7 +752,6 @@ __global__ __launch_bounds__(256, 2) void pgn_attn_w64r_kernel(AttnArgs a) {
         m_run[qb] = -1.0e30f;
         l_run[qb] = 0.f;
     }
-    const f32x2_t c2 = {a.c, a.c};
 
     // prologue: the Q loads above are older than the DMAs, so "all but the newest tile" covers them and tile 0
     load_tile(0, 0);
@@ -850,39 +851,22 @@ __global__ __launch_bounds__(256, 2) void pgn_attn_w64r_kernel(AttnArgs a) {
             f32x2_t lsum2[2];
             auto probabilities = [&]() __attribute__((always_inline)) {
                 const float mc = m_run[qb] * a.c;
-                if constexpr (PACKED) {
-                    const f32x2_t nmc2 = {-mc, -mc};
+                // PLAIN fp32 instructions on purpose: on gfx950 v_fma_f32 / v_add_f32 / v_cvt_pk issue underneath a
+                // running MFMA at no cost, while the packed forms (v_pk_fma_f32, v_pk_add_f32) hold the matrix
+                // pipe for 4.6-6.5 cycles each (scripts/ubench_overlap.hip).  This file is compiled with
+                // -fno-slp-vectorize so that the scalar statements below stay scalar.
+                const float nmc = -mc;
+                float ls[4];
 #pragma unroll
-                    for (int kb = 0; kb < 2; ++kb)
+                for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-                        for (int r = 0; r < 16; r += 2) {
-                            f32x2_t x = {sacc[qb][kb][r], sacc[qb][kb][r + 1]};
-                            x = __builtin_elementwise_fma(x, c2, nmc2);
-                            f32x2_t p = {__builtin_amdgcn_exp2f(x[0]), __builtin_amdgcn_exp2f(x[1])};
-                            if (kb == 0 && r < 4) lsum2[r >> 1] = p;     // two chains, no zero-initialised adds
-                            else lsum2[(r >> 1) & 1] += p;
-                            pf[qb][kb][r >> 3][r & 7] = Cvt<DT>::from_f32(p[0]);
-                            pf[qb][kb][r >> 3][(r & 7) + 1] = Cvt<DT>::from_f32(p[1]);
-                        }
-                    lsum2[0] += lsum2[1];
-                } else {
-                    // PLAIN fp32 instructions on purpose: on gfx950 v_fma_f32 / v_add_f32 / v_cvt_pk issue underneath a
-                    // running MFMA at no cost, while the packed forms (v_pk_fma_f32, v_pk_add_f32) hold the matrix
-                    // pipe for 4.6-6.5 cycles each (scripts/ubench_overlap.hip).  This file is compiled with
-                    // -fno-slp-vectorize so that the scalar statements below stay scalar.
-                    const float nmc = -mc;
-                    float ls[4];
-#pragma unroll
-                    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[qb][kb][r], a.c, nmc));
-                            if (kb == 0 && r < 4) ls[r] = p;             // four chains
-                            else ls[r & 3] += p;
-                            pf[qb][kb][r >> 3][r & 7] = Cvt<DT>::from_f32(p);
-                        }
-                    lsum2[0] = f32x2_t{ls[0] + ls[2], ls[1] + ls[3]};
-                }
+                    for (int r = 0; r < 16; ++r) {
+                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[qb][kb][r], a.c, nmc));
+                        if (kb == 0 && r < 4) ls[r] = p;             // four chains
+                        else ls[r & 3] += p;
+                        pf[qb][kb][r >> 3][r & 7] = Cvt<DT>::from_f32(p);
+                    }
+                lsum2[0] = f32x2_t{ls[0] + ls[2], ls[1] + ls[3]};
             };
             if constexpr (SUMCHK) {
                 // No row maximum on the common path: the probabilities are taken against the current reference and
@@ -1403,7 +1387,7 @@ __global__ __launch_bounds__(256, 2) void pgn_attn_x16_kernel(AttnArgs a) {
 #endif  // PGN_TUNING_HOOKS (pgn_attn_x16_kernel)
 
 #ifdef PGN_TUNING_HOOKS
-int g_attn_variant = 0;  // 20 = the ring kernel on 16x16x32 MFMAs, 0 = shipped heuristic, 1 = 4 waves x 32 rows, 3 = 4 waves x 64 rows (two LDS-DMA buffers), 6 = 64 rows with the three-buffer ring and a row maximum per tile, 7 = the shipped ring kernel forced, 8 / 9 / 10 = its earlier forms (packed fp32 softmax arithmetic; plain arithmetic in the old order; the same without the first-tile branch), 16 = 8 waves x 32 rows
+int g_attn_variant = 0;  // 20 = the ring kernel on 16x16x32 MFMAs, 0 = shipped heuristic, 1 = 4 waves x 32 rows, 3 = 4 waves x 64 rows (two LDS-DMA buffers), 6 = 64 rows with the three-buffer ring and a row maximum per tile, 7 = the shipped ring kernel forced, 9 / 10 = its earlier forms (the old order; the same without the first-tile branch), 16 = 8 waves x 32 rows
 #else
 constexpr int g_attn_variant = 0;
 #endif
@@ -1473,7 +1457,7 @@ extern "C" int pgn_attention_fwd(const void* q, const void* k, const void* v, vo
     bool w64 = att_takes_ring_kernel(B, H, Nq, Nk, D, key_bias != nullptr);
     if (g_attn_variant == 16 && D == 64) nw = 8;
     if (g_attn_variant == 1 || nw == 8) w64 = false;
-    if (g_attn_variant == 3 || (g_attn_variant >= 6 && g_attn_variant <= 10) || g_attn_variant == 20)
+    if (g_attn_variant == 3 || (g_attn_variant >= 6 && g_attn_variant <= 10 && g_attn_variant != 8) || g_attn_variant == 20)
         w64 = D == 64 && key_bias == nullptr;
 #ifdef PGN_TUNING_HOOKS
     const bool x16 = g_attn_variant == 20;   // the ring kernel on 16x16x32 MFMAs (pgn_attn_x16_kernel)
@@ -1508,10 +1492,9 @@ extern "C" int pgn_attention_fwd(const void* q, const void* k, const void* v, vo
     else if (w64) hipLaunchKernelGGL((pgn_attn_w64_kernel<DT>), grid, block, 0, s, a);
 #define PGN_ATT_LAUNCH_RING_MAX(DT) /* the earlier forms take full key tiles only */ \
     if (!ragged && x16) hipLaunchKernelGGL((pgn_attn_x16_kernel<DT, false>), grid, block, 0, s, a); else \
-    if (!ragged && !sumchk) hipLaunchKernelGGL((pgn_attn_w64r_kernel<DT, false, true, 0>), grid, block, 0, s, a); else \
-    if (!ragged && g_attn_variant == 8) hipLaunchKernelGGL((pgn_attn_w64r_kernel<DT, true, true, 0>), grid, block, 0, s, a); else \
-    if (!ragged && g_attn_variant == 9) hipLaunchKernelGGL((pgn_attn_w64r_kernel<DT, true, false, 0>), grid, block, 0, s, a); else \
-    if (!ragged && g_attn_variant == 10) hipLaunchKernelGGL((pgn_attn_w64r_kernel<DT, true, false, 1>), grid, block, 0, s, a); else
+    if (!ragged && !sumchk) hipLaunchKernelGGL((pgn_attn_w64r_kernel<DT, false, 0>), grid, block, 0, s, a); else \
+    if (!ragged && g_attn_variant == 9) hipLaunchKernelGGL((pgn_attn_w64r_kernel<DT, true, 0>), grid, block, 0, s, a); else \
+    if (!ragged && g_attn_variant == 10) hipLaunchKernelGGL((pgn_attn_w64r_kernel<DT, true, 1>), grid, block, 0, s, a); else
 #else
 #define PGN_ATT_LAUNCH_8W(DT, BIAS)
 #define PGN_ATT_LAUNCH_RING_MAX(DT)
@@ -1521,8 +1504,8 @@ extern "C" int pgn_attention_fwd(const void* q, const void* k, const void* v, vo
     do {                                                                                                          \
         if (ring) {                                                                                               \
             PGN_ATT_LAUNCH_RING_MAX(DT)                                                                           \
-            if (ragged) hipLaunchKernelGGL((pgn_attn_w64r_kernel<DT, true, false, 2, true>), grid, block, 0, s, a); \
-            else hipLaunchKernelGGL((pgn_attn_w64r_kernel<DT, true, false, 2>), grid, block, 0, s, a);            \
+            if (ragged) hipLaunchKernelGGL((pgn_attn_w64r_kernel<DT, true, 2, true>), grid, block, 0, s, a); \
+            else hipLaunchKernelGGL((pgn_attn_w64r_kernel<DT, true, 2>), grid, block, 0, s, a);            \
         }                                                                                                         \
         PGN_ATT_LAUNCH_W64_2BUF(DT)                                                                               \
         else if (D == 64) {                                                                                       \

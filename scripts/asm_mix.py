@@ -3,7 +3,7 @@
 import re, subprocess, sys
 from collections import Counter
 src, pat = sys.argv[1], sys.argv[2]
-subprocess.run(["/opt/rocm/bin/hipcc", "-O3", "-std=c++17", "--offload-arch=gfx950", "-S", "--cuda-device-only", "-o", "/tmp/_mix.s", src] + sys.argv[3:], check=True, stderr=subprocess.DEVNULL)
+subprocess.run(["/opt/rocm/bin/hipcc", "-O3", "-std=c++17", "--offload-arch=gfx950", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-S", "--cuda-device-only", "-o", "/tmp/_mix.s", src] + sys.argv[3:], check=True, stderr=subprocess.DEVNULL)
 s = open("/tmp/_mix.s").read()
 m = re.search(r"^(\S*" + pat + r"\S*):", s, re.M)
 start = m.start(); end = s.index(".Lfunc_end", start)
