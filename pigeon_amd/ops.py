@@ -914,6 +914,8 @@ def cached_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
         out = torch.empty(T, Hq, D, dtype=q.dtype, device=dev)
     elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
         raise ValueError("cached_attention: out must match q, with a contiguous last dim")
+    elif (T > 1 and out.stride(0) == 0) or (Hq > 1 and out.stride(1) == 0):
+        raise ValueError("cached_attention: the rows of out are one (an expanded tensor)")
     if T == 0 or R == 0:
         return out
     _some(N, H, W)

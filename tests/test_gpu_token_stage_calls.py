@@ -160,3 +160,18 @@ def test_sizes_that_would_be_cut_to_32_bits_are_refused():
     for page_size in (2 ** 32 + 16, -2 ** 32 + 64, 2 ** 31, 0, -16):
         with pytest.raises(NotImplementedError):
             ops.page_advance(i32(2), i32(2), table, i32(4), i32(1), page_size, 2)
+
+
+def test_an_output_whose_rows_are_one_is_refused():
+    cache, table, lens, g = _attention_inputs(3, 1, 64)
+    q = torch.randn(3, 2, 64, generator=g).to(torch.bfloat16).to(DEV)
+    for out in (q[:1].clone().expand(3, 2, 64), q[:, :1].clone().expand(3, 2, 64)):
+        with pytest.raises(ValueError, match="out"):
+            ops.cached_attention(q, *cache, table, lens, out=out)
+    one = q[:1, :1].clone()                                         # an axis of length 1 may have any stride
+    got = ops.cached_attention(q[:1, :1], *cache, table[:1], lens[:1], out=one.as_strided((1, 1, 64), (0, 0, 1)))
+    assert torch.equal(got, ops.cached_attention(q[:1, :1].contiguous(), *cache, table[:1], lens[:1]))
+    turned = torch.empty(2, 3, 64, dtype=q.dtype, device=DEV).transpose(0, 1)                   # heads before tokens
+    assert torch.equal(ops.cached_attention(q, *cache, table, lens, out=turned), ops.cached_attention(q, *cache, table, lens))
+    same = q.clone()                                                # in place of the queries
+    assert torch.equal(ops.cached_attention(same, *cache, table, lens, out=same), ops.cached_attention(q, *cache, table, lens))
