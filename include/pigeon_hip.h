@@ -27,7 +27,7 @@
 extern "C" {
 #endif
 
-#define PGN_VERSION 112 /* 0.1.3: + pgn_bias_residual_add_stats, pgn_groupnorm_silu_nhwc_pre (GroupNorm statistics emitted by the launch that produces the tensor); 0.1.2: the channels-last GroupNorm entries take their choice of form as bits of `act` (the library reads no environment); 0.1.1: + pgn_token_embed, pgn_attention_causal_fwd, pgn_groupnorm_silu_nhwc_static */
+#define PGN_VERSION 112 /* the token stage's entry points came without a new number: a caller asks for the symbols; 0.1.3: + pgn_bias_residual_add_stats, pgn_groupnorm_silu_nhwc_pre (GroupNorm statistics emitted by the launch that produces the tensor); 0.1.2: the channels-last GroupNorm entries take their choice of form as bits of `act` (the library reads no environment); 0.1.1: + pgn_token_embed, pgn_attention_causal_fwd, pgn_groupnorm_silu_nhwc_static */
 
 #define PGN_OK 0
 #define PGN_ERR_INVALID (-1)     /* null pointer, non-positive size, bad enum, misalignment */
@@ -439,8 +439,9 @@ int pgn_cache_write(const void* k, const void* v, int dtype, const int64_t* slot
  * of its request (window must be 0).  A row that sees no key is zero.  Rows of no request (behind starts[R]) are left as
  * they were.  Table entries that name no page hide their keys.  Keys that a row does not see do not reach it, whatever
  * their bytes hold.  The same call gives the same bits; where a request's keys are split goes by the lengths of all, so
- * its last bits may differ in other company.  Sums are fp32 and divided at the end: values beyond 2^127 / (256 keys) may overflow.  W * P is at
- * most PGN_CACHED_MAX_KEYS.  workspace: pgn_cached_attention_workspace_bytes bytes, 16-byte aligned, contents irrelevant. */
+ * its last bits may differ in other company.  Probabilities are rounded to the 16-bit type for their product with the
+ * values.  Sums are fp32 and divided at the end: values beyond 2^127 / (256 keys) may overflow.  W * P is at most
+ * PGN_CACHED_MAX_KEYS.  workspace: pgn_cached_attention_workspace_bytes bytes, 16-byte aligned, contents irrelevant. */
 #define PGN_CACHED_MAX_KEYS 268435456
 size_t pgn_cached_attention_workspace_bytes(int num_tokens, int R, int packed, int Hq, int Hkv, int head_dim, int W,
                                             int page_size);
@@ -459,7 +460,8 @@ int pgn_cached_attention(const void* q, int dtype, const void* k_pages, const vo
  *     or NaN, it keeps no others
  *   the id drawn is the first, in index order, whose running sum of kept weights exceeds u times their sum
  * temperature <= 0 or NaN takes the first id in rank; a row without any logit above -inf gives -1.  Weights are computed
- * in 64 bits and summed as integers of 2^-45: the same ids every time. */
+ * in 64 bits and rounded to multiples of 2^-45, which min_p compares and the sums add up: the same ids every time.  An id
+ * whose weight is under 2^-46 of the largest has none and is not drawn, at u = 0 neither. */
 #define PGN_SAMPLE_MAX_IDS 262144
 int pgn_sample_tokens(const void* logits, int dtype, int64_t stride, int B, int V, const float* u,
                       const float* temperature, float temperature_all, const int32_t* top_k, int top_k_all,

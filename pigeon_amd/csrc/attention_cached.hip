@@ -540,7 +540,7 @@ __global__ __launch_bounds__(PGN_CA_THREADS) void pgn_cached_rows16_kernel(const
 
 // The kernel for prompts: 128 rows of a request, 32 to a wave, 64 keys at a time.
 //
-// What bounds it is arithmetic: the matrix units are busy for 35 % of the time and the vector units for 50 %, mostly with
+// What bounds it is arithmetic: the matrix units are busy for 35 % of the time and the vector units for 49 %, mostly with
 // the softmax (scaling, exp2, sum and rounding of 32 numbers a lane against 32 matrix instructions at head dim 128) and
 // the widening of bytes, which is done ONCE per workgroup, on the way into LDS, not in every wave.  4 prompts of 2048
 // tokens, 32 heads by 128: 520 to 535 us, 820 to 844 TFLOP/s (a library product of 16384^3 reaches 1346); in fp16 562.

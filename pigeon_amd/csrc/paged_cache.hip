@@ -16,16 +16,16 @@ namespace {
 // ------------------------------------------------------------------------------------------------ page_advance
 // One workgroup does the bookkeeping: it is a chain of three prefix sums over the requests (pages given back, tokens
 // added, pages wanted) whose results every later step needs, 4 bytes a request.  The pages themselves are then moved
-// flat, one thread a page: a thread finds its request by bisection in the prefix sums, which lie in LDS.
+// flat, four a thread at a time: a thread finds their requests by bisection in the prefix sums, which lie in LDS.
 // A chain of short steps is bound by their latency, and a barrier of 16 waves is the longest of them, so a call takes no
-// more waves than it has work for (us, back to back on the GPU, with 64, 256, 512 and 1024 threads):
-//   64 requests and slots  4.8  5.6  6.4  7.8        512 requests and slots       27  11   6.8  8.2
-//   64 and 512             8.9  6.4  6.4  7.9        512 and 4096                 63  21  12.5 10.9
-//   256 and 256            14   5.8  6.5  8.0        512 and 16384, two launches  31  14  10.7 12.0
-//   64 and 2048            23   11   9.0  8.9        16 and 8192, two launches   8.8 8.4   9.0 10.3
+// more waves than it has work for (us a call in a replayed graph, pages of 16, with 64, 256, 512 and 1024 threads):
+//   64 requests and slots  4.2  4.8  5.5  6.5        512 requests and slots       21 8.5   5.7  6.8
+//   64 and 512             8.1  5.6  5.3  6.6        512 and 4096                 55  19  11.6  9.8
+//   256 and 256            12   5.1  5.4  6.7        512 and 16384, two launches  23  12  10.0 11.0
+//   64 and 2048            23   10   7.8  7.6        16 and 8192, two launches   8.4 8.1   8.1  9.2
 #define PGN_ADV_THREADS 1024
 // Up to this many slots the bookkeeping workgroup fills the slot map itself (one launch); above it a second, wide launch
-// does (512 requests, 4096 slots: 10.9 us against 10.5; 64 and 16384: 22 against 9.1).
+// does (512 requests, 4096 slots: 9.8 us against 11.0; 64 and 16384: 22 against 9.0).
 #define PGN_ADV_FUSED_SLOTS 4096
 
 __device__ __forceinline__ int64_t adv_pages(int64_t tokens, int shift) {

@@ -14,8 +14,8 @@
 // with its barriers (some 20 of 0.3 us).  256 bf16 rows of 131072 with top-p take 91 us, 14 of them for the first pass (67 MB at
 // 4.8 TB/s), 33 for the bins and 11 to 21 for the stretches; 64 rows of 48386 with a top-k of 50 19 us; one fp32 row 27 us.
 //   top-k   the k-th largest of the 1024 threads' own maxima, known after the first pass, is at most the k-th largest
-//           logit: one more pass gathers what is not below its bin, some 1.1 k ids, and the rest (k, p, min-p, draw) is
-//           done among those in LDS;
+//           logit: one more pass gathers the ids up to its bin, some 1.1 k, and the rest (k, p, min-p, draw) is done
+//           among those in LDS;
 //   top-p   a pass adds the weights to the bins (whole numbers: an fp32 addition in LDS takes seven times as long), which
 //           says in which bin the border is; the next pass gathers the ids of that bin, where the border is found by a
 //           sort, and sums what is kept by stretches of the row.  A bin with more ids than the list takes (thousands of
