@@ -175,3 +175,38 @@ def test_an_output_whose_rows_are_one_is_refused():
     assert torch.equal(ops.cached_attention(q, *cache, table, lens, out=turned), ops.cached_attention(q, *cache, table, lens))
     same = q.clone()                                                # in place of the queries
     assert torch.equal(ops.cached_attention(same, *cache, table, lens, out=same), ops.cached_attention(q, *cache, table, lens))
+
+
+# ------------------------------------------------------------------------------------------------ two at once
+def test_calls_on_two_streams_at_once_keep_apart():
+    """Split attention, top-p sampling and the bookkeeping of two batches side by side: each call has its own workspace."""
+    g = torch.Generator().manual_seed(5)
+    P, D, H, W = 64, 128, 2, 150
+    batches = []
+    for R in (1, 3):
+        N = R * W + 4
+        cache = [torch.randn(N, H, P, D, generator=g).to(torch.float8_e4m3fn).to(DEV), torch.randn(N, H, D, P, generator=g).to(torch.float8_e4m3fn).to(DEV),
+                 torch.ones(N, H, device=DEV), torch.ones(N, H, device=DEV)]
+        table = torch.randperm(N, generator=g)[:R * W].view(R, W).to(torch.int32).to(DEV)
+        lens = torch.randint(5000, W * P - 1, (R,), generator=g, dtype=torch.int32).to(DEV)
+        q = torch.randn(R, 4 * H, D, generator=g).to(torch.bfloat16).to(DEV)
+        logits, u = torch.randn(R, 60000, generator=g).to(DEV) * 2, torch.rand(R, generator=g).to(DEV)
+        batches.append((cache, table, lens, q, logits, u, torch.arange(N, dtype=torch.int32, device=DEV)))
+
+    def step(b):
+        cache, table, lens, q, logits, u, pool = b
+        held, t, free, count = lens.clone(), table.clone(), pool.clone(), torch.full((1,), 4, dtype=torch.int32, device=DEV)
+        plan = ops.page_advance(held, torch.ones_like(held), t, free, count, P, len(held))
+        return ops.cached_attention(q, *cache, table, lens), ops.sample_tokens(logits, u, top_p=0.95), plan["slots"], held, t
+    want = [step(b) for b in batches]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(step(batches[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for out in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(out, want[i]))
